@@ -33,6 +33,10 @@ pub const MITOK_PRODUCTION: c_int = 1;
 /// "the network's own rate"
 pub const MITOK_ALL_LAYERS: u32 = 0xFFFF_FFFF;
 pub const MITOK_NETWORK_RATE: u32 = 0xFFFF_FFFF;
+pub const MITOK_NO_PARENT: u32 = 0xFFFF_FFFF;
+pub const MITOK_NO_TOKEN: u32 = 0xFFFF_FFFF;
+pub const MITOK_NO_ROW: u32 = 0xFFFF_FFFF;
+pub const MITOK_TREE_MAX_NODES: u32 = 256;
 
 pub const MITOK_TIME_VOCAB: c_int = 1;
 pub const MITOK_TIME_LAYER_GEMM: c_int = 2;
@@ -118,6 +122,43 @@ extern "C" {
     // rows * vocab <= 1048576 and rows <= 4096; overlapping calls on one GPU race.
     pub fn mitok_greedy_decoding_noalloc(net: *mut MitokNetwork, logits: *const c_double, rows: u32, vocab: u32,
                                          out_ids: *mut u32) -> c_int;
+    // operators of a serving loop: no counterpart in the reference
+    pub fn mitok_tree_attention_device(
+        net: *mut MitokNetwork, d_q: *const c_double, d_k_cache: *const c_double, d_v_cache: *const c_double,
+        d_bias: *const c_double, bias_stride: u64, kv_lens: *const u32, parents: *const u32, counts: *const u32,
+        batch: u32, nodes: u32, heads: u32, head_dim: u32, max_ctx: u32, weigh_nodes: u32,
+        d_weights: *mut c_double, d_out: *mut c_double
+    ) -> c_int;
+    pub fn mitok_tree_step(
+        net: *mut MitokNetwork, ids: *const u32, parents: *const u32, counts: *const u32, batch: u32, nodes: u32,
+        weigh_nodes: u32, out_ids: *mut u32, out_logits: *mut c_double
+    ) -> c_int;
+    pub fn mitok_tree_step_device(
+        net: *mut MitokNetwork, ids: *const u32, parents: *const u32, counts: *const u32, batch: u32, nodes: u32,
+        weigh_nodes: u32, d_logits: *mut c_double
+    ) -> c_int;
+    pub fn mitok_tree_accept(
+        net: *mut MitokNetwork, path: *const u32, path_lens: *const u32, batch: u32, max_path: u32
+    ) -> c_int;
+    pub fn mitok_evict_rows_device(
+        net: *mut MitokNetwork, d_k_cache: *const c_double, d_v_cache: *const c_double,
+        d_weights: *const c_double, kv_lens: *const u32, batch: u32, heads: u32, head_dim: u32, max_ctx: u32,
+        keep: u32, sinks: u32, recent: u32, d_k_out: *mut c_double, d_v_out: *mut c_double,
+        d_weights_out: *mut c_double, out_ctx: u32, d_kept: *mut u32, out_lens: *mut u32
+    ) -> c_int;
+    pub fn mitok_evict_rows(
+        net: *mut MitokNetwork, batch: u32, keep: u32, sinks: u32, recent: u32, out_lens: *mut u32
+    ) -> c_int;
+    pub fn mitok_process_logits_device(
+        net: *mut MitokNetwork, d_logits: *const c_double, rows: u32, vocab: u32, d_history: *const u32,
+        max_history: u32, d_penalties: *const c_double, d_bias_ids: *const u32, d_bias: *const c_double,
+        max_bias: u32, d_allowed: *const u32, d_out: *mut c_double, d_out_ids: *mut u32
+    ) -> c_int;
+    pub fn mitok_process_logits(
+        net: *mut MitokNetwork, logits: *const c_double, rows: u32, vocab: u32, history: *const u32,
+        max_history: u32, penalties: *const c_double, bias_ids: *const u32, bias: *const c_double, max_bias: u32,
+        allowed: *const u32, out: *mut c_double, out_ids: *mut u32
+    ) -> c_int;
 
     // measurement and scheduling (no counterpart in the reference)
     pub fn mitok_last_timings(net: *mut MitokNetwork, t3: *mut c_double) -> c_int;

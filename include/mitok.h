@@ -50,6 +50,13 @@ extern "C" {
 #define MITOK_ALL_LAYERS 0xFFFFFFFFu
 #define MITOK_NETWORK_RATE 0xFFFFFFFFu
 
+/* operators of a serving loop: a drafted token without a parent among the
+ * drafted ones; no token (an unused entry, or no answer); no cached row */
+#define MITOK_NO_PARENT 0xFFFFFFFFu
+#define MITOK_NO_TOKEN 0xFFFFFFFFu
+#define MITOK_NO_ROW 0xFFFFFFFFu
+#define MITOK_TREE_MAX_NODES 256
+
 /* kernel classes for mitok_timing_enable */
 #define MITOK_TIME_VOCAB 1       /* the vocab Linear (the Linear before Softmax) */
 #define MITOK_TIME_LAYER_GEMM 2  /* Q/K/V and FFN projections of one-row (decode) calls */
@@ -295,6 +302,112 @@ int mitok_greedy_decoding_device(mitok_network* net, const double* d_logits, uin
  * threads) race; calls through one network are serialised by its stream. */
 int mitok_greedy_decoding_noalloc(mitok_network* net, const double* logits, uint32_t rows, uint32_t vocab,
                                   uint32_t* out_ids);
+
+/* ---- operators of a serving loop (no reference counterpart) ----
+ * Drafted tokens checked several at a time, rows evicted from the cache by the
+ * attention they received, and rules that turn logits into a token.  The
+ * *_device entry points work on device arrays of the network's GPU (checked:
+ * in one allocation, aligned to 16 bytes for complex arrays and to their
+ * elements otherwise; outputs overlap nothing but where in place is allowed).
+ * They run on the network's stream, behind everything queued on the device's
+ * default stream before the call (work on other streams has to be finished),
+ * and are complete on return; so they cannot be captured into a graph.
+ * Lengths, parents and paths are host arrays. */
+
+/* Attention of a tree of drafted tokens over a KV cache.  Sequence b has
+ * kv_lens[b] committed rows and counts[b] <= nodes drafted ones (counts NULL:
+ * nodes of each; at most MITOK_TREE_MAX_NODES), whose keys and values already
+ * lie behind them: node i in slot kv_lens[b] + i.  parents[b][i] < i, or
+ * MITOK_NO_PARENT.  Node i attends over the committed rows, its ancestors and
+ * itself:
+ *   score(i, t) = Re(sum_e q_i[e] k_t[e]) / (1e-8 + sqrt(head_dim)) + bias[h][column(t)]
+ *   column(t) = t for a committed row, kv_lens[b] + depth for a drafted one
+ *   out_i = sum_t softmax(score(i, .))_t v_t
+ * (scale_attention_scores and bias row 0, masked_attention_head.rs:184-208,
+ * 453-465), so a chain of nodes gives what decode steps one by one give.  A
+ * row that a node does not see has no part in its output, finite or not; rows
+ * past counts[b] are zero.
+ *   d_q, d_out [batch][nodes][heads * head_dim] complex
+ *   d_k_cache, d_v_cache [batch][heads][max_ctx][head_dim] complex, head_dim <= 256
+ *   d_bias [heads] rows of real numbers, bias_stride apart, or NULL
+ *   d_weights [batch][heads][max_ctx] or NULL: the softmax weights that the
+ *     first weigh_nodes nodes give each slot are summed; committed slots are
+ *     added to, the drafted ones set. */
+int mitok_tree_attention_device(mitok_network* net, const double* d_q, const double* d_k_cache,
+                                const double* d_v_cache, const double* d_bias, uint64_t bias_stride,
+                                const uint32_t* kv_lens, const uint32_t* parents, const uint32_t* counts,
+                                uint32_t batch, uint32_t nodes, uint32_t heads, uint32_t head_dim, uint32_t max_ctx,
+                                uint32_t weigh_nodes, double* d_weights, double* d_out);
+/* A tree of drafted tokens through the whole stack, on the caches that
+ * mitok_prefill (or a forward_only mitok_predict) left: ids, parents
+ * [batch][nodes], counts as above.  A node's output is what decode steps along
+ * its path would give (RoPE position and bias column by its depth).
+ * out_ids [batch][nodes] or NULL: the greedy id after each node (MITOK_NO_TOKEN
+ * past counts[b]); out_logits [batch][nodes][vocab] or NULL: its Re-logits.
+ * weigh_nodes > 0: the attention that the first weigh_nodes nodes pay is kept
+ * per layer, head and cached row, for mitok_evict_rows (1: the root, a token
+ * already decided).  The caches' committed rows stay as they are: mitok_tree_accept
+ * commits nodes, any other call on the caches drops them.  Every sequence
+ * needs room for `nodes` rows.  On an error of the pass the caches are dropped. */
+int mitok_tree_step(mitok_network* net, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts,
+                    uint32_t batch, uint32_t nodes, uint32_t weigh_nodes, uint32_t* out_ids, double* out_logits);
+/* mitok_tree_step with the logits [batch][nodes][vocab] left in device memory,
+ * where mitok_process_logits_device reads them (rows past counts[b] have no
+ * meaning). */
+int mitok_tree_step_device(mitok_network* net, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts,
+                           uint32_t batch, uint32_t nodes, uint32_t weigh_nodes, double* d_logits);
+/* Commits the nodes path[b][0 .. path_lens[b]) of the last mitok_tree_step, a
+ * chain from a node without a parent downwards (path [batch][max_path]; 0
+ * nodes: none): their rows become the cache's next ones.  A following
+ * mitok_decode_step(NULL) feeds the greedy id after the last of them. */
+int mitok_tree_accept(mitok_network* net, const uint32_t* path, const uint32_t* path_lens, uint32_t batch,
+                      uint32_t max_path);
+
+/* Eviction from a cache by accumulated attention weight.  A sequence of more
+ * than `keep` rows keeps, in every head, its first `sinks`, its last `recent`
+ * (sinks + recent <= keep) and of the others those of largest weight (equal
+ * weights, and NaN, which counts as less than any number: the lowest slot
+ * first); others keep all.  The kept rows of keys, values and weights go, in
+ * order, to slots 0, 1, ... of the output arrays [batch][heads][out_ctx]...;
+ * slots behind them stay as they were.  In place: d_k_out == d_k_cache,
+ * d_v_out == d_v_cache, d_weights_out == d_weights and out_ctx == max_ctx.
+ * d_kept [batch][heads][keep] or NULL: the slots kept, then MITOK_NO_ROW.
+ * out_lens (host) [batch]: rows kept. */
+int mitok_evict_rows_device(mitok_network* net, const double* d_k_cache, const double* d_v_cache,
+                            const double* d_weights, const uint32_t* kv_lens, uint32_t batch, uint32_t heads,
+                            uint32_t head_dim, uint32_t max_ctx, uint32_t keep, uint32_t sinks, uint32_t recent,
+                            double* d_k_out, double* d_v_out, double* d_weights_out, uint32_t out_ctx,
+                            uint32_t* d_kept, uint32_t* out_lens);
+/* The same in place on every attention layer's cache, by the weights that
+ * mitok_tree_step(weigh_nodes > 0) kept since the prompt (rows that other
+ * calls appended weigh 0; MITOK_ERR_STATE if no step weighed).  Later tokens
+ * keep their RoPE positions; a bias column goes by the row's place in the
+ * cache.  out_lens [batch] or NULL: rows left.  Drops an uncommitted tree. */
+int mitok_evict_rows(mitok_network* net, uint32_t batch, uint32_t keep, uint32_t sinks, uint32_t recent,
+                     uint32_t* out_lens);
+
+/* Rules on rows of logits, then the greedy id.  For token t of row r, seen
+ * c > 0 times in the row's history: x = x > 0 ? x / repetition : x * repetition,
+ * then x -= frequency * c + presence; then x += its bias; a token whose bit
+ * is 0 in `allowed` becomes -inf (whatever it was).
+ *   d_history [rows][max_history], d_penalties [rows][3] (repetition > 0,
+ *     presence, frequency); max_history 0: neither is read
+ *   d_bias_ids, d_bias [rows][max_bias]: of equal ids the last entry counts
+ *   d_allowed [rows][(vocab + 31) / 32] bits (t at bit t % 32 of word t / 32) or NULL
+ * MITOK_NO_TOKEN entries of the history and the ids are skipped; another id
+ * >= vocab is MITOK_ERR_ARG.  d_out [rows][vocab] or NULL: the logits after
+ * the rules (d_logits itself: in place).  d_out_ids [rows] or NULL: the last
+ * index of the largest one, MITOK_NO_TOKEN if none is above -inf.  A NaN that
+ * is allowed is MITOK_ERR_NAN, as in greedy_decoding (sampling_methods.rs:5-18). */
+int mitok_process_logits_device(mitok_network* net, const double* d_logits, uint32_t rows, uint32_t vocab,
+                                const uint32_t* d_history, uint32_t max_history, const double* d_penalties,
+                                const uint32_t* d_bias_ids, const double* d_bias, uint32_t max_bias,
+                                const uint32_t* d_allowed, double* d_out, uint32_t* d_out_ids);
+/* The same on host arrays. */
+int mitok_process_logits(mitok_network* net, const double* logits, uint32_t rows, uint32_t vocab,
+                         const uint32_t* history, uint32_t max_history, const double* penalties,
+                         const uint32_t* bias_ids, const double* bias, uint32_t max_bias, const uint32_t* allowed,
+                         double* out, uint32_t* out_ids);
 
 /* ---- measurement (no reference counterpart: the reference prints wall
  * clock only, transformer_network.rs:307-310) ---- */

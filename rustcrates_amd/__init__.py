@@ -26,6 +26,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmitok.so")
 
 TRAINING, PRODUCTION = 0, 1
+# a drafted token without a parent, no token, no cached row; nodes of a tree at most
+NO_PARENT = NO_TOKEN = NO_ROW = 0xFFFFFFFF
+TREE_MAX_NODES = 256
 TIME_VOCAB, TIME_LAYER_GEMM, TIME_ATTENTION, TIME_STEP, TIME_PREFILL_GEMM = 1, 2, 3, 4, 5
 
 ERRORS = {1: "ERR_ARG", 2: "ERR_HIP", 3: "ERR_STATE", 4: "ERR_NAN", 5: "ERR_NOMEM"}
@@ -71,6 +74,16 @@ SIGNATURES = {
     "mitok_greedy_decoding_device": (_i32, [_P, _P, _u32, _u32, _P]),
     "mitok_forward_layers_device": (_i32, [_P, _u32, _u32, _P, _P, _u32, _u32, _P, _i32, _P]),
     "mitok_greedy_decoding_noalloc": (_i32, [_P, _P, _u32, _u32, _P]),
+    "mitok_tree_attention_device": (_i32, [_P, _P, _P, _P, _P, _u64, _P, _P, _P, _u32, _u32, _u32, _u32, _u32, _u32, _P,
+                                           _P]),
+    "mitok_tree_step": (_i32, [_P, _P, _P, _P, _u32, _u32, _u32, _P, _P]),
+    "mitok_tree_step_device": (_i32, [_P, _P, _P, _P, _u32, _u32, _u32, _P]),
+    "mitok_tree_accept": (_i32, [_P, _P, _P, _u32, _u32]),
+    "mitok_evict_rows_device": (_i32, [_P, _P, _P, _P, _P, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _P, _P, _P, _u32,
+                                       _P, _P]),
+    "mitok_evict_rows": (_i32, [_P, _u32, _u32, _u32, _u32, _P]),
+    "mitok_process_logits_device": (_i32, [_P, _P, _u32, _u32, _P, _u32, _P, _P, _P, _u32, _P, _P, _P]),
+    "mitok_process_logits": (_i32, [_P, _P, _u32, _u32, _P, _u32, _P, _P, _P, _u32, _P, _P, _P]),
     "mitok_last_timings": (_i32, [_P, _P]),
     "mitok_timing_enable": (_i32, [_P, _i32]),
     "mitok_timing_read": (_i32, [_P, _P, _P, _P, _P]),
@@ -117,7 +130,7 @@ def _ptr(a):
 
 
 def _dev(p):
-    return C.c_void_p(p.ptr if isinstance(p, DeviceBuffer) else int(p))
+    return None if p is None else C.c_void_p(p.ptr if isinstance(p, DeviceBuffer) else int(p))
 
 
 class DeviceBuffer:
@@ -174,6 +187,18 @@ def _c128(a, n=None, what="tensor"):
     if n is not None and a.size != n:
         raise ValueError(f"{what}: {a.size} elements, expected {n}")
     return a
+
+
+def _u32_rows(a, what, shape=None):
+    """A contiguous uint32 matrix (signed -1 becomes 0xFFFFFFFF)."""
+    a = np.asarray(a)
+    if a.ndim != 2 or (shape is not None and a.shape != shape):
+        raise ValueError(f"{what}: shape {a.shape}, expected {shape or '(rows, columns)'}")
+    if a.dtype != np.uint32:
+        if a.dtype.kind not in "iu" or (a.size and (a.min() < -1 or a.max() > 0xFFFFFFFF)):
+            raise ValueError(f"{what}: not 32-bit whole numbers")
+        a = (a.astype(np.int64) & 0xFFFFFFFF).astype(np.uint32)
+    return np.ascontiguousarray(a)
 
 
 def _u32_vec(a, n, what):
@@ -541,6 +566,127 @@ class Network:
         out = np.empty(rows, np.uint32)
         _check(self._lib.mitok_greedy_decoding(self._h, _ptr(logits), rows, V, _ptr(out)))
         return out
+
+    # ---- operators of a serving loop ----
+    def tree_attention_device(self, d_q, d_k_cache, d_v_cache, kv_lens, parents, heads, head_dim, max_ctx, d_out,
+                              counts=None, bias=None, bias_stride=0, weights=None, weigh_nodes=0):
+        """Attention of a tree of drafted tokens over a KV cache in device
+        memory (mitok_tree_attention_device).  parents [B][nodes]: each node's
+        parent, an earlier node of its sequence, or -1 / NO_PARENT; kv_lens [B]
+        committed rows, counts [B] nodes used (None: all).  Node i sits in slot
+        kv_lens[b] + i; d_q and d_out are [B][nodes][heads * head_dim] complex,
+        the caches [B][heads][max_ctx][head_dim]; bias: [heads] rows of f64,
+        bias_stride apart; weights [B][heads][max_ctx] f64 takes the attention
+        that the first weigh_nodes nodes pay."""
+        par = _u32_rows(parents, "parents")
+        B, nodes = par.shape
+        lens = _u32_vec(kv_lens, B, "kv_lens")
+        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        _check(self._lib.mitok_tree_attention_device(self._h, _dev(d_q), _dev(d_k_cache), _dev(d_v_cache), _dev(bias),
+                                                     int(bias_stride), _ptr(lens), _ptr(par), _ptr(cnt), B, nodes,
+                                                     heads, head_dim, max_ctx, int(weigh_nodes), _dev(weights),
+                                                     _dev(d_out)))
+
+    def tree_step(self, ids, parents, counts=None, weigh_nodes=0, want_logits=False):
+        """A tree of drafted tokens [B][nodes] through the stack, on the caches
+        (mitok_tree_step): the greedy id after each node [B][nodes] (NO_TOKEN
+        past counts[b]) and, with want_logits, its Re-logits [B][nodes][V].
+        tree_accept commits nodes."""
+        ids = _u32_rows(ids, "ids")
+        B, nodes = ids.shape
+        par = _u32_rows(parents, "parents", (B, nodes))
+        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        out = np.empty((B, nodes), np.uint32)
+        logits = np.empty((B, nodes, self.vocab), np.float64) if want_logits else None
+        _check(self._lib.mitok_tree_step(self._h, _ptr(ids), _ptr(par), _ptr(cnt), B, nodes, int(weigh_nodes),
+                                         _ptr(out), _ptr(logits)))
+        return (out, logits) if want_logits else out
+
+    def tree_step_device(self, ids, parents, d_logits, counts=None, weigh_nodes=0):
+        """tree_step with the logits [B][nodes][V] f64 left in device memory."""
+        ids = _u32_rows(ids, "ids")
+        B, nodes = ids.shape
+        par = _u32_rows(parents, "parents", (B, nodes))
+        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        _check(self._lib.mitok_tree_step_device(self._h, _ptr(ids), _ptr(par), _ptr(cnt), B, nodes, int(weigh_nodes),
+                                                _dev(d_logits)))
+
+    def tree_accept(self, path, path_lens=None):
+        """Commits nodes path[b][:path_lens[b]] of the last tree_step, from a
+        node without a parent downwards (mitok_tree_accept)."""
+        path = _u32_rows(path, "path")
+        B, most = path.shape
+        lens = np.full(B, most, np.uint32) if path_lens is None else _u32_vec(path_lens, B, "path_lens")
+        _check(self._lib.mitok_tree_accept(self._h, _ptr(path), _ptr(lens), B, most))
+
+    def evict_rows_device(self, d_k_cache, d_v_cache, d_weights, kv_lens, heads, head_dim, max_ctx, keep, sinks, recent,
+                          d_k_out, d_v_out, d_weights_out, out_ctx, kept=None):
+        """Of each sequence's kv_lens[b] cached rows `keep` stay in every head:
+        the first `sinks`, the last `recent` and those of largest weight, packed
+        into the output arrays (mitok_evict_rows_device; the same arrays: in
+        place).  kept [B][heads][keep] u32: their slots.  Returns the rows left [B]."""
+        lens = np.ascontiguousarray(kv_lens, dtype=np.uint32)
+        if lens.ndim != 1:
+            raise ValueError(f"kv_lens: shape {lens.shape}, expected (batch,)")
+        out = np.empty(lens.shape, np.uint32)
+        _check(self._lib.mitok_evict_rows_device(self._h, _dev(d_k_cache), _dev(d_v_cache), _dev(d_weights), _ptr(lens),
+                                                 len(lens), heads, head_dim, max_ctx, keep, sinks, recent,
+                                                 _dev(d_k_out), _dev(d_v_out), _dev(d_weights_out), out_ctx,
+                                                 _dev(kept), _ptr(out)))
+        return out
+
+    def evict_rows(self, batch, keep, sinks=0, recent=0):
+        """evict_rows_device in place on every layer's cache, by the attention
+        that tree_step(weigh_nodes > 0) kept (mitok_evict_rows).  Returns the
+        rows left per sequence."""
+        out = np.empty(int(batch), np.uint32)
+        _check(self._lib.mitok_evict_rows(self._h, int(batch), int(keep), int(sinks), int(recent), _ptr(out)))
+        return out
+
+    def process_logits_device(self, d_logits, rows, vocab, out=None, ids=None, history=None, max_history=0,
+                              penalties=None, bias_ids=None, bias=None, max_bias=0, allowed=None):
+        """Penalties for repeated tokens, biases and a mask of allowed tokens on
+        [rows][vocab] f64 logits in device memory, then the greedy ids
+        (mitok_process_logits_device has the layouts).  out: the logits after
+        the rules; ids [rows] u32; either may be None."""
+        _check(self._lib.mitok_process_logits_device(self._h, _dev(d_logits), rows, vocab, _dev(history),
+                                                     int(max_history), _dev(penalties), _dev(bias_ids), _dev(bias),
+                                                     int(max_bias), _dev(allowed), _dev(out), _dev(ids)))
+
+    def process_logits(self, logits, history=None, penalties=None, bias_ids=None, bias=None, allowed=None,
+                       want_logits=True):
+        """process_logits_device on host arrays: logits [rows][V]; history
+        [rows][H] token ids and penalties [rows][3] (repetition, presence,
+        frequency); bias_ids, bias [rows][b]; allowed [rows][V] truth values.
+        Entries of -1 / NO_TOKEN are skipped.  Returns (logits, ids)."""
+        x = np.ascontiguousarray(logits, dtype=np.float64)
+        if x.ndim != 2:
+            raise ValueError(f"logits: shape {x.shape}, expected (rows, vocab)")
+        R, V = x.shape
+        h = p = bi = bv = al = None
+        if history is not None:
+            h = _u32_rows(history, "history")
+            p = np.ascontiguousarray(penalties, dtype=np.float64)
+            if h.shape[0] != R or p.shape != (R, 3):
+                raise ValueError(f"history {h.shape}, penalties {p.shape}: expected ({R}, n) and ({R}, 3)")
+        if bias_ids is not None:
+            bi = _u32_rows(bias_ids, "bias_ids")
+            bv = np.ascontiguousarray(bias, dtype=np.float64)
+            if bi.shape[0] != R or bv.shape != bi.shape:
+                raise ValueError(f"bias_ids {bi.shape}, bias {bv.shape}: expected two of ({R}, n)")
+        if allowed is not None:
+            ok = np.asarray(allowed, dtype=bool)
+            if ok.shape != (R, V):
+                raise ValueError(f"allowed: shape {ok.shape}, expected ({R}, {V})")
+            bits = np.zeros((R, -(-V // 32) * 32), bool)
+            bits[:, :V] = ok
+            al = np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view("<u4")
+        out = np.empty_like(x) if want_logits else None
+        ids = np.empty(R, np.uint32)
+        _check(self._lib.mitok_process_logits(self._h, _ptr(x), R, V, _ptr(h), 0 if h is None else h.shape[1], _ptr(p),
+                                              _ptr(bi), _ptr(bv), 0 if bi is None else bi.shape[1], _ptr(al),
+                                              _ptr(out), _ptr(ids)))
+        return out, ids
 
     # ---- measurement ----
     def last_timings(self):

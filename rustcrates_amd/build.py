@@ -18,7 +18,8 @@ SRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmitok.so")
 SOURCES = ["kernels.hip", "gemm.hip", "gemm_mfma.hip", "attention.hip", "resident.hip", "resident_k1.hip", "resident_k2.hip",
-           "resident_k4.hip", "resident_k8.hip", "train.hip", "wavelet_init.hip", "network.hip"]
+           "resident_k4.hip", "resident_k8.hip", "train.hip", "wavelet_init.hip", "tree_attention.hip",
+           "serving.hip", "network.hip"]
 ARCH = os.environ.get("MITOK_ARCH", "gfx950")
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"

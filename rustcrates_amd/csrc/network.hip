@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -21,6 +22,7 @@
 #include <vector>
 
 #include "../../include/mitok.h"
+#include "serving.hpp"
 #include "train.hpp"
 
 namespace mitok {
@@ -138,6 +140,7 @@ struct SelfAttentionLayer : Layer {  // self_attention_layer.rs:16-25 + masked_a
   DevBuf bias_re;  // [heads][max_ctx][max_ctx]  Re(bias_pos): only the real part reaches the softmax
   DevBuf gamma, beta;
   DevBuf kc, vc;  // [cache_B][heads][max_ctx][dh]
+  DevBuf aw;      // [cache_B][heads][max_ctx] attention each cached row received (mitok_tree_step)
   // training state: AdamW moments of wqkv and of the Norm's gamma and beta;
   // updates so far of the heads and of the Norm, counted apart because
   // reset_previous_gradient resets the heads' previous gradient but not the
@@ -300,6 +303,7 @@ struct Spec {
   int S_first = 0, T = 0;            // sizing: rows per sequence before the call's compressions (0: none
                                      // follow; S is the most they reach) and its target rows
   int ctx_bound = 0;                 // keys a decode step of this call can reach (0: the layers' context)
+  const TreeAttn* tree = nullptr;    // a drafted tree's rows on the cache: its lengths, ancestors and workspace
 };
 
 struct Timing {
@@ -385,6 +389,24 @@ struct mitok_network {
   // length minus its cached rows (positions count the uncompressed prompt)
   mitok::DevBuf pos_off_d;
   bool pos_off = false;
+  std::vector<int> pos_off_h;  // the same on the host, while pos_off
+  // the last mitok_tree_step's nodes behind the committed rows, until another
+  // call uses the cache: nodes per sequence, their parents and counts
+  bool tree_valid = false;
+  uint32_t tree_n = 0;
+  std::vector<uint32_t> tree_parents, tree_counts;
+  bool tree_weighed = false;        // that step weighed attention
+  mitok::DevBuf tree_ids, tree_rng;  // its greedy ids [B][n]; rows whose weights it started at zero
+  // cached rows whose weights in the layers' aw are kept, per sequence; empty:
+  // no step has weighed attention since the prompt
+  std::vector<uint32_t> aw_len;
+  // operators of a serving loop (serving.hpp): host staging and its device
+  // copy, scratch, and the words their kernels set on an error
+  char* op_host = nullptr;
+  size_t op_host_bytes = 0;
+  mitok::DevBuf op_tab, op_ws;
+  uint32_t* op_err = nullptr;
+  hipEvent_t op_event = nullptr;
   // the last stateless pass's vocab Linear input rows [head_B * head_S][d]
   // (in act0/act1) and its softmax output (probs), which mitok_backward_head
   // differentiates; any later call clears head_valid
@@ -639,6 +661,7 @@ static int compressed_rows(const WaveletLayer* W, int S, int T) {
 
 static int prepare(Net* n, const Spec& sp) {
   n->head_valid = false;  // the workspaces that held the last stateless pass's head input are reused
+  n->tree_valid = false;
   const Dims dm = net_dims(n);
   const size_t rows = (size_t)sp.B * sp.S;
   const size_t c16 = sizeof(double2);
@@ -880,7 +903,26 @@ static int enqueue_forward(Net* n, const Spec& sp) {
         a.H = H;
         a.dh = dh;
         a.scale = 1.0 / (1e-8 + sqrt((double)dh));  // scale_attention_scores (masked_attention_head.rs:453-465)
-        if (sp.mode == MODE_CACHED && S == 1) {
+        if (sp.tree) {
+          TreeAttn t = *sp.tree;
+          t.q = q;
+          t.ldq = t.ldo = d;
+          t.kc = e.kc;
+          t.vc = e.vc;
+          t.ctx = A->max_ctx;
+          t.bias = a.bias_re;  // row 0 of each head's table, as a decode step
+          t.bias_stride = (long)A->max_ctx * A->max_ctx;
+          t.H = H;
+          t.dh = dh;
+          t.scale = a.scale;
+          t.weights = t.weigh ? A->aw.as<double>() : nullptr;
+          t.out = cat;
+          {
+            TimeScope ts(n, MITOK_TIME_ATTENTION, 0.0);
+            tree_attention(st, t);
+          }
+          layernorm(st, cat, cur, nxt, rows, d, A->eps, A->gamma.as<double2>(), A->beta.as<double2>());
+        } else if (sp.mode == MODE_CACHED && S == 1) {
           // key chunks, then one row transform: chunk combine + residual + Norm (self_attention_layer.rs:101-124)
           AttnSplit o = split_buffers(n, attention_split_plan(a), B, H);
           {
@@ -1799,6 +1841,12 @@ static int ensure_rope_for(Net* n, uint32_t first, uint32_t last, int positions)
   return OK;
 }
 
+// RoPE position of sequence b's next token: its cached rows, and what the cache
+// no longer holds of the tokens before
+static uint32_t next_position(const Net* n, uint32_t b) {
+  return n->kv_len_h[b] + (n->pos_off && b < n->pos_off_h.size() ? (uint32_t)n->pos_off_h[b] : 0u);
+}
+
 static int rope_positions_needed(const Net* n) {
   uint32_t m = min_ctx(n);
   return (int)std::max<uint32_t>(m == UINT32_MAX ? 512u : m, 512u);
@@ -1876,6 +1924,11 @@ int mitok_network_create(int device, mitok_network** out) {
   if (!rc && hipStreamCreateWithFlags(&n->stream, hipStreamNonBlocking) != hipSuccess)
     rc = fail(ERR_HIP, "hipStreamCreate failed");
   if (!rc) rc = noalloc_scratch(device, &n->scratch);
+  if (!rc && hipHostMalloc((void**)&n->op_err, OE_WORDS * sizeof(uint32_t), hipHostMallocCoherent) != hipSuccess)
+    rc = fail(ERR_NOMEM, "hipHostMalloc of the error words failed");
+  if (!rc) memset(n->op_err, 0, OE_WORDS * sizeof(uint32_t));
+  if (!rc && hipEventCreateWithFlags(&n->op_event, hipEventDisableTiming) != hipSuccess)
+    rc = fail(ERR_HIP, "hipEventCreate failed");
   if (!rc) rc = n->err_d.reserve(2 * sizeof(uint32_t));
   if (!rc) rc = n->sync_cnt.reserve((size_t)SYNC_COUNTERS * sizeof(uint32_t));
   if (!rc) {
@@ -1899,6 +1952,9 @@ void mitok_network_destroy(mitok_network* n) {
   collect_timing(n);
   for (hipEvent_t e : n->timing.pool) (void)hipEventDestroy(e);
   n->layers.clear();
+  if (n->op_event) (void)hipEventDestroy(n->op_event);
+  if (n->op_err) (void)hipHostFree(n->op_err);
+  if (n->op_host) (void)hipHostFree(n->op_host);
   if (n->stream) (void)hipStreamDestroy(n->stream);
   delete n;
 }
@@ -2201,6 +2257,8 @@ int mitok_reset(mitok_network* n) {
   n->cache_valid = false;
   n->cache_B = 0;
   n->kv_len_h.clear();
+  n->tree_valid = false;
+  n->aw_len.clear();
   return OK;
 }
 
@@ -2354,6 +2412,7 @@ static int begin_call(Net* n, const uint32_t* lens, uint32_t B, uint32_t S, cons
     for (uint32_t b = 0; b < B; ++b) off[b] = (int)lens[b] - (int)ln[b];
     keep_i.push_back(off);
     TRY(upload(n, n->pos_off_d, keep_i.back().data(), (size_t)B * sizeof(int)));
+    n->pos_off_h = off;
   }
   if (sp.mode == MODE_CACHED) {
     n->dec_tsum = 0.0;
@@ -2384,6 +2443,7 @@ static void end_call(Net* n, const Spec& sp, const uint32_t* lens) {
     n->cache_B = sp.B;
     const uint32_t* cl = cached_lens(n, lens);
     n->kv_len_h.assign(cl, cl + sp.B);  // the cache keeps each sequence's own rows
+    n->aw_len.clear();
   } else if (sp.mode == MODE_CACHED) {
     for (uint32_t b = 0; b < (uint32_t)sp.B; ++b) n->kv_len_h[b] += 1;
   }
@@ -2844,8 +2904,8 @@ static int decode_step_impl(Net* n, const uint32_t* ids, uint32_t B, uint32_t* o
   hipStream_t st = n->stream;
   const uint32_t V = n->layers[n->layers.size() - 2]->d_out;
   const bool want_logits = out_logits != nullptr;
-  uint32_t kv_max = 0;
-  for (uint32_t b = 0; b < B; ++b) kv_max = std::max(kv_max, n->kv_len_h[b]);
+  uint32_t kv_max = 0;  // the largest RoPE position
+  for (uint32_t b = 0; b < B; ++b) kv_max = std::max(kv_max, next_position(n, b));
   Spec dec = decode_spec(n, B);
   TRY(prepare(n, dec));
   TRY(reserve(n, n->hist_d, (size_t)B * sizeof(uint32_t)));
@@ -3541,6 +3601,690 @@ int mitok_greedy_decoding_noalloc(mitok_network* n, const double* logits, uint32
   HIP_TRY(hipMemcpyAsync(out_ids, ids, rows * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
   HIP_TRY(hipStreamSynchronize(n->stream));
   return check_err_word(n);
+}
+
+// ===========================================================================
+// operators of a serving loop (serving.hpp)
+// ===========================================================================
+// a x b x ..., or SIZE_MAX where that passes 64 bits
+static size_t times(std::initializer_list<size_t> f) {
+  size_t p = 1;
+  for (size_t x : f)
+    if (__builtin_mul_overflow(p, x, &p)) return SIZE_MAX;
+  return p;
+}
+
+// A caller's device array: in range (check_device_range) and aligned to its elements.
+static int check_device_array(const Net* n, const void* p, size_t bytes, size_t align, const char* what) {
+  if (bytes == SIZE_MAX) return fail(ERR_ARG, "%s: its size passes 64 bits", what);
+  if ((uintptr_t)p % align) return fail(ERR_ARG, "%s is not aligned to %zu bytes", what, align);
+  return check_device_range(n, p, bytes, what);
+}
+
+struct Span {
+  const void* p;
+  size_t bytes;
+  const char* what;
+};
+static bool overlap(const Span& a, const Span& b) {
+  return a.p && b.p && (const char*)a.p < (const char*)b.p + b.bytes && (const char*)b.p < (const char*)a.p + a.bytes;
+}
+static int check_apart(const Span& out, std::initializer_list<Span> others) {
+  for (const Span& o : others)
+    if (overlap(out, o)) return fail(ERR_ARG, "%s and %s overlap", out.what, o.what);
+  return OK;
+}
+
+// The network's stream goes on behind what the caller has queued on the
+// device's default stream, where frameworks fill their tensors; an idle default
+// stream costs one query.
+static int behind_default_stream(Net* n) {
+  const hipError_t q = hipStreamQuery(nullptr);
+  if (q == hipSuccess) return OK;
+  (void)hipGetLastError();
+  if (q != hipErrorNotReady) return fail(ERR_HIP, "the default stream: %s", hipGetErrorString(q));
+  HIP_TRY(hipEventRecord(n->op_event, nullptr));
+  HIP_TRY(hipStreamWaitEvent(n->stream, n->op_event, 0));
+  return OK;
+}
+
+// `bytes` of pinned staging (valid until the next call of this) and as many on the device
+static int op_staging(Net* n, size_t bytes) {
+  if (bytes > n->op_host_bytes) {
+    if (n->op_host) (void)hipHostFree(n->op_host);
+    n->op_host = nullptr;
+    n->op_host_bytes = 0;
+    const size_t want = std::max<size_t>(2 * bytes, 16384);
+    if (hipHostMalloc((void**)&n->op_host, want, hipHostMallocDefault) != hipSuccess) {
+      (void)hipGetLastError();
+      n->op_host = nullptr;
+      return fail(ERR_NOMEM, "hipHostMalloc of %zu bytes failed", want);
+    }
+    n->op_host_bytes = want;
+  }
+  return alloc(n, n->op_tab, n->op_host_bytes);
+}
+static int op_upload(Net* n, size_t bytes) {
+  HIP_TRY(hipMemcpyAsync(n->op_tab.p, n->op_host, bytes, hipMemcpyHostToDevice, n->stream));
+  return OK;
+}
+
+// Waits for the network's stream and turns the operators' error words into a code.
+static int op_finish(Net* n) {
+  HIP_TRY(hipGetLastError());
+  HIP_TRY(hipStreamSynchronize(n->stream));
+  uint32_t w[OE_WORDS];
+  for (int i = 0; i < OE_WORDS; ++i) {
+    w[i] = __atomic_load_n(&n->op_err[i], __ATOMIC_ACQUIRE);
+    if (w[i]) __atomic_store_n(&n->op_err[i], 0u, __ATOMIC_RELEASE);
+  }
+  if (w[OE_BAD_TOKEN]) return fail(ERR_ARG, "a token id of the history or the biases is outside the vocabulary");
+  if (w[OE_BAD_PENALTY]) return fail(ERR_ARG, "penalties must be finite and the repetition penalty above 0");
+  if (w[OE_NAN]) return fail(ERR_NAN, "greedy_decoding: NaN in logits (sampling_methods.rs:12)");
+  return OK;
+}
+
+// per-chunk argmax partials of `rows` logit rows (in am_v, am_i)
+static int stage_rules(Net* n, uint32_t rows, uint32_t V) {
+  const size_t parts = (size_t)rows * logit_chunks((int)V);
+  TRY(reserve(n, n->am_v, parts * sizeof(double)));
+  return reserve(n, n->am_i, parts * sizeof(int));
+}
+static void bind_rules(Net* n, LogitRules& r) {
+  r.part_v = n->am_v.as<double>();
+  r.part_i = n->am_i.as<int>();
+  r.counters = n->sync_cnt.as<uint32_t>();
+  r.err = n->op_err;
+}
+
+// ---- trees ----
+// parents and counts of a call; NULL counts: every node is used
+static int check_tree(const uint32_t* parents, const uint32_t* counts, uint32_t B, uint32_t nodes) {
+  if (!B || !nodes) return fail(ERR_ARG, "tree: empty batch or no nodes");
+  if (nodes > (uint32_t)TREE_MAX_NODES) return fail(ERR_ARG, "tree: %u nodes, at most %d", nodes, TREE_MAX_NODES);
+  for (uint32_t b = 0; b < B; ++b) {
+    const uint32_t c = counts ? counts[b] : nodes;
+    if (c > nodes) return fail(ERR_ARG, "tree: counts[%u]=%u above %u nodes", b, c, nodes);
+    for (uint32_t i = 0; i < c; ++i) {
+      const uint32_t p = parents[(size_t)b * nodes + i];
+      if (p != MITOK_NO_PARENT && p >= i)
+        return fail(ERR_ARG, "tree: node %u of sequence %u has parent %u: parents come before their children", i, b, p);
+    }
+  }
+  return OK;
+}
+
+// Lengths, counts, depths and ancestor bits of a call's trees, staged and
+// uploaded to op_tab; fills a's pointers and sizes.  *depth: the nodes' depths
+// [B][nodes] in the staging.
+static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, const uint32_t* counts, uint32_t B,
+                      uint32_t nodes, TreeAttn& a, const int** depth = nullptr) {
+  const int words = (int)(nodes + 63) / 64;
+  const size_t bn = (size_t)B * nodes;
+  const size_t seen_b = bn * words * sizeof(unsigned long long);
+  const size_t bytes = seen_b + (2 * (size_t)B + bn) * sizeof(int);
+  TRY(op_staging(n, bytes));
+  auto* seen = (unsigned long long*)n->op_host;
+  int* kv = (int*)(n->op_host + seen_b);
+  int* cnt = kv + B;
+  int* dep = cnt + B;
+  memset(seen, 0, seen_b);
+  a.T_max = 0;
+  for (uint32_t b = 0; b < B; ++b) {
+    const uint32_t c = counts ? counts[b] : nodes;
+    kv[b] = (int)kv_lens[b];
+    cnt[b] = (int)c;
+    a.T_max = std::max(a.T_max, kv[b] + cnt[b]);
+    for (uint32_t i = 0; i < nodes; ++i) {
+      unsigned long long* s = seen + ((size_t)b * nodes + i) * words;
+      int& d = dep[(size_t)b * nodes + i];
+      d = 0;
+      if (i >= c) continue;
+      const uint32_t p = parents[(size_t)b * nodes + i];
+      if (p != MITOK_NO_PARENT) {
+        memcpy(s, seen + ((size_t)b * nodes + p) * words, words * sizeof(*s));
+        d = dep[(size_t)b * nodes + p] + 1;
+      }
+      s[i >> 6] |= 1ull << (i & 63);
+    }
+  }
+  if (depth) *depth = dep;
+  TRY(op_upload(n, bytes));
+  const char* t = (const char*)n->op_tab.p;
+  a.seen = (const unsigned long long*)t;
+  a.words = words;
+  a.kv_len = (const int*)(t + seen_b);
+  a.count = a.kv_len + B;
+  a.depth = a.count + B;
+  a.B = (int)B;
+  a.n = (int)nodes;
+  return OK;
+}
+
+int mitok_tree_attention_device(mitok_network* n, const double* d_q, const double* d_k, const double* d_v,
+                                const double* d_bias, uint64_t bias_stride, const uint32_t* kv_lens,
+                                const uint32_t* parents, const uint32_t* counts, uint32_t B, uint32_t nodes,
+                                uint32_t heads, uint32_t dh, uint32_t ctx, uint32_t weigh_nodes, double* d_weights,
+                                double* d_out) {
+  if (!n || !d_q || !d_k || !d_v || !kv_lens || !parents || !d_out) return fail(ERR_ARG, "tree attention: null argument");
+  TRY(check_tree(parents, counts, B, nodes));
+  if (!heads || !dh || !ctx || ctx > (uint32_t)INT32_MAX) return fail(ERR_ARG, "tree attention: bad shape");
+  if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "tree attention: head dim %u > %d unsupported", dh, TREE_MAX_DH);
+  if (B > 65535 || heads > 65535) return fail(ERR_ARG, "tree attention: batch and heads at most 65535");
+  if (weigh_nodes && !d_weights) return fail(ERR_ARG, "tree attention: weigh_nodes without weights");
+  if (weigh_nodes > nodes) return fail(ERR_ARG, "tree attention: weigh_nodes %u above %u nodes", weigh_nodes, nodes);
+  uint32_t longest = 0;
+  for (uint32_t b = 0; b < B; ++b) {
+    const uint64_t end = (uint64_t)kv_lens[b] + (counts ? counts[b] : nodes);
+    if (end > ctx) return fail(ERR_ARG, "tree attention: kv_lens[%u]=%u and its nodes exceed max_ctx %u", b, kv_lens[b], ctx);
+    longest = std::max(longest, (uint32_t)end);
+  }
+  if (d_bias && heads > 1 && bias_stride < longest)
+    return fail(ERR_ARG, "tree attention: bias_stride %llu below the %u slots used", (unsigned long long)bias_stride, longest);
+  if (bias_stride > (uint64_t)INT64_MAX / 16) return fail(ERR_ARG, "tree attention: bias_stride out of range");
+  TRY(set_device(n));
+  const size_t qb = times({B, nodes, heads, dh, sizeof(double2)}), cb = times({B, heads, ctx, dh, sizeof(double2)});
+  const size_t wb = times({B, heads, ctx, sizeof(double)});
+  const size_t strides = times({heads - 1, (size_t)bias_stride, sizeof(double)});
+  const size_t bb = strides > SIZE_MAX / 2 ? SIZE_MAX : strides + (size_t)longest * sizeof(double);
+  TRY(check_device_array(n, d_q, qb, 16, "q"));
+  TRY(check_device_array(n, d_k, cb, 16, "k_cache"));
+  TRY(check_device_array(n, d_v, cb, 16, "v_cache"));
+  TRY(check_device_array(n, d_out, qb, 16, "out"));
+  if (d_bias) TRY(check_device_array(n, d_bias, bb, 8, "bias"));
+  if (d_weights) TRY(check_device_array(n, d_weights, wb, 8, "weights"));
+  const Span q = {d_q, qb, "q"}, k = {d_k, cb, "k_cache"}, v = {d_v, cb, "v_cache"}, bi = {d_bias, bb, "bias"};
+  const Span w = {weigh_nodes ? d_weights : nullptr, wb, "weights"}, o = {d_out, qb, "out"};
+  TRY(check_apart(o, {q, k, v, bi, w}));
+  TRY(check_apart(w, {q, k, v, bi}));
+  TreeAttn a;
+  a.q = (const double2*)d_q;
+  a.ldq = a.ldo = (long)heads * dh;
+  a.kc = (const double2*)d_k;
+  a.vc = (const double2*)d_v;
+  a.bias = d_bias;
+  a.bias_stride = (long)bias_stride;
+  a.H = (int)heads;
+  a.dh = (int)dh;
+  a.ctx = (int)ctx;
+  a.scale = 1.0 / (1e-8 + sqrt((double)dh));  // as the layers' (masked_attention_head.rs:453-465)
+  a.weigh = (int)weigh_nodes;
+  a.weights = weigh_nodes ? d_weights : nullptr;
+  a.out = (double2*)d_out;
+  TRY(behind_default_stream(n));
+  TRY(stage_tree(n, kv_lens, parents, counts, B, nodes, a));
+  TRY(alloc(n, n->op_ws, tree_ws_bytes(a)));
+  a.ws = n->op_ws.p;
+  tree_attention(n->stream, a);
+  return op_finish(n);
+}
+
+// The next tokens' tree through every layer (mitok_tree_step).
+static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts, uint32_t B,
+                          uint32_t nodes, uint32_t weigh, uint32_t* out_ids, double* out_logits, double* d_logits) {
+  hipStream_t st = n->stream;
+  const uint32_t V = n->layers[n->layers.size() - 2]->d_out;
+  const size_t rows = (size_t)B * nodes;
+  Spec sp;
+  sp.B = (int)B;
+  sp.S = (int)nodes;
+  sp.mode = MODE_CACHED;
+  sp.last = (uint32_t)n->layers.size();
+  TRY(prepare(n, sp));
+  TRY(stage_rules(n, (uint32_t)rows, V));
+  TRY(alloc(n, n->tree_ids, rows * sizeof(uint32_t)));
+  TRY(alloc(n, n->tree_rng, 2 * (size_t)B * sizeof(int)));
+  TreeAttn tree;
+  const int* depth = nullptr;
+  // the rows whose weights are kept so far, zero for those appended since
+  std::vector<int> from(B), to(B);
+  int most = 0;
+  if (weigh) {
+    for (auto& L : n->layers)
+      if (L->kind == K_SELF_ATTENTION) {
+        auto* A = (SelfAttentionLayer*)L.get();
+        TRY(alloc(n, A->aw, (size_t)B * A->heads * A->max_ctx * sizeof(double)));
+      }
+    for (uint32_t b = 0; b < B; ++b) {
+      from[b] = n->aw_len.empty() ? 0 : (int)std::min(n->aw_len[b], n->kv_len_h[b]);
+      to[b] = (int)n->kv_len_h[b];
+      most = std::max(most, to[b] - from[b]);
+    }
+  }
+  size_t ws = 0;
+  for (auto& L : n->layers)
+    if (L->kind == K_SELF_ATTENTION) {
+      auto* A = (SelfAttentionLayer*)L.get();
+      TreeAttn t;
+      t.B = (int)B, t.n = (int)nodes, t.H = (int)A->heads, t.dh = (int)A->dh, t.weigh = (int)weigh;
+      t.T_max = (int)A->max_ctx;
+      ws = std::max(ws, tree_ws_bytes(t));
+    }
+  TRY(alloc(n, n->op_ws, ws));
+  TRY(stage_tree(n, n->kv_len_h.data(), parents, counts, B, nodes, tree, &depth));
+  tree.ws = n->op_ws.p;
+  tree.weigh = (int)weigh;
+  std::vector<uint32_t> padded(rows), mask(rows);
+  std::vector<int> pos(rows);
+  int maxpos = 0;
+  for (uint32_t b = 0; b < B; ++b)
+    for (uint32_t i = 0; i < nodes; ++i) {
+      const size_t r = (size_t)b * nodes + i;
+      const bool used = i < (counts ? counts[b] : nodes);
+      padded[r] = used ? ids[r] : 1u;
+      mask[r] = used ? 1u : 0u;
+      pos[r] = (int)next_position(n, b) + depth[r];
+      maxpos = std::max(maxpos, pos[r]);
+    }
+  TRY(ensure_rope_for(n, 0, sp.last, std::max(rope_positions_needed(n), maxpos + 1)));
+  TRY(upload(n, n->ids_d, padded.data(), rows * sizeof(uint32_t)));
+  TRY(upload(n, n->mask_d, mask.data(), rows * sizeof(uint32_t)));
+  TRY(upload(n, n->pos_d, pos.data(), rows * sizeof(int)));
+  std::vector<int> kv(n->kv_len_h.begin(), n->kv_len_h.end());
+  TRY(upload(n, n->kv_len_d, kv.data(), B * sizeof(int)));
+  if (weigh && most > 0) {
+    HIP_TRY(hipMemcpyAsync(n->tree_rng.p, from.data(), B * sizeof(int), hipMemcpyHostToDevice, st));
+    HIP_TRY(hipMemcpyAsync(n->tree_rng.as<int>() + B, to.data(), B * sizeof(int), hipMemcpyHostToDevice, st));
+    for (auto& L : n->layers)
+      if (L->kind == K_SELF_ATTENTION) {
+        auto* A = (SelfAttentionLayer*)L.get();
+        zero_weights(st, A->aw.as<double>(), (int)B, (int)A->heads, A->max_ctx, n->tree_rng.as<int>(),
+                     n->tree_rng.as<int>() + B, most);
+      }
+  }
+  sp.ids = n->ids_d.as<uint32_t>();
+  sp.mask = n->mask_d.as<uint32_t>();
+  sp.pos = n->pos_d.as<int>();
+  sp.out_re = d_logits ? d_logits : n->logits_re.as<double>();
+  sp.tree = &tree;
+  TRY(enqueue_forward(n, sp));
+  LogitRules r;
+  r.x = sp.out_re;
+  r.rows = (int)rows;
+  r.V = (int)V;
+  r.row_mask = sp.mask;
+  r.ids = n->tree_ids.as<uint32_t>();
+  bind_rules(n, r);
+  logit_rules(st, r);
+  if (out_ids) HIP_TRY(hipMemcpyAsync(out_ids, n->tree_ids.p, rows * sizeof(uint32_t), hipMemcpyDeviceToHost, st));
+  if (out_logits) HIP_TRY(hipMemcpyAsync(out_logits, sp.out_re, rows * V * sizeof(double), hipMemcpyDeviceToHost, st));
+  const int rc = op_finish(n);
+  collect_timing(n);
+  TRY(check_err_word(n));  // the first cause
+  TRY(rc);
+  if (weigh) n->aw_len = n->kv_len_h;
+  n->tree_valid = true;
+  n->tree_weighed = weigh != 0;
+  n->tree_n = nodes;
+  n->tree_parents.assign(parents, parents + rows);
+  n->tree_counts.assign(B, nodes);
+  if (counts) n->tree_counts.assign(counts, counts + B);
+  return OK;
+}
+
+static int tree_step_checked(Net* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts, uint32_t B,
+                             uint32_t nodes, uint32_t weigh, uint32_t* out_ids, double* out_logits, double* d_logits) {
+  if (!n || !ids || !parents) return fail(ERR_ARG, "null argument");
+  TRY(check_stack(n));
+  if (!n->cache_valid) return fail(ERR_STATE, "tree_step before prefill (no KV cache)");
+  if (B != n->cache_B) return fail(ERR_STATE, "cached batch %u != %u; prefill first", n->cache_B, B);
+  TRY(check_tree(parents, counts, B, nodes));
+  if (weigh > nodes) return fail(ERR_ARG, "weigh_nodes %u above %u nodes", weigh, nodes);
+  const uint32_t mc = min_ctx(n);
+  if (mc == UINT32_MAX) return fail(ERR_STATE, "tree_step: the stack has no attention layer");
+  const uint32_t V0 = ((const EmbeddingLayer*)n->layers[0].get())->vocab;
+  for (uint32_t b = 0; b < B; ++b) {
+    if ((uint64_t)n->kv_len_h[b] + nodes > mc)
+      return fail(ERR_ARG, "context %u and %u nodes exceed max context %u", n->kv_len_h[b], nodes, mc);
+    for (uint32_t i = 0; i < (counts ? counts[b] : nodes); ++i)
+      if (ids[(size_t)b * nodes + i] >= V0)
+        return fail(ERR_ARG, "No token embedding found: token id %u >= vocab %u (embedding_layer.rs:305)",
+                    ids[(size_t)b * nodes + i], V0);
+  }
+  TRY(set_device(n));
+  if (d_logits) {
+    const uint32_t V = n->layers[n->layers.size() - 2]->d_out;
+    TRY(check_device_array(n, d_logits, times({B, nodes, V, sizeof(double)}), 8, "logits"));
+    TRY(behind_default_stream(n));
+  }
+  const int rc = tree_step_impl(n, ids, parents, counts, B, nodes, weigh, out_ids, out_logits, d_logits);
+  if (rc) (void)mitok_reset(n);
+  return rc;
+}
+
+int mitok_tree_step(mitok_network* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts, uint32_t B,
+                    uint32_t nodes, uint32_t weigh_nodes, uint32_t* out_ids, double* out_logits) {
+  return tree_step_checked(n, ids, parents, counts, B, nodes, weigh_nodes, out_ids, out_logits, nullptr);
+}
+
+int mitok_tree_step_device(mitok_network* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts,
+                           uint32_t B, uint32_t nodes, uint32_t weigh_nodes, double* d_logits) {
+  if (!d_logits) return fail(ERR_ARG, "null argument");
+  return tree_step_checked(n, ids, parents, counts, B, nodes, weigh_nodes, nullptr, nullptr, d_logits);
+}
+
+int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* path_lens, uint32_t B, uint32_t max_path) {
+  if (!n || !path || !path_lens || !max_path) return fail(ERR_ARG, "null argument");
+  if (!n->tree_valid) return fail(ERR_STATE, "tree_accept without a tree_step before it");
+  if (B != n->cache_B) return fail(ERR_STATE, "cached batch %u != %u", n->cache_B, B);
+  for (uint32_t b = 0; b < B; ++b) {
+    if (path_lens[b] > max_path) return fail(ERR_ARG, "path_lens[%u]=%u above %u", b, path_lens[b], max_path);
+    uint32_t before = MITOK_NO_PARENT;
+    for (uint32_t k = 0; k < path_lens[b]; ++k) {
+      const uint32_t i = path[(size_t)b * max_path + k];
+      if (i >= n->tree_counts[b]) return fail(ERR_ARG, "path of sequence %u: node %u of %u", b, i, n->tree_counts[b]);
+      if (n->tree_parents[(size_t)b * n->tree_n + i] != before)
+        return fail(ERR_ARG, "path of sequence %u: node %u does not follow the one before it", b, i);
+      before = i;
+    }
+  }
+  TRY(set_device(n));
+  hipStream_t st = n->stream;
+  // [path | rows moved | committed rows | last node | rows then]; a path without gaps stays where it is
+  const size_t bp = (size_t)B * max_path;
+  TRY(op_staging(n, (bp + 4 * (size_t)B) * sizeof(int)));
+  uint32_t* p = (uint32_t*)n->op_host;
+  int *moved = (int*)(p + bp), *base = moved + B, *last = base + B, *then = last + B, most = 0;
+  memcpy(p, path, bp * sizeof(uint32_t));
+  for (uint32_t b = 0; b < B; ++b) {
+    const uint32_t len = path_lens[b];
+    moved[b] = len && path[(size_t)b * max_path + len - 1] != len - 1 ? (int)len : 0;
+    base[b] = (int)n->kv_len_h[b];
+    last[b] = len ? (int)path[(size_t)b * max_path + len - 1] : -1;
+    then[b] = base[b] + (int)len;
+    most = std::max(most, moved[b]);
+  }
+  TRY(op_upload(n, (bp + 4 * (size_t)B) * sizeof(int)));
+  const uint32_t* dp = n->op_tab.as<uint32_t>();
+  const int* dm = (const int*)(dp + bp);
+  for (auto& L : n->layers) {
+    if (L->kind != K_SELF_ATTENTION || !most) continue;
+    auto* A = (SelfAttentionLayer*)L.get();
+    CacheMove m;
+    m.k = m.ko = A->kc.as<double2>();
+    m.v = m.vo = A->vc.as<double2>();
+    if (!n->aw_len.empty()) m.w = m.wo = A->aw.as<double>();
+    m.B = (int)B;
+    m.H = (int)A->heads;
+    m.dh = (int)A->dh;
+    m.ctx = m.ctx_out = A->max_ctx;
+    m.base = dm + B;
+    m.idx = dp;
+    m.idx_b = max_path;
+    m.rows = dm;
+    m.rows_max = most;
+    cache_move(st, m);
+  }
+  pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, dm + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
+  HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, then, B * sizeof(int), hipMemcpyHostToDevice, st));  // decode steps read it
+  TRY(op_finish(n));
+  const bool weighed = !n->aw_len.empty();
+  for (uint32_t b = 0; b < B; ++b) {
+    const bool whole = weighed && n->aw_len[b] == n->kv_len_h[b];
+    n->kv_len_h[b] += path_lens[b];
+    if (whole && n->tree_weighed) n->aw_len[b] = n->kv_len_h[b];
+  }
+  n->tree_valid = false;
+  return OK;
+}
+
+// ---- eviction ----
+static int check_evict(uint32_t keep, uint32_t sinks, uint32_t recent) {
+  if (!keep || keep > (uint32_t)INT32_MAX) return fail(ERR_ARG, "evict: keep %u", keep);
+  if ((uint64_t)sinks + recent > keep) return fail(ERR_ARG, "evict: %u sinks and %u recent rows exceed keep %u", sinks, recent, keep);
+  return OK;
+}
+
+int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d_v, const double* d_weights,
+                            const uint32_t* kv_lens, uint32_t B, uint32_t heads, uint32_t dh, uint32_t ctx,
+                            uint32_t keep, uint32_t sinks, uint32_t recent, double* d_k_out, double* d_v_out,
+                            double* d_weights_out, uint32_t out_ctx, uint32_t* d_kept, uint32_t* out_lens) {
+  if (!n || !d_k || !d_v || !d_weights || !kv_lens || !d_k_out || !d_v_out || !d_weights_out || !out_lens)
+    return fail(ERR_ARG, "evict: null argument");
+  if (!B || !heads || !dh || !ctx || ctx > (uint32_t)INT32_MAX || B > 65535 || heads > 65535)
+    return fail(ERR_ARG, "evict: bad shape");
+  if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "evict: head dim %u > %d unsupported", dh, TREE_MAX_DH);
+  TRY(check_evict(keep, sinks, recent));
+  uint32_t longest = 0;
+  for (uint32_t b = 0; b < B; ++b) {
+    if (kv_lens[b] > ctx) return fail(ERR_ARG, "evict: kv_lens[%u]=%u exceeds max_ctx %u", b, kv_lens[b], ctx);
+    longest = std::max(longest, kv_lens[b]);
+  }
+  const uint32_t stay = std::min(longest, keep);
+  if (stay > out_ctx) return fail(ERR_ARG, "evict: %u rows do not fit out_ctx %u", stay, out_ctx);
+  TRY(set_device(n));
+  const size_t cb = times({B, heads, ctx, dh, sizeof(double2)}), co = times({B, heads, out_ctx, dh, sizeof(double2)});
+  const size_t wb = times({B, heads, ctx, sizeof(double)}), wo = times({B, heads, out_ctx, sizeof(double)});
+  const size_t kb = times({B, heads, keep, sizeof(uint32_t)});
+  TRY(check_device_array(n, d_k, cb, 16, "k_cache"));
+  TRY(check_device_array(n, d_v, cb, 16, "v_cache"));
+  TRY(check_device_array(n, d_weights, wb, 8, "weights"));
+  TRY(check_device_array(n, d_k_out, co, 16, "k_out"));
+  TRY(check_device_array(n, d_v_out, co, 16, "v_out"));
+  TRY(check_device_array(n, d_weights_out, wo, 8, "weights_out"));
+  if (d_kept) TRY(check_device_array(n, d_kept, kb, 4, "kept"));
+  const Span k = {d_k, cb, "k_cache"}, v = {d_v, cb, "v_cache"}, w = {d_weights, wb, "weights"};
+  const Span ko = {d_k_out, co, "k_out"}, vo = {d_v_out, co, "v_out"}, wt = {d_weights_out, wo, "weights_out"};
+  const Span ke = {d_kept, kb, "kept"};
+  // in place: all three arrays, of one size; otherwise nothing may overlap
+  const bool in_place = d_k_out == d_k && d_v_out == d_v && d_weights_out == d_weights && out_ctx == ctx;
+  TRY(check_apart(ko, {vo, wt}));
+  TRY(check_apart(wt, {vo}));
+  if (!in_place) {
+    TRY(check_apart(ko, {k, v, w}));
+    TRY(check_apart(vo, {k, v, w}));
+    TRY(check_apart(wt, {k, v, w}));
+  }
+  TRY(check_apart(ke, {k, v, w, ko, vo, wt}));
+  TRY(behind_default_stream(n));
+  TRY(op_staging(n, 2 * (size_t)B * sizeof(int)));
+  int *kv = (int*)n->op_host, *rows = kv + B;
+  for (uint32_t b = 0; b < B; ++b) {
+    kv[b] = (int)kv_lens[b];
+    rows[b] = (int)std::min(kv_lens[b], keep);
+  }
+  if (!d_kept) TRY(alloc(n, n->op_ws, kb));
+  TRY(op_upload(n, 2 * (size_t)B * sizeof(int)));
+  EvictSelect e;
+  e.w = d_weights;
+  e.kv_len = n->op_tab.as<int>();
+  e.B = (int)B;
+  e.H = (int)heads;
+  e.ctx = ctx;
+  e.T_max = (int)longest;
+  e.keep = (int)keep;
+  e.sinks = (int)sinks;
+  e.recent = (int)recent;
+  e.kept = d_kept ? d_kept : n->op_ws.as<uint32_t>();
+  evict_select(n->stream, e);
+  CacheMove m;
+  m.k = (const double2*)d_k;
+  m.v = (const double2*)d_v;
+  m.w = d_weights;
+  m.ko = (double2*)d_k_out;
+  m.vo = (double2*)d_v_out;
+  m.wo = d_weights_out;
+  m.B = (int)B;
+  m.H = (int)heads;
+  m.dh = (int)dh;
+  m.ctx = ctx;
+  m.ctx_out = out_ctx;
+  m.idx = e.kept;
+  m.idx_b = (long)heads * keep;
+  m.idx_h = keep;
+  m.rows = e.kv_len + B;
+  m.rows_max = (int)stay;
+  cache_move(n->stream, m);
+  TRY(op_finish(n));
+  for (uint32_t b = 0; b < B; ++b) out_lens[b] = std::min(kv_lens[b], keep);
+  return OK;
+}
+
+int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks, uint32_t recent, uint32_t* out_lens) {
+  if (!n) return fail(ERR_ARG, "null network");
+  TRY(check_evict(keep, sinks, recent));
+  if (!n->cache_valid) return fail(ERR_STATE, "evict before prefill (no KV cache)");
+  if (n->aw_len.empty()) return fail(ERR_STATE, "evict: no tree_step has weighed attention since the prompt");
+  if (B != n->cache_B) return fail(ERR_STATE, "cached batch %u != %u", n->cache_B, B);
+  TRY(set_device(n));
+  hipStream_t st = n->stream;
+  // rows appended by other calls since the last weighed step have no weight yet
+  TRY(op_staging(n, 4 * (size_t)B * sizeof(int)));
+  int *kv = (int*)n->op_host, *rows = kv + B, *from = rows + B, *off = from + B, most = 0, longest = 0;
+  bool any = false;
+  const bool had_off = n->pos_off && n->pos_off_h.size() == B;
+  for (uint32_t b = 0; b < B; ++b) {
+    kv[b] = (int)n->kv_len_h[b];
+    rows[b] = (int)std::min(n->kv_len_h[b], keep);
+    from[b] = (int)std::min(n->aw_len[b], n->kv_len_h[b]);
+    off[b] = (had_off ? n->pos_off_h[b] : 0) + kv[b] - rows[b];
+    most = std::max(most, kv[b] - from[b]);
+    longest = std::max(longest, kv[b]);
+    any = any || rows[b] != kv[b];
+  }
+  n->tree_valid = false;
+  if (any) {
+    size_t kb = 0;
+    for (auto& L : n->layers)
+      if (L->kind == K_SELF_ATTENTION)
+        kb = std::max(kb, times({B, ((SelfAttentionLayer*)L.get())->heads, keep, sizeof(uint32_t)}));
+    TRY(alloc(n, n->op_ws, kb));
+    TRY(op_upload(n, 4 * (size_t)B * sizeof(int)));
+    const int* t = n->op_tab.as<int>();
+    for (auto& L : n->layers) {
+      if (L->kind != K_SELF_ATTENTION) continue;
+      auto* A = (SelfAttentionLayer*)L.get();
+      zero_weights(st, A->aw.as<double>(), (int)B, (int)A->heads, A->max_ctx, t + 2 * B, t, most);
+      EvictSelect e;
+      e.w = A->aw.as<double>();
+      e.kv_len = t;
+      e.B = (int)B;
+      e.H = (int)A->heads;
+      e.ctx = A->max_ctx;
+      e.T_max = longest;
+      e.keep = (int)keep;
+      e.sinks = (int)sinks;
+      e.recent = (int)recent;
+      e.kept = n->op_ws.as<uint32_t>();
+      evict_select(st, e);
+      CacheMove m;
+      m.k = m.ko = A->kc.as<double2>();
+      m.v = m.vo = A->vc.as<double2>();
+      m.w = m.wo = A->aw.as<double>();
+      m.B = (int)B;
+      m.H = (int)A->heads;
+      m.dh = (int)A->dh;
+      m.ctx = m.ctx_out = A->max_ctx;
+      m.idx = e.kept;
+      m.idx_b = (long)A->heads * keep;
+      m.idx_h = keep;
+      m.rows = t + B;
+      m.rows_max = std::min(longest, (int)keep);
+      cache_move(st, m);
+    }
+    // later tokens stand where they would without the eviction
+    if (!n->pos_off) drop_graph(n);
+    n->pos_off = true;
+    TRY(reserve(n, n->pos_off_d, (size_t)B * sizeof(int)));
+    HIP_TRY(hipMemcpyAsync(n->pos_off_d.p, off, B * sizeof(int), hipMemcpyHostToDevice, st));
+    HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, rows, B * sizeof(int), hipMemcpyHostToDevice, st));
+    const int rc = op_finish(n);
+    if (rc) {
+      (void)mitok_reset(n);
+      return rc;
+    }
+    n->pos_off_h.assign(off, off + B);
+    for (uint32_t b = 0; b < B; ++b) n->kv_len_h[b] = (uint32_t)rows[b];
+    n->aw_len = n->kv_len_h;
+  }
+  if (out_lens) memcpy(out_lens, n->kv_len_h.data(), B * sizeof(uint32_t));
+  return OK;
+}
+
+// ---- logits to a token ----
+int mitok_process_logits_device(mitok_network* n, const double* d_logits, uint32_t rows, uint32_t V,
+                                const uint32_t* d_history, uint32_t max_history, const double* d_penalties,
+                                const uint32_t* d_bias_ids, const double* d_bias, uint32_t max_bias,
+                                const uint32_t* d_allowed, double* d_out, uint32_t* d_out_ids) {
+  if (!n || !d_logits || !rows || !V) return fail(ERR_ARG, "process_logits: bad arguments");
+  if (!d_out && !d_out_ids) return fail(ERR_ARG, "process_logits: neither logits nor ids wanted");
+  if (rows > (uint32_t)INT32_MAX || V > (uint32_t)INT32_MAX - 64 || max_history > (uint32_t)INT32_MAX ||
+      max_bias > (uint32_t)INT32_MAX)
+    return fail(ERR_ARG, "process_logits: a size beyond 31 bits");
+  if (max_history && (!d_history || !d_penalties)) return fail(ERR_ARG, "process_logits: a history needs its tokens and penalties");
+  if (max_bias && (!d_bias_ids || !d_bias)) return fail(ERR_ARG, "process_logits: biases need their ids and values");
+  TRY(set_device(n));
+  const size_t xb = times({rows, V, sizeof(double)}), hb = times({rows, max_history, sizeof(uint32_t)});
+  const size_t pb = times({rows, 3, sizeof(double)}), ib = times({rows, max_bias, sizeof(uint32_t)}), bb = times({rows, max_bias, sizeof(double)});
+  const size_t mb = times({rows, (V + 31) / 32, sizeof(uint32_t)}), ob = times({rows, sizeof(uint32_t)});
+  const bool hist = max_history != 0, bias = max_bias != 0;
+  TRY(check_device_array(n, d_logits, xb, 8, "logits"));
+  if (hist) TRY(check_device_array(n, d_history, hb, 4, "history"));
+  if (hist) TRY(check_device_array(n, d_penalties, pb, 8, "penalties"));
+  if (bias) TRY(check_device_array(n, d_bias_ids, ib, 4, "bias_ids"));
+  if (bias) TRY(check_device_array(n, d_bias, bb, 8, "bias"));
+  if (d_allowed) TRY(check_device_array(n, d_allowed, mb, 4, "allowed"));
+  if (d_out) TRY(check_device_array(n, d_out, xb, 8, "out"));
+  if (d_out_ids) TRY(check_device_array(n, d_out_ids, ob, 4, "out_ids"));
+  const Span x = {d_logits, xb, "logits"}, h = {hist ? d_history : nullptr, hb, "history"},
+             p = {hist ? d_penalties : nullptr, pb, "penalties"}, bi = {bias ? d_bias_ids : nullptr, ib, "bias_ids"},
+             bv = {bias ? d_bias : nullptr, bb, "bias"}, al = {d_allowed, mb, "allowed"}, o = {d_out, xb, "out"},
+             id = {d_out_ids, ob, "out_ids"};
+  TRY(check_apart(o, {h, p, bi, bv, al, id}));
+  if (d_out != d_logits) TRY(check_apart(o, {x}));
+  TRY(check_apart(id, {x, h, p, bi, bv, al}));
+  TRY(behind_default_stream(n));
+  TRY(stage_rules(n, rows, V));
+  LogitRules r;
+  r.x = d_logits;
+  r.rows = (int)rows;
+  r.V = (int)V;
+  r.history = hist ? d_history : nullptr;
+  r.hist = (int)max_history;
+  r.penalties = hist ? d_penalties : nullptr;
+  r.bias_ids = d_bias_ids;
+  r.bias = d_bias;
+  r.nb = (int)max_bias;
+  r.allowed = d_allowed;
+  r.out = d_out;
+  r.ids = d_out_ids;
+  bind_rules(n, r);
+  logit_rules(n->stream, r);
+  return op_finish(n);
+}
+
+int mitok_process_logits(mitok_network* n, const double* logits, uint32_t rows, uint32_t V, const uint32_t* history,
+                         uint32_t max_history, const double* penalties, const uint32_t* bias_ids, const double* bias,
+                         uint32_t max_bias, const uint32_t* allowed, double* out, uint32_t* out_ids) {
+  if (!n || !logits || !rows || !V) return fail(ERR_ARG, "process_logits: bad arguments");
+  if (max_history && (!history || !penalties)) return fail(ERR_ARG, "process_logits: a history needs its tokens and penalties");
+  if (max_bias && (!bias_ids || !bias)) return fail(ERR_ARG, "process_logits: biases need their ids and values");
+  TRY(set_device(n));
+  DevBuf x, h, p, bi, bv, al, id;
+  const auto put = [&](DevBuf& b, const void* src, size_t bytes) -> int {
+    if (bytes == SIZE_MAX) return fail(ERR_ARG, "process_logits: a size passes 64 bits");
+    if (!src || !bytes) return OK;
+    TRY(alloc(n, b, bytes));
+    HIP_TRY(hipMemcpyAsync(b.p, src, bytes, hipMemcpyHostToDevice, n->stream));
+    return OK;
+  };
+  TRY(put(x, logits, times({rows, V, sizeof(double)})));
+  if (max_history) {
+    TRY(put(h, history, times({rows, max_history, sizeof(uint32_t)})));
+    TRY(put(p, penalties, times({rows, 3, sizeof(double)})));
+  }
+  TRY(put(bi, bias_ids, times({rows, max_bias, sizeof(uint32_t)})));
+  TRY(put(bv, bias, times({rows, max_bias, sizeof(double)})));
+  TRY(put(al, allowed, times({rows, ((size_t)V + 31) / 32, sizeof(uint32_t)})));
+  if (out_ids) TRY(alloc(n, id, rows * sizeof(uint32_t)));
+  const int rc = mitok_process_logits_device(n, x.as<double>(), rows, V, h.as<uint32_t>(), max_history, p.as<double>(),
+                                             bi.as<uint32_t>(), bv.as<double>(), max_bias, al.as<uint32_t>(),
+                                             out ? x.as<double>() : nullptr, id.as<uint32_t>());
+  TRY(rc);
+  if (out) HIP_TRY(hipMemcpyAsync(out, x.p, (size_t)rows * V * sizeof(double), hipMemcpyDeviceToHost, n->stream));
+  if (out_ids) HIP_TRY(hipMemcpyAsync(out_ids, id.p, rows * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
+  HIP_TRY(hipStreamSynchronize(n->stream));
+  return OK;
 }
 
 int mitok_last_timings(mitok_network* n, double* t3) {

@@ -1,0 +1,116 @@
+// serving.hpp — launch wrappers of the operators of a serving loop over the KV
+// cache: attention of drafted token trees (tree_attention.hip), eviction of
+// cached rows and the rules that turn logits into a token (serving.hip).
+//
+// As in kernels.hpp, every wrapper enqueues on `st` and neither synchronises
+// nor allocates.
+#pragma once
+
+#include "kernels.hpp"
+
+namespace mitok {
+
+// Words a kernel sets and the host reads once the stream is idle (pinned host
+// memory: no copy back).  Plain stores of 1, so any number of lanes may set one.
+enum OpErrWord : int { OE_BAD_TOKEN = 0, OE_NAN = 1, OE_BAD_PENALTY = 2, OE_WORDS = 4 };
+
+constexpr int TREE_MAX_NODES = 256;
+constexpr int TREE_WORDS = TREE_MAX_NODES / 64;
+constexpr int TREE_MAX_DH = 256;
+
+// ---- attention of a tree of drafted tokens ----
+// Node i of sequence b sits in cache slot kv_len[b] + i and sees the slots
+// before kv_len[b], its ancestors and itself:
+//   s(i, t) = Re(q_i . k_t) * scale + bias[h][column(t)],
+//   column(t) = t, or kv_len[b] + depth(j) for node j's slot
+//   out_i = sum_t softmax(s(i, .))_t v_t
+// weights (if not null): [b][h][t] += the sum over the first `weigh` nodes of
+// their softmax weights at the committed slots, = at the nodes' slots.
+struct TreeAttn {
+  const double2* q = nullptr;  // [B][n][ldq]; head h at column h * dh
+  long ldq = 0;
+  const double2* kc = nullptr;  // [B][H][ctx][dh]
+  const double2* vc = nullptr;
+  const double* bias = nullptr;  // [H][bias_stride] or null
+  long bias_stride = 0;
+  const int* kv_len = nullptr;         // [B]
+  const int* count = nullptr;          // [B] nodes used; rows past them are zero
+  const int* depth = nullptr;          // [B][n]
+  const unsigned long long* seen = nullptr;  // [B][n][words]: bit j of a node: itself or an ancestor
+  int words = 1;
+  int B = 0, n = 0, H = 0, dh = 0, ctx = 0;
+  int T_max = 0;  // the largest kv_len + count (sizing)
+  double scale = 1.0;
+  int weigh = 0;
+  double* weights = nullptr;  // [B][H][ctx]
+  double2* out = nullptr;     // [B][n][ldo]
+  long ldo = 0;
+  void* ws = nullptr;  // tree_ws_bytes
+};
+size_t tree_ws_bytes(const TreeAttn& a);
+void tree_attention(hipStream_t st, const TreeAttn& a);
+
+// ---- rows of a cache moved to its front, or to another cache's ----
+struct CacheMove {
+  const double2* k = nullptr;  // [B][H][ctx][dh]
+  const double2* v = nullptr;
+  const double* w = nullptr;  // [B][H][ctx] weights, or null
+  double2* ko = nullptr;      // [B][H][ctx_out][dh]; the same pointers: in place
+  double2* vo = nullptr;
+  double* wo = nullptr;
+  int B = 0, H = 0, dh = 0;
+  long ctx = 0, ctx_out = 0;
+  const int* base = nullptr;      // [B] slot that both sides count from, or null: 0
+  const uint32_t* idx = nullptr;  // row r of (b, h) comes from slot base + idx[b * idx_b + h * idx_h + r]; ascending
+  long idx_b = 0, idx_h = 0;
+  const int* rows = nullptr;  // [B] rows moved
+  int rows_max = 0;
+};
+void cache_move(hipStream_t st, const CacheMove& m);
+
+// ---- which rows an eviction keeps ----
+// Of kv_len[b] rows, `keep` stay where there are more: the first `sinks`, the
+// last `recent` and the others of largest weight (equal ones and NaN, which
+// counts as less than any number: the lowest slot first).  kept
+// [B][H][keep]: their slots ascending, then NO_ROW; rows [B]: min(kv_len, keep).
+constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
+struct EvictSelect {
+  const double* w = nullptr;  // [B][H][ctx]
+  const int* kv_len = nullptr;
+  int B = 0, H = 0;
+  long ctx = 0;
+  int T_max = 0;
+  int keep = 0, sinks = 0, recent = 0;
+  uint32_t* kept = nullptr;
+};
+void evict_select(hipStream_t st, const EvictSelect& e);
+
+// w[b][h][from[b] .. to[b]) = 0
+void zero_weights(hipStream_t st, double* w, int B, int H, long ctx, const int* from, const int* to, int most);
+// dec_ids[b] = ids[b * n + last[b]] where last[b] >= 0
+void pick_ids(hipStream_t st, const uint32_t* ids, int n, const int* last, int B, uint32_t* dec_ids);
+
+// ---- logits to a token ----
+constexpr uint32_t NO_TOKEN = 0xFFFFFFFFu;
+struct LogitRules {
+  const double* x = nullptr;  // [rows][V]
+  int rows = 0, V = 0;
+  const uint32_t* history = nullptr;  // [rows][hist] token ids, NO_TOKEN entries skipped
+  int hist = 0;
+  const double* penalties = nullptr;  // [rows][3]: repetition, presence, frequency
+  const uint32_t* bias_ids = nullptr;  // [rows][nb], NO_TOKEN entries skipped; of equal ids the last counts
+  const double* bias = nullptr;
+  int nb = 0;
+  const uint32_t* allowed = nullptr;   // [rows][(V + 31) / 32] bits
+  const uint32_t* row_mask = nullptr;  // [rows] or null: rows with 0 are skipped, their id NO_TOKEN
+  double* out = nullptr;               // [rows][V] or null; x itself: in place
+  uint32_t* ids = nullptr;             // [rows] or null
+  double* part_v = nullptr;            // [rows][logit_chunks(V)]
+  int* part_i = nullptr;
+  uint32_t* counters = nullptr;  // SYNC_COUNTERS words, zero
+  uint32_t* err = nullptr;       // OpErrWord
+};
+int logit_chunks(int V);
+void logit_rules(hipStream_t st, const LogitRules& r);
+
+}  // namespace mitok
