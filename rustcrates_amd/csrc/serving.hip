@@ -1,6 +1,8 @@
 // serving.hip — the other operators of a serving loop: rows evicted from the KV
 // cache by the attention they received, and the rules that turn logits into a
 // token (penalties for repeated tokens, biases, a mask of allowed tokens).
+#include <algorithm>
+
 #include "serving.hpp"
 
 namespace mitok {
@@ -8,84 +10,215 @@ namespace mitok {
 // ===========================================================================
 // eviction
 // ===========================================================================
-// a double as an integer of the same order; NaN is the least, -0 equals +0
+// a double as an integer of the same order, at least 2; NaN is 1, -0 equals +0
 __device__ __forceinline__ unsigned long long order_key(double w) {
-  if (isnan(w)) return 0ull;
+  if (isnan(w)) return 1ull;
   const unsigned long long u = (unsigned long long)__double_as_longlong(w + 0.0);
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-// One block per (head, sequence).  A slot between the sinks and the recent rows
-// stays if fewer than keep - sinks - recent others come before it (larger
-// weight, or equal and a lower slot); a scan gives the kept slots their places.
-__global__ __launch_bounds__(1024) void k_evict_select(EvictSelect e) {
-  __shared__ int total[16], carry;
+// One block per (head, sequence).  The least key that stays is found by
+// bisection between the smallest and the largest: each round counts the keys at
+// or above the middle (a compare and a ballot per key, held in registers), and
+// ends early once that is as many as have to stay: about 20 rounds of 0.1 us
+// for weights that differ, 64 at most.  Of equal least keys the lowest slots
+// stay; scans over the slots give ranks and places.  NK: slots per thread, 0:
+// any number, read again each round.
+template <int NK>
+__global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
+  __shared__ unsigned long long ext[2][4];
+  __shared__ int part[2][4];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int L = e.kv_len[b];
   const double* w = e.w + ((long)b * e.H + h) * e.ctx;
   uint32_t* kept = e.kept + ((long)b * e.H + h) * e.keep;
-  const int lo = e.sinks, hi = L - e.recent, most = e.keep - e.sinks - e.recent;
-  if (tid == 0) carry = 0;
-  __syncthreads();
-  for (int t0 = 0; t0 < L; t0 += 1024) {
-    const int t = t0 + tid;
-    bool stay = t < L;
-    if (stay && L > e.keep && t >= lo && t < hi) {
-      const unsigned long long mine = order_key(w[t]);
-      int before = 0;
-      for (int s = lo; s < hi; ++s) {
-        const unsigned long long k = order_key(w[s]);
-        before += k > mine || (k == mine && s < t) ? 1 : 0;
-      }
-      stay = before < most;
-    }
-    const unsigned long long vote = __ballot(stay);
-    if (lane == 0) total[wave] = __popcll(vote);
-    __syncthreads();
-    int at = carry + __popcll(vote & ((1ull << lane) - 1));
-    for (int x = 0; x < wave; ++x) at += total[x];
-    if (stay) kept[at] = (uint32_t)t;
-    __syncthreads();
-    if (tid == 0)
-      for (int x = 0; x < 16; ++x) carry += total[x];
-    __syncthreads();
+  for (int r = min(L, e.keep) + tid; r < e.keep; r += 256) kept[r] = NO_ROW;
+  if (L <= e.keep) {
+    for (int t = tid; t < L; t += 256) kept[t] = (uint32_t)t;
+    return;
   }
-  for (int r = min(L, e.keep) + tid; r < e.keep; r += 1024) kept[r] = NO_ROW;
-}
-
-void evict_select(hipStream_t st, const EvictSelect& e) {
-  hipLaunchKernelGGL(k_evict_select, dim3(e.H, e.B), dim3(1024), 0, st, e);
-}
-
-// One block per (head, sequence), 64 rows at a time: read, then written.  Kept
-// slots ascend, so a row moves to a place at or before its own and no write
-// reaches a row that a later step reads: in place is as good as to another cache.
-__global__ __launch_bounds__(256) void k_cache_move(CacheMove m) {
-  const int h = blockIdx.x, b = blockIdx.y, dh = m.dh;
-  const long bh = (long)b * m.H + h;
-  const uint32_t* idx = m.idx + b * m.idx_b + h * m.idx_h;
-  const int base = m.base ? m.base[b] : 0, rows = m.rows[b];
-  const double2* src[2] = {m.k + (bh * m.ctx + base) * dh, m.v + (bh * m.ctx + base) * dh};
-  double2* dst[2] = {m.ko + (bh * m.ctx_out + base) * dh, m.vo + (bh * m.ctx_out + base) * dh};
-  for (int r = 0; r < rows; ++r) {
-    const long s = idx[r];
-    double2 x[2];
-    double w = 0.0;
-    const int e = threadIdx.x;
-    if (e < dh)
-      for (int p = 0; p < 2; ++p) x[p] = src[p][s * dh + e];
-    if (e == 0 && m.w) w = m.w[bh * m.ctx + base + s];
+  const int lo = e.sinks, hi = L - e.recent, most = e.keep - e.sinks - e.recent;
+  const int nk = NK ? NK : (L + 255) / 256;
+  unsigned long long held[NK ? NK : 1];
+  // slots between the sinks and the recent rows; the others never count (0)
+  const auto load = [&](int k) {
+    const int t = 256 * k + tid;
+    return t >= lo && t < hi ? order_key(w[t]) : 0ull;
+  };
+  const auto key = [&](int k) { return NK ? held[NK ? k : 0] : load(k); };
+  if constexpr (NK > 0) {
+#pragma unroll
+    for (int k = 0; k < NK; ++k) held[k] = load(k);
+  }
+  int round = 0;
+  const auto count = [&](unsigned long long least) {  // keys >= least, in the whole block
+    int c = 0;
+#pragma unroll NK ? NK : 1
+    for (int k = 0; k < nk; ++k) c += __popcll(__ballot(key(k) >= least));
+    if (lane == 0) part[round & 1][wave] = c;
     __syncthreads();
-    if (e < dh)
-      for (int p = 0; p < 2; ++p) dst[p][(long)r * dh + e] = x[p];
-    if (e == 0 && m.w) m.wo[bh * m.ctx_out + base + r] = w;
+    c = part[round & 1][0] + part[round & 1][1] + part[round & 1][2] + part[round & 1][3];
+    ++round;
+    return c;
+  };
+  // count(>= low) >= most > count(>= high)
+  unsigned long long low = ~0ull, high = 0;
+#pragma unroll NK ? NK : 1
+  for (int k = 0; k < nk; ++k) {
+    const unsigned long long x = key(k);
+    if (x) low = min(low, x);
+    high = max(high, x);
+  }
+  for (int d = 32; d; d >>= 1) {
+    low = min(low, (unsigned long long)__shfl_xor((long long)low, d));
+    high = max(high, (unsigned long long)__shfl_xor((long long)high, d));
+  }
+  if (lane == 0) ext[0][wave] = low, ext[1][wave] = high;
+  __syncthreads();
+  low = min(min(ext[0][0], ext[0][1]), min(ext[0][2], ext[0][3]));
+  high = max(max(ext[1][0], ext[1][1]), max(ext[1][2], ext[1][3])) + 1;  // a key is below 2^64 - 1
+  int equal = 0;  // of the keys == low, how many stay
+  if (most == 0) {
+    low = ~0ull;
+  } else {
+    bool found = false;
+    while (high - low > 1) {
+      const unsigned long long mid = low + (high - low) / 2;
+      const int c = count(mid);
+      if (c >= most) low = mid;
+      else high = mid;
+      if (c == most) {
+        found = true;
+        break;
+      }
+    }
+    equal = found ? L : most - count(low + 1);
+  }
+  // places, 256 slots at a time
+  int before = 0, ties = 0;
+  __syncthreads();  // the last count has been read
+#pragma unroll NK ? NK : 1
+  for (int k = 0; k < nk; ++k) {
+    const int t = 256 * k + tid;
+    const unsigned long long x = key(k);
+    const unsigned long long eq = __ballot(x == low), below = (1ull << lane) - 1;
+    if (lane == 0) part[0][wave] = __popcll(eq);
+    __syncthreads();
+    int rank = ties + __popcll(eq & below);
+    for (int v = 0; v < wave; ++v) rank += part[0][v];
+    ties += part[0][0] + part[0][1] + part[0][2] + part[0][3];
+    const bool stay = t < L && (t < lo || t >= hi || x > low || (x == low && rank < equal));
+    const unsigned long long st = __ballot(stay);
+    if (lane == 0) part[1][wave] = __popcll(st);
+    __syncthreads();
+    int at = before + __popcll(st & below);
+    for (int v = 0; v < wave; ++v) at += part[1][v];
+    before += part[1][0] + part[1][1] + part[1][2] + part[1][3];
+    if (stay) kept[at] = (uint32_t)t;
+  }
+}
+
+// keys in registers up to the widest context of a layer (6144); the smallest
+// variant that holds the call's slots
+void evict_select(hipStream_t st, const EvictSelect& e) {
+  const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(e.H, e.B), dim3(256), 0, st, e); };
+  if (e.T_max <= 512) go(k_evict_select<2>);
+  else if (e.T_max <= 2048) go(k_evict_select<8>);
+  else if (e.T_max <= 6144) go(k_evict_select<24>);
+  else go(k_evict_select<0>);
+}
+
+constexpr int MV_PER = 8;  // 16-byte elements of a thread in flight
+__device__ __forceinline__ void st_stream(double2* p, double2 v) {
+  v2d x = {v.x, v.y};
+  __builtin_nontemporal_store(x, (MITOK_GLOBAL v2d*)p);
+}
+
+// To another cache: 256 * MV_PER elements of one (head, sequence)'s keys (y 0)
+// or values (y 1) per block, each read once and written once.
+__global__ __launch_bounds__(256) void k_cache_copy(CacheMove m, int parts) {
+  const int bh = blockIdx.x / parts, part = blockIdx.x % parts, b = bh / m.H, h = bh - b * m.H, dh = m.dh;
+  const int base = m.base ? m.base[b] : 0, rows = m.rows[b];
+  const uint32_t* idx = m.idx + b * m.idx_b + h * m.idx_h;
+  if (blockIdx.y == 2) {
+    for (int r = part * 256 + threadIdx.x; r < rows; r += parts * 256)
+      m.wo[(long)bh * m.ctx_out + base + r] = m.w[(long)bh * m.ctx + base + idx[r]];
+    return;
+  }
+  const double2* src = (blockIdx.y ? m.v : m.k) + ((long)bh * m.ctx + base) * dh;
+  double2* dst = (blockIdx.y ? m.vo : m.ko) + ((long)bh * m.ctx_out + base) * dh;
+  const long all = (long)rows * dh;
+  const long x0 = (long)part * (256 * MV_PER) + threadIdx.x;
+  if (x0 >= all) return;
+  int r = (int)(x0 / dh), e = (int)(x0 - (long)r * dh);
+  const int dr = 256 / dh, de = 256 - dr * dh;
+  double2 v[MV_PER];
+#pragma unroll
+  for (int k = 0; k < MV_PER; ++k) {
+    if (r < rows) v[k] = ld_stream(src + (long)idx[r] * dh + e);
+    r += dr;
+    e += de;
+    if (e >= dh) e -= dh, ++r;
+  }
+#pragma unroll
+  for (int k = 0; k < MV_PER; ++k)
+    if (x0 + 256 * k < all) st_stream(dst + x0 + 256 * k, v[k]);
+}
+
+// In place: a block moves one 8-wide slice of the columns (a cache line) of one
+// (head, sequence)'s keys or values, 32 * MV_PER rows at a time: all read, then
+// all written.  The slots ascend, so a row moves to a place at or before its
+// own, and no write reaches a row that a later step reads.
+__global__ __launch_bounds__(256) void k_cache_pack(CacheMove m, int slices) {
+  const int bh = blockIdx.x / slices, sl = blockIdx.x % slices, b = bh / m.H, h = bh - b * m.H, dh = m.dh;
+  const int base = m.base ? m.base[b] : 0, rows = m.rows[b];
+  const uint32_t* idx = m.idx + b * m.idx_b + h * m.idx_h;
+  if (blockIdx.y == 2) {
+    if (sl) return;
+    double* w = m.wo + (long)bh * m.ctx + base;
+    for (int r0 = 0; r0 < rows; r0 += 256) {
+      const int r = r0 + threadIdx.x;
+      const double x = r < rows ? w[idx[r]] : 0.0;
+      __syncthreads();
+      if (r < rows) w[r] = x;
+      __syncthreads();
+    }
+    return;
+  }
+  MITOK_GLOBAL v2d* at = (MITOK_GLOBAL v2d*)((blockIdx.y ? m.vo : m.ko) + ((long)bh * m.ctx + base) * dh);
+  const int e = sl * 8 + (threadIdx.x & 7), q = threadIdx.x >> 3;
+  const bool in = e < dh;
+  for (int r0 = 0; r0 < rows; r0 += 32 * MV_PER) {
+    v2d v[MV_PER];
+    unsigned move = 0;
+#pragma unroll
+    for (int k = 0; k < MV_PER; ++k) {
+      const int r = r0 + 32 * k + q;
+      const int from = r < rows ? (int)idx[r] : r;
+      v[k] = v2d{0.0, 0.0};
+      if (in && from != r) {
+        move |= 1u << k;
+        v[k] = at[(long)from * dh + e];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < MV_PER; ++k)
+      if (move >> k & 1) at[(long)(r0 + 32 * k + q) * dh + e] = v[k];
     __syncthreads();
   }
 }
 
 void cache_move(hipStream_t st, const CacheMove& m) {
   if (m.rows_max <= 0) return;
-  hipLaunchKernelGGL(k_cache_move, dim3(m.H, m.B), dim3(256), 0, st, m);
+  const unsigned y = m.w ? 3 : 2;
+  if (m.ko == m.k) {
+    const int slices = (m.dh + 7) / 8;
+    hipLaunchKernelGGL(k_cache_pack, dim3((unsigned)(m.B * m.H * slices), y), dim3(256), 0, st, m, slices);
+  } else {
+    const int parts = (int)(((long)m.rows_max * m.dh + 256 * MV_PER - 1) / (256 * MV_PER));
+    hipLaunchKernelGGL(k_cache_copy, dim3((unsigned)((long)m.B * m.H * parts), y), dim3(256), 0, st, m, parts);
+  }
 }
 
 __global__ void k_zero_weights(double* w, int H, long ctx, const int* from, const int* to) {
@@ -115,23 +248,32 @@ __device__ __forceinline__ void set_err(uint32_t* err, int word) {
   __hip_atomic_store(err + word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-constexpr int LR_CHUNK = 4096;
-int logit_chunks(int V) { return (V + LR_CHUNK - 1) / LR_CHUNK; }
+// tokens per block: 4096, or 1024 where that leaves most of the chip idle
+constexpr int LR_WIDE = 4096, LR_NARROW = 1024;
+int logit_chunks(int V) { return (V + LR_NARROW - 1) / LR_NARROW; }
 
-// One block per row, a chunk of the vocabulary at a time: the chunk's
-// occurrences in the history and its last bias entry are gathered in LDS
-// (integer atomics, so their order does not show), then its logits are read,
-// changed, written and compared.
-__global__ __launch_bounds__(256) void k_logit_rules(LogitRules r) {
-  __shared__ uint32_t count[LR_CHUNK], entry[LR_CHUNK];
+// One block per (chunk of the vocabulary, row).  Its logits are requested first;
+// the chunk's occurrences in the history and its last bias entry are gathered
+// in LDS meanwhile (integer atomics, so their order does not show); then each
+// logit is changed, written and compared, so it is read once and written once.
+// The row's last block joins the chunks' maxima.
+template <int CH>
+__global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
+  constexpr int PER = CH / 256;
+  __shared__ __align__(16) uint32_t count[CH], entry[CH];
+  __shared__ uint32_t words[CH / 32];
   __shared__ double sv[4];
   __shared__ int si[4];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = r.V;
+  const int row = row0 + blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = r.V;
+  const int c0 = blockIdx.x * CH, len = min(CH, V - c0);
   if (r.row_mask && !r.row_mask[row]) {
-    if (tid == 0 && r.ids) r.ids[row] = NO_TOKEN;
+    if (tid == 0 && c0 == 0 && r.ids) r.ids[row] = NO_TOKEN;
     return;
   }
-  const double* x = r.x + (long)row * V;
+  const double* x = r.x + (long)row * V + c0;
+  double y[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) y[k] = tid + 256 * k < len ? x[tid + 256 * k] : 0.0;
   double theta = 1.0, presence = 0.0, frequency = 0.0;
   if (r.penalties) {
     theta = r.penalties[3 * (long)row];
@@ -140,14 +282,15 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r) {
     if (tid == 0 && !(theta > 0.0 && isfinite(theta) && isfinite(presence) && isfinite(frequency)))
       set_err(r.err, OE_BAD_PENALTY);
   }
-  const int hist = r.penalties ? r.hist : 0;
-  double bv = -INFINITY;
-  int bi = -1;
-  for (int c0 = 0; c0 < V; c0 += LR_CHUNK) {
-    const int len = min(LR_CHUNK, V - c0);
-    for (int i = tid; i < len; i += 256) count[i] = entry[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < hist; i += 256) {
+  const bool ruled = r.hist > 0 || r.nb > 0;
+  if (ruled) {
+    for (int i = tid; i < CH / 4; i += 256) ((uint4*)count)[i] = ((uint4*)entry)[i] = make_uint4(0, 0, 0, 0);
+  }
+  if (r.allowed)
+    for (int i = tid; i < (len + 31) / 32; i += 256) words[i] = r.allowed[(long)row * ((V + 31) / 32) + c0 / 32 + i];
+  __syncthreads();
+  if (ruled) {
+    for (int i = tid; i < r.hist; i += 256) {
       const uint32_t t = r.history[(long)row * r.hist + i];
       if (t != NO_TOKEN && t >= (uint32_t)V) set_err(r.err, OE_BAD_TOKEN);
       if (t - (uint32_t)c0 < (uint32_t)len) atomicAdd(&count[t - c0], 1u);
@@ -158,36 +301,61 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r) {
       if (t - (uint32_t)c0 < (uint32_t)len) atomicMax(&entry[t - c0], (uint32_t)i + 1);
     }
     __syncthreads();
-    for (int i = tid; i < len; i += 256) {
-      const int t = c0 + i;
-      double y = x[t];
+  }
+  double bv = -INFINITY;
+  int bi = -1;
+  bool nan = false;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int i = tid + 256 * k;
+    if (i >= len) break;
+    if (ruled) {
       const uint32_t c = count[i], en = entry[i];
       if (c) {
-        y = y > 0.0 ? y / theta : y * theta;
-        y -= frequency * (double)c + presence;
+        y[k] = y[k] > 0.0 ? y[k] / theta : y[k] * theta;
+        y[k] -= frequency * (double)c + presence;
       }
-      if (en) y += r.bias[(long)row * r.nb + en - 1];
-      const bool ok = !r.allowed || (r.allowed[(long)row * ((V + 31) / 32) + (t >> 5)] >> (t & 31)) & 1;
-      if (!ok) y = -INFINITY;
-      if (r.out) r.out[(long)row * V + t] = y;
-      if (ok) {
-        if (isnan(y)) set_err(r.err, OE_NAN);
-        argmax_combine(bv, bi, y, t);
-      }
+      if (en) y[k] += r.bias[(long)row * r.nb + en - 1];
     }
-    __syncthreads();
+    const bool ok = !r.allowed || ((words[i >> 5] >> (i & 31)) & 1);
+    if (!ok) y[k] = -INFINITY;
+    nan |= isnan(y[k]);
+    argmax_combine(bv, bi, y[k], c0 + i);
+    if (r.out) __builtin_nontemporal_store(y[k], (MITOK_GLOBAL double*)(r.out + (long)row * V + c0 + i));
   }
+  if (__ballot(nan) && lane == 0) set_err(r.err, OE_NAN);
+  if (!r.ids) return;
   wave_argmax(bv, bi);
   if (lane == 0) sv[wave] = bv, si[wave] = bi;
   __syncthreads();
-  if (tid == 0 && r.ids) {
+  const int chunks = gridDim.x;
+  if (tid == 0) {
     for (int w = 1; w < 4; ++w) argmax_combine(bv, bi, sv[w], si[w]);
-    r.ids[row] = bv > -INFINITY ? (uint32_t)bi : NO_TOKEN;  // nothing allowed is above -inf
+    if (chunks == 1) r.ids[row] = bv > -INFINITY ? (uint32_t)bi : NO_TOKEN;  // nothing allowed is above -inf
+    else {
+      st_dev(r.part_v + (long)row * chunks + blockIdx.x, bv);
+      st_dev(r.part_i + (long)row * chunks + blockIdx.x, bi);
+    }
+  }
+  if (chunks == 1 || !arrive_last(r.counters + blockIdx.y, chunks)) return;
+  if (wave == 0) {
+    bv = -INFINITY;
+    bi = -1;
+    for (int c = lane; c < chunks; c += 64)
+      argmax_combine(bv, bi, ld_dev(r.part_v + (long)row * chunks + c), ld_dev(r.part_i + (long)row * chunks + c));
+    wave_argmax(bv, bi);
+    if (lane == 0) r.ids[row] = bv > -INFINITY ? (uint32_t)bi : NO_TOKEN;
   }
 }
 
 void logit_rules(hipStream_t st, const LogitRules& r) {
-  hipLaunchKernelGGL(k_logit_rules, dim3(r.rows), dim3(256), 0, st, r);
+  const bool wide = (long)((r.V + LR_WIDE - 1) / LR_WIDE) * r.rows >= 512;
+  const int chunks = wide ? (r.V + LR_WIDE - 1) / LR_WIDE : logit_chunks(r.V);
+  for (int row0 = 0; row0 < r.rows; row0 += 32768) {  // a counter per row of a launch
+    const dim3 grid(chunks, std::min(r.rows - row0, 32768));
+    if (wide) hipLaunchKernelGGL(k_logit_rules<LR_WIDE>, grid, dim3(256), 0, st, r, row0);
+    else hipLaunchKernelGGL(k_logit_rules<LR_NARROW>, grid, dim3(256), 0, st, r, row0);
+  }
 }
 
 }  // namespace mitok
