@@ -280,6 +280,13 @@ static WaveletTaps wavelet_taps(int S, int L, uint32_t mode) {
 
 enum RunMode { MODE_PREFILL = 0, MODE_CACHED = 1, MODE_STATELESS = 2 };
 
+// a drafted tree's pass: its lengths, ancestors and workspace, and for each
+// attention layer in order how its work is cut up
+struct TreePass {
+  TreeAttn a;
+  std::vector<TreePlan> plans;
+};
+
 struct Spec {
   int B = 0, S = 0;
   int mode = MODE_STATELESS;
@@ -303,7 +310,7 @@ struct Spec {
   int S_first = 0, T = 0;            // sizing: rows per sequence before the call's compressions (0: none
                                      // follow; S is the most they reach) and its target rows
   int ctx_bound = 0;                 // keys a decode step of this call can reach (0: the layers' context)
-  const TreeAttn* tree = nullptr;    // a drafted tree's rows on the cache: its lengths, ancestors and workspace
+  const TreePass* tree = nullptr;    // a drafted tree's rows on the cache
 };
 
 struct Timing {
@@ -791,6 +798,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
   const uint32_t* lens = sp.lens;
   const int* pos = sp.pos;
   size_t wi = 0;  // next wavelet stage
+  size_t ti = 0;  // next plan of a tree's pass
   bool real = false;  // the rows in cur have zero imaginary parts: a Norm leaves Re(x) + 0i (norm_layer.rs:64-130)
   // a pass that backward may differentiate leaves every layer's input in that
   // layer's own buffer; another alternates between two
@@ -904,7 +912,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
         a.dh = dh;
         a.scale = 1.0 / (1e-8 + sqrt((double)dh));  // scale_attention_scores (masked_attention_head.rs:453-465)
         if (sp.tree) {
-          TreeAttn t = *sp.tree;
+          TreeAttn t = sp.tree->a;
           t.q = q;
           t.ldq = t.ldo = d;
           t.kc = e.kc;
@@ -919,7 +927,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
           t.out = cat;
           {
             TimeScope ts(n, MITOK_TIME_ATTENTION, 0.0);
-            tree_attention(st, t);
+            tree_attention(st, t, sp.tree->plans[ti++]);
           }
           layernorm(st, cat, cur, nxt, rows, d, A->eps, A->gamma.as<double2>(), A->beta.as<double2>());
         } else if (sp.mode == MODE_CACHED && S == 1) {
@@ -3714,32 +3722,48 @@ static int check_tree(const uint32_t* parents, const uint32_t* counts, uint32_t 
   return OK;
 }
 
-// Lengths, counts, depths and ancestor bits of a call's trees, staged and
-// uploaded to op_tab; fills a's pointers and sizes.  *depth: the nodes' depths
-// [B][nodes] in the staging.
+// Lengths, counts, depths, ancestor bits and the plans of `layers` (heads and
+// head dims; one plan each, in order), staged and uploaded to op_tab; fills
+// the pass's pointers and sizes and reserves its workspace.  *depth: the nodes'
+// depths [B][nodes] in the staging.
 static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, const uint32_t* counts, uint32_t B,
-                      uint32_t nodes, TreeAttn& a, const int** depth = nullptr) {
+                      uint32_t nodes, uint32_t weigh, const std::vector<std::pair<int, int>>& layers, TreePass& pass,
+                      const int** depth = nullptr) {
   const int words = (int)(nodes + 63) / 64;
   const size_t bn = (size_t)B * nodes;
+  std::vector<int> kv(kv_lens, kv_lens + B), cnt(B), lists;
+  for (uint32_t b = 0; b < B; ++b) cnt[b] = (int)(counts ? counts[b] : nodes);
+  TreeAttn& a = pass.a;
+  a.B = (int)B;
+  a.n = (int)nodes;
+  a.weigh = (int)weigh;
+  pass.plans.clear();
+  size_t ws = 0;
+  for (size_t k = 0; k < layers.size(); ++k) {
+    a.H = layers[k].first;
+    a.dh = layers[k].second;
+    const size_t same = std::find(layers.begin(), layers.end(), layers[k]) - layers.begin();
+    pass.plans.push_back(same < k ? pass.plans[same] : tree_plan(a, kv.data(), cnt.data(), lists));
+    ws = std::max(ws, tree_ws_bytes(a, pass.plans.back()));
+  }
+  TRY(alloc(n, n->op_ws, ws));
+  a.ws = n->op_ws.p;
   const size_t seen_b = bn * words * sizeof(unsigned long long);
-  const size_t bytes = seen_b + (2 * (size_t)B + bn) * sizeof(int);
+  const size_t lists_at = (seen_b + (2 * (size_t)B + bn) * sizeof(int) + 15) & ~(size_t)15;
+  const size_t bytes = lists_at + lists.size() * sizeof(int);
   TRY(op_staging(n, bytes));
   auto* seen = (unsigned long long*)n->op_host;
-  int* kv = (int*)(n->op_host + seen_b);
-  int* cnt = kv + B;
-  int* dep = cnt + B;
+  int* dep = (int*)(n->op_host + seen_b) + 2 * B;
   memset(seen, 0, seen_b);
-  a.T_max = 0;
-  for (uint32_t b = 0; b < B; ++b) {
-    const uint32_t c = counts ? counts[b] : nodes;
-    kv[b] = (int)kv_lens[b];
-    cnt[b] = (int)c;
-    a.T_max = std::max(a.T_max, kv[b] + cnt[b]);
+  memcpy(n->op_host + seen_b, kv.data(), B * sizeof(int));
+  memcpy(n->op_host + seen_b + B * sizeof(int), cnt.data(), B * sizeof(int));
+  memcpy(n->op_host + lists_at, lists.data(), lists.size() * sizeof(int));
+  for (uint32_t b = 0; b < B; ++b)
     for (uint32_t i = 0; i < nodes; ++i) {
       unsigned long long* s = seen + ((size_t)b * nodes + i) * words;
       int& d = dep[(size_t)b * nodes + i];
       d = 0;
-      if (i >= c) continue;
+      if ((int)i >= cnt[b]) continue;
       const uint32_t p = parents[(size_t)b * nodes + i];
       if (p != MITOK_NO_PARENT) {
         memcpy(s, seen + ((size_t)b * nodes + p) * words, words * sizeof(*s));
@@ -3747,7 +3771,6 @@ static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, 
       }
       s[i >> 6] |= 1ull << (i & 63);
     }
-  }
   if (depth) *depth = dep;
   TRY(op_upload(n, bytes));
   const char* t = (const char*)n->op_tab.p;
@@ -3756,8 +3779,10 @@ static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, 
   a.kv_len = (const int*)(t + seen_b);
   a.count = a.kv_len + B;
   a.depth = a.count + B;
-  a.B = (int)B;
-  a.n = (int)nodes;
+  for (TreePlan& p : pass.plans) {
+    p.chunks = (const int4*)(t + lists_at) + p.at / 4;
+    p.splits = (const int*)(p.chunks + p.entries);
+  }
   return OK;
 }
 
@@ -3797,25 +3822,21 @@ int mitok_tree_attention_device(mitok_network* n, const double* d_q, const doubl
   const Span w = {weigh_nodes ? d_weights : nullptr, wb, "weights"}, o = {d_out, qb, "out"};
   TRY(check_apart(o, {q, k, v, bi, w}));
   TRY(check_apart(w, {q, k, v, bi}));
-  TreeAttn a;
+  TreePass pass;
+  TreeAttn& a = pass.a;
   a.q = (const double2*)d_q;
   a.ldq = a.ldo = (long)heads * dh;
   a.kc = (const double2*)d_k;
   a.vc = (const double2*)d_v;
   a.bias = d_bias;
   a.bias_stride = (long)bias_stride;
-  a.H = (int)heads;
-  a.dh = (int)dh;
   a.ctx = (int)ctx;
   a.scale = 1.0 / (1e-8 + sqrt((double)dh));  // as the layers' (masked_attention_head.rs:453-465)
-  a.weigh = (int)weigh_nodes;
   a.weights = weigh_nodes ? d_weights : nullptr;
   a.out = (double2*)d_out;
   TRY(behind_default_stream(n));
-  TRY(stage_tree(n, kv_lens, parents, counts, B, nodes, a));
-  TRY(alloc(n, n->op_ws, tree_ws_bytes(a)));
-  a.ws = n->op_ws.p;
-  tree_attention(n->stream, a);
+  TRY(stage_tree(n, kv_lens, parents, counts, B, nodes, weigh_nodes, {{(int)heads, (int)dh}}, pass));
+  tree_attention(n->stream, a, pass.plans[0]);
   return op_finish(n);
 }
 
@@ -3834,7 +3855,7 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
   TRY(stage_rules(n, (uint32_t)rows, V));
   TRY(alloc(n, n->tree_ids, rows * sizeof(uint32_t)));
   TRY(alloc(n, n->tree_rng, 2 * (size_t)B * sizeof(int)));
-  TreeAttn tree;
+  TreePass tree;
   const int* depth = nullptr;
   // the rows whose weights are kept so far, zero for those appended since
   std::vector<int> from(B), to(B);
@@ -3851,19 +3872,13 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
       most = std::max(most, to[b] - from[b]);
     }
   }
-  size_t ws = 0;
+  std::vector<std::pair<int, int>> shapes;
   for (auto& L : n->layers)
     if (L->kind == K_SELF_ATTENTION) {
       auto* A = (SelfAttentionLayer*)L.get();
-      TreeAttn t;
-      t.B = (int)B, t.n = (int)nodes, t.H = (int)A->heads, t.dh = (int)A->dh, t.weigh = (int)weigh;
-      t.T_max = (int)A->max_ctx;
-      ws = std::max(ws, tree_ws_bytes(t));
+      shapes.push_back({(int)A->heads, (int)A->dh});
     }
-  TRY(alloc(n, n->op_ws, ws));
-  TRY(stage_tree(n, n->kv_len_h.data(), parents, counts, B, nodes, tree, &depth));
-  tree.ws = n->op_ws.p;
-  tree.weigh = (int)weigh;
+  TRY(stage_tree(n, n->kv_len_h.data(), parents, counts, B, nodes, weigh, shapes, tree, &depth));
   std::vector<uint32_t> padded(rows), mask(rows);
   std::vector<int> pos(rows);
   int maxpos = 0;

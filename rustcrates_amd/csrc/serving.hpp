@@ -6,6 +6,8 @@
 // nor allocates.
 #pragma once
 
+#include <vector>
+
 #include "kernels.hpp"
 
 namespace mitok {
@@ -39,7 +41,6 @@ struct TreeAttn {
   const unsigned long long* seen = nullptr;  // [B][n][words]: bit j of a node: itself or an ancestor
   int words = 1;
   int B = 0, n = 0, H = 0, dh = 0, ctx = 0;
-  int T_max = 0;  // the largest kv_len + count (sizing)
   double scale = 1.0;
   int weigh = 0;
   double* weights = nullptr;  // [B][H][ctx]
@@ -47,8 +48,21 @@ struct TreeAttn {
   long ldo = 0;
   void* ws = nullptr;  // tree_ws_bytes
 };
-size_t tree_ws_bytes(const TreeAttn& a);
-void tree_attention(hipStream_t st, const TreeAttn& a);
+// How a call's work is cut up, from its lengths (host arrays): each sequence's
+// slots in chunks, the longest first.  The lists are appended to `table`;
+// chunks and splits are set to them once they are on the device.
+struct TreePlan {
+  int ng = 1;      // groups of 16 nodes per block
+  int entries = 0; // chunks of all sequences
+  int nsplit = 1;  // the most of one sequence
+  int T = 0;       // the most slots of one sequence
+  size_t at = 0;   // first word of the lists in the table
+  const int4* chunks = nullptr;  // [entries]: sequence, first slot, end, index in the sequence
+  const int* splits = nullptr;   // [B] chunks of each sequence
+};
+TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& table);
+size_t tree_ws_bytes(const TreeAttn& a, const TreePlan& p);
+void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p);
 
 // ---- rows of a cache moved to its front, or to another cache's ----
 struct CacheMove {

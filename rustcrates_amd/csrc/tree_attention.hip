@@ -24,99 +24,88 @@
 // by their maxima.
 // D[i][j] of a 16x16 tile sits at lane j + 16 * (i % 4), element i / 4.
 #include <algorithm>
+#include <cmath>
 
 #include "serving.hpp"
 
 namespace mitok {
 
-// chunk partials: max and sum of (row of the workspace, node), and the
-// unnormalised output; scores of the weighed nodes [B][H][T][weigh]
+// chunk partials: max, sum and unnormalised output of a node, and the scores
+// of the weighed nodes
 struct TreeWs {
-  double* m = nullptr;  // [B][H][n][nsplit]
+  double* m = nullptr;   // [B][H][n][nsplit]
   double* l = nullptr;
   double2* o = nullptr;  // [B][H][n][nsplit][dh] (nsplit > 1)
   double* x = nullptr;   // [B][H][T][weigh]
 };
-struct TreePlan {
-  int ng = 1, nsplit = 1, ch = 64, T = 0;
-  TreeWs ws;
+
+// A block's place: chunk entry * H + head, and its first node.
+struct TreeAt {
+  int b, h, bh, L, cnt, t0, t1, s, n0;
+  __device__ __forceinline__ TreeAt(const TreeAttn& a, const TreePlan& p, int nodes) {
+    const int e = blockIdx.x / a.H;
+    const int4 c = p.chunks[e];
+    b = c.x, t0 = c.y, t1 = c.z, s = c.w;
+    h = blockIdx.x - e * a.H;
+    bh = b * a.H + h;
+    L = a.kv_len[b];
+    cnt = a.count[b];
+    n0 = blockIdx.y * nodes;
+  }
+  // rows of nodes [n0, n0 + nodes) that are not used: zero, by the sequence's first chunk
+  __device__ __forceinline__ void clear(const TreeAttn& a, int nodes) const {
+    if (s) return;
+    const int from = max(n0, cnt), rows = min(n0 + nodes, a.n) - from;
+    for (int x = threadIdx.x; x < rows * a.dh; x += 256)
+      a.out[((long)b * a.n + from + x / a.dh) * a.ldo + (long)h * a.dh + x % a.dh] = make_double2(0.0, 0.0);
+  }
 };
 
-template <int DHP, int NG, bool FULL>
-__global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p) {
-  constexpr int KG = 4 / NG;    // waves that share a node group's slots
-  constexpr int U = DHP / 4;    // 16-byte key loads of a lane per tile, two MFMAs each
-  constexpr int CT = DHP / 16;  // 16-column tiles of the values
-  constexpr bool PRE = DHP <= 64;  // the next tile's rows wait in registers
-  constexpr int OSTR = DHP + 1;    // LDS row of a node's output: nodes in different banks
-  constexpr size_t Q_BYTES = (size_t)NG * U * 64 * sizeof(double2), O_BYTES = (size_t)NG * 16 * OSTR * sizeof(double2);
-  __shared__ __align__(16) unsigned char lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
-  __shared__ double sm[4][16], sl[4][16];
-  double2* qs = (double2*)lds;  // [NG][U][64], then the merged outputs [NG * 16][OSTR]
-  double2* os = (double2*)lds;
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ng = wave % NG, kg = wave / NG;
-  const int node = lane & 15, kq = lane >> 4;
-  const int chunk = blockIdx.x % p.nsplit, bh = blockIdx.x / p.nsplit, b = bh / a.H, h = bh - b * a.H;
-  const int n0 = blockIdx.y * 16 * NG, dh = a.dh;
-  const int L = a.kv_len[b], cnt = a.count[b], T = cnt ? L + cnt : 0;
-  const int t0 = chunk * p.ch, t1 = min(T, t0 + p.ch);
-  if (n0 >= cnt || t0 >= T) {
-    // unused nodes give zero; a chunk past the sequence leaves nothing to join
-    if (chunk == 0)
-      for (int x = tid; x < 16 * NG * dh; x += 256) {
-        const int i = n0 + x / dh, e = x % dh;
-        if (i < a.n && i >= cnt) a.out[((long)b * a.n + i) * a.ldo + (long)h * dh + e] = make_double2(0.0, 0.0);
-      }
-    return;
+// Bits e of a tile's slots t + 4 e + kq that node i sees; a tile of committed slots: all
+__device__ __forceinline__ unsigned tree_sees(const TreeAttn& a, const TreeAt& at, int t, int kq, int i) {
+  if (t + 16 <= at.L) return 15u;
+  unsigned vis = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int j = t + 4 * e + kq - at.L;
+    bool see = j < 0;
+    if (j >= 0 && j < at.cnt && i < at.cnt) see = (a.seen[((long)at.b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1;
+    if (see) vis |= 1u << e;
   }
-  const double2* K = a.kc + (long)bh * a.ctx * dh;
-  const double2* V = a.vc + (long)bh * a.ctx * dh;
-  const double* bias = a.bias ? a.bias + (long)h * a.bias_stride : nullptr;
-  const int i = n0 + 16 * ng + node;  // this lane's node
-
-  for (int x = tid; x < NG * U * 64; x += 256) {
-    const int ln = x & 63, u = (x >> 6) % U, g = x / (64 * U);
-    const int r = n0 + 16 * g + (ln & 15), e = 4 * u + (ln >> 4);
-    double2 q = make_double2(0.0, 0.0);
-    if (r < cnt && e < dh) q = a.q[((long)b * a.n + r) * a.ldq + (long)h * dh + e];
-    qs[x] = make_double2(q.x * a.scale, -q.y * a.scale);
+  return vis;
+}
+// the biases of slots t + 4 e + kq
+__device__ __forceinline__ void tree_bias(const TreeAttn& a, const TreeAt& at, int t, int kq, double (&bf)[4]) {
+  if (!a.bias) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    int col = min(t + 4 * e + kq, at.t1 - 1);
+    if (t + 16 > at.L && col >= at.L) col = at.L + a.depth[(long)at.b * a.n + col - at.L];
+    bf[e] = a.bias[(long)at.h * a.bias_stride + col];
   }
-  __syncthreads();
-  const double2* qw = qs + ng * U * 64 + lane;
+}
+// the weighed nodes' scores, [slot][node]
+__device__ __forceinline__ void tree_scores(const TreeAttn& a, const TreePlan& p, const TreeWs& ws, const TreeAt& at,
+                                            int t, int kq, int i, const v4d& s) {
+  if (i >= a.weigh) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (t + 4 * e + kq < at.t1) ws.x[((long)at.bh * p.T + t + 4 * e + kq) * a.weigh + i] = s[e];
+}
 
+// One wave's running softmax over 16-slot tiles for the node lane % 16, and
+// its output (column 16 c + 4 e + lane / 16).
+template <int DHP>
+struct TreeRun {
+  static constexpr int CT = DHP / 16;
   v4d o_re[CT], o_im[CT];
-  double m = -INFINITY, l = 0.0;  // of this lane's node; l over this lane's slots alone
+  double m = -INFINITY, l = 0.0;  // l over this lane's slots alone
+  __device__ __forceinline__ TreeRun() {
 #pragma unroll
-  for (int c = 0; c < CT; ++c) o_re[c] = o_im[c] = v4d{0.0, 0.0, 0.0, 0.0};
-
-  // a tile's key row of this lane and its value rows 4 q + kq; a row past
-  // `end` is row end - 1, with weight 0.  Padded columns: keys of 0 (0 times an
-  // infinity would be NaN), and value columns that nobody reads.
-  const auto key_at = [&](int t, int u, int end) {
-    const uint32_t at = (uint32_t)min(node, end - 1 - t) * (uint32_t)dh + kq;
-    if (!FULL && 4 * u + kq >= dh) return make_double2(0.0, 0.0);
-    return ld_glb(K + (long)t * dh + at + 4 * u);
-  };
-  const auto value_at = [&](int t, int q, int c, int end) {
-    const uint32_t at = (uint32_t)min(4 * q + kq, end - 1 - t) * (uint32_t)dh;
-    if (FULL) return ld_glb(V + (long)t * dh + (at + node) + 16 * c);
-    return ld_glb(V + (long)t * dh + (at + (uint32_t)min(node + 16 * c, dh - 1)));
-  };
-  const auto score = [&](v4d& s, int u, double2 k) {
-    const double2 q = qw[u * 64];
-    s = __builtin_amdgcn_mfma_f64_16x16x4f64(k.x, q.x, s, 0, 0, 0);
-    s = __builtin_amdgcn_mfma_f64_16x16x4f64(k.y, q.y, s, 0, 0, 0);
-  };
-  const auto keep_scores = [&](const v4d& s, int t, int end) {
-    if (i >= a.weigh) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (t + 4 * e + kq < end) p.ws.x[((long)bh * p.T + t + 4 * e + kq) * a.weigh + i] = s[e];
-  };
-  // the running maximum and sum take a tile's scores, which become its weights
-  const auto soften = [&](v4d& s) {
+    for (int c = 0; c < CT; ++c) o_re[c] = o_im[c] = v4d{0.0, 0.0, 0.0, 0.0};
+  }
+  // a tile's scores become its weights
+  __device__ __forceinline__ void soften(v4d& s) {
     double x, y;
     pair16_f64(fmax(fmax(s[0], s[1]), fmax(s[2], s[3])), x, y);
     pair32_f64(fmax(x, y), x, y);
@@ -133,121 +122,170 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
     l = l * keep + ls;
 #pragma unroll
     for (int c = 0; c < CT; ++c) o_re[c] *= keep, o_im[c] *= keep;
-  };
-  const auto output = [&](const v4d& s, int q, int c, double2 v) {
+  }
+  __device__ __forceinline__ void output(const v4d& s, int q, int c, double2 v) {
     o_re[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(v.x, s[q], o_re[c], 0, 0, 0);
     o_im[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(v.y, s[q], o_im[c], 0, 0, 0);
-  };
-
-  // committed slots: every node sees them
-  const int tc = min(t1, L);
-  {
-    double2 kf[PRE ? U : 1], vf[PRE ? 4 : 1][PRE ? CT : 1];
-    double bf[4] = {0.0, 0.0, 0.0, 0.0};
-    const auto load_keys = [&](int t) {
-      if constexpr (PRE) {
+  }
+  // Values that are not finite are left out of a tile's products, where 0 times
+  // them is NaN in the rows of nodes that do not see them, and added here to
+  // those that do, slot by slot.
+  __device__ __forceinline__ void add_left_out(const TreeAt& at, const double2* V, int dh, int t, const v4d& s, unsigned vis) {
+    const int lane = threadIdx.x & 63, node = lane & 15, kq = lane >> 4;
+    for (int k = 0; k < 16 && t + k < at.t1; ++k) {
+      const int from = node + 16 * (k & 3), q = k >> 2;
+      const double pk = __shfl(q == 0 ? s[0] : q == 1 ? s[1] : q == 2 ? s[2] : s[3], from);
+      const bool see = (__shfl((int)vis, from) >> q) & 1;
 #pragma unroll
-        for (int u = 0; u < U; ++u) kf[u] = key_at(t, u, tc);
-      }
-      if (bias) {
+      for (int c = 0; c < CT; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) bf[e] = bias[min(t + 4 * e + kq, tc - 1)];
-      }
-    };
-    const auto load_values = [&](int t) {
-      if constexpr (PRE) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int c = 0; c < CT; ++c) vf[q][c] = value_at(t, q, c, tc);
-      }
-    };
-    int t = t0 + 16 * kg;
-    if (t < tc) {
-      load_keys(t);
-      load_values(t);
-    }
-    for (; t < tc; t += 16 * KG) {
-      v4d s = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        score(s, u, PRE ? kf[PRE ? u : 0] : key_at(t, u, tc));
-        if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four queries at a time in registers
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = t + 4 * e + kq < tc ? s[e] + bf[e] : -INFINITY;
-      keep_scores(s, t, tc);
-      const bool more = t + 16 * KG < tc;
-      if (more || !PRE) load_keys(t + (more ? 16 * KG : 0));
-      soften(s);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-#pragma unroll
-        for (int c = 0; c < CT; ++c) output(s, q, c, PRE ? vf[PRE ? q : 0][PRE ? c : 0] : value_at(t, q, c, tc));
-        if (!PRE) __builtin_amdgcn_sched_barrier(0);
-      }
-      if (more) load_values(t + 16 * KG);
+        for (int e = 0; e < 4; ++e) {
+          const int col = 16 * c + 4 * e + kq;
+          if (see && col < dh) {
+            const double2 v = V[(long)(t + k) * dh + col];
+            if (!isfinite(v.x)) o_re[c][e] += pk * v.x;
+            if (!isfinite(v.y)) o_im[c][e] += pk * v.y;
+          }
+        }
     }
   }
+};
+__device__ __forceinline__ bool tree_finite(double2& v) {  // what is not finite becomes 0
+  const bool nx = !isfinite(v.x), ny = !isfinite(v.y);
+  if (nx) v.x = 0.0;
+  if (ny) v.y = 0.0;
+  return !(nx || ny);
+}
 
-  // the nodes' own slots: a node sees its ancestors and itself
-  for (int t = max(t0, L) + 16 * kg; t < t1; t += 16 * KG) {
-    v4d s = {0.0, 0.0, 0.0, 0.0};
+// A node's output row element: final where the sequence has one chunk, else the chunk's part.
+__device__ __forceinline__ void tree_put(const TreeAttn& a, const TreePlan& p, const TreeWs& ws, const TreeAt& at, int k,
+                                         int e, double2 v, double sum) {
+  if (p.nsplit == 1) a.out[((long)at.b * a.n + k) * a.ldo + (long)at.h * a.dh + e] = make_double2(v.x / sum, v.y / sum);
+  else ws.o[(((long)at.bh * a.n + k) * p.nsplit + at.s) * a.dh + e] = v;
+}
+__device__ __forceinline__ void tree_put_sum(const TreeAttn& a, const TreePlan& p, const TreeWs& ws, const TreeAt& at,
+                                             int i, double m, double l) {
+  if (i >= at.cnt || (p.nsplit == 1 && i >= a.weigh)) return;
+  const long x = ((long)at.bh * a.n + i) * p.nsplit + at.s;
+  ws.m[x] = m;
+  ws.l[x] = l;
+}
+
+template <int DHP, int NG, bool FULL>
+__global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p, TreeWs ws) {
+  constexpr int KG = 4 / NG;       // waves that share a node group's slots
+  constexpr int U = DHP / 4;       // 16-byte key loads of a lane per tile, two MFMAs each
+  constexpr int CT = DHP / 16;     // 16-column tiles of the values
+  constexpr bool PRE = DHP <= 64;  // the next tile's rows wait in registers
+  constexpr int OSTR = DHP + 1;    // LDS row of a node's output: nodes in different banks
+  constexpr int PARTS = DHP <= 64 ? KG : 1;  // LDS holds this many waves' outputs of each node group
+  constexpr size_t Q_BYTES = (size_t)NG * U * 64 * sizeof(double2);
+  constexpr size_t O_BYTES = (size_t)PARTS * NG * 16 * OSTR * sizeof(double2);
+  __shared__ __align__(16) unsigned char lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
+  __shared__ double sm[4][16], sl[4][16], sum[NG][16];
+  double2* qs = (double2*)lds;  // [NG][U][64], then outputs [PARTS][NG * 16][OSTR]
+  double2* os = (double2*)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ng = wave % NG, kg = wave / NG;
+  const int node = lane & 15, kq = lane >> 4, dh = a.dh;
+  const TreeAt at(a, p, 16 * NG);
+  at.clear(a, 16 * NG);
+  if (at.n0 >= at.cnt) return;
+  const int t0 = at.t0, t1 = at.t1;
+  const double2* K = a.kc + (long)at.bh * a.ctx * dh;
+  const double2* V = a.vc + (long)at.bh * a.ctx * dh;
+  const int i = at.n0 + 16 * ng + node;  // this lane's node
+  const double2* qw = qs + ng * U * 64 + lane;
+
+  // a tile's key row of this lane and its value rows 4 q + kq; a slot past the
+  // end reads the last one's, with weight 0.  Padded columns: keys of 0 (0 times
+  // an infinity would be NaN), and value columns that nobody reads.
+  const auto key_at = [&](int t, int u) {
+    const uint32_t x = (uint32_t)min(node, t1 - 1 - t) * (uint32_t)dh + kq;
+    if (!FULL && 4 * u + kq >= dh) return make_double2(0.0, 0.0);
+    return ld_glb(K + (long)t * dh + x + 4 * u);
+  };
+  const auto value_at = [&](int t, int q, int c) {
+    const uint32_t x = (uint32_t)min(4 * q + kq, t1 - 1 - t) * (uint32_t)dh;
+    if (FULL) return ld_glb(V + (long)t * dh + (x + node) + 16 * c);
+    return ld_glb(V + (long)t * dh + (x + (uint32_t)min(node + 16 * c, dh - 1)));
+  };
+  double2 kf[PRE ? U : 1], vf[PRE ? 4 : 1][PRE ? CT : 1];
+  double bf[4] = {0.0, 0.0, 0.0, 0.0};
+  const auto load_keys = [&](int t) {
+    if constexpr (PRE) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) kf[u] = key_at(t, u);
+    }
+    tree_bias(a, at, t, kq, bf);
+  };
+  const auto load_values = [&](int t) {
+    if constexpr (PRE) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) vf[q][c] = value_at(t, q, c);
+    }
+  };
+  int t = t0 + 16 * kg;
+  if (t < t1) {
+    load_keys(t);
+    load_values(t);
+  }
+  // the queries, behind the first tile's loads
+  for (int x = tid; x < NG * U * 64; x += 256) {
+    const int ln = x & 63, u = (x >> 6) % U, g = x / (64 * U);
+    const int r = at.n0 + 16 * g + (ln & 15), e = 4 * u + (ln >> 4);
+    double2 q = make_double2(0.0, 0.0);
+    if (r < at.cnt && e < dh) q = a.q[((long)at.b * a.n + r) * a.ldq + (long)at.h * dh + e];
+    qs[x] = make_double2(q.x * a.scale, -q.y * a.scale);
+  }
+  __syncthreads();
+
+  TreeRun<DHP> run;
+  for (; t < t1; t += 16 * KG) {
+    v4d s = {0.0, 0.0, 0.0, 0.0}, z = s;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      score(s, u, key_at(t, u, t1));
-      if (u % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+      const double2 k = PRE ? kf[PRE ? u : 0] : key_at(t, u), q = qw[u * 64];
+      s = __builtin_amdgcn_mfma_f64_16x16x4f64(k.x, q.x, s, 0, 0, 0);
+      z = __builtin_amdgcn_mfma_f64_16x16x4f64(k.y, q.y, z, 0, 0, 0);
+      if (u % (PRE ? 4 : 16) == (PRE ? 3 : 15)) __builtin_amdgcn_sched_barrier(0);  // so many operands at a time in registers
     }
-    unsigned vis = 0;  // bit e: slot t + 4 e + kq is seen by this lane's node
+    const unsigned vis = tree_sees(a, at, t, kq, i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int j = t + 4 * e + kq - L;
-      const bool see = j < t1 - L && i < cnt && ((a.seen[((long)b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1);
-      if (see) vis |= 1u << e;
-      if (see && bias) s[e] += bias[L + a.depth[(long)b * a.n + j]];
-      if (!see) s[e] = -INFINITY;
+    for (int e = 0; e < 4; ++e) s[e] = (vis >> e & 1) && t + 4 * e + kq < t1 ? s[e] + z[e] + bf[e] : -INFINITY;
+    tree_scores(a, p, ws, at, t, kq, i, s);
+    const bool more = t + 16 * KG < t1;
+    if (more) load_keys(t + 16 * KG);
+    run.soften(s);
+    const bool drafted = t + 16 > at.L;
+    bool fine = true;
+    if (PRE && drafted) {
+#pragma unroll
+      for (int q = 0; q < (PRE ? 4 : 0); ++q)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) fine &= tree_finite(vf[q][c]);
     }
-    keep_scores(s, t, t1);
-    soften(s);
-    // values that are not finite are left out of the products, where 0 times
-    // them is NaN in the rows of the nodes that do not see them ...
-    bool bad = false;
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < 4; ++q) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        double2 v = value_at(t, q, c, t1);
-        const bool nx = !isfinite(v.x), ny = !isfinite(v.y);
-        bad |= nx || ny;
-        if (nx) v.x = 0.0;
-        if (ny) v.y = 0.0;
-        output(s, q, c, v);
-        if (c % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        double2 v = PRE ? vf[PRE ? q : 0][PRE ? c : 0] : value_at(t, q, c);
+        if (!PRE && drafted) fine &= tree_finite(v);
+        run.output(s, q, c, v);
       }
-    // ... and added to the others: output column 16 c + 4 e + kq, slot by slot
-    if (__ballot(bad)) {
-      for (int k = 0; k < 16 && t + k < t1; ++k) {
-        const int from = node + 16 * (k & 3), q = k >> 2;
-        const double pk = __shfl(q == 0 ? s[0] : q == 1 ? s[1] : q == 2 ? s[2] : s[3], from);
-        const bool see = (__shfl((int)vis, from) >> q) & 1;
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = 16 * c + 4 * e + kq;
-            if (see && col < dh) {
-              const double2 v = V[(long)(t + k) * dh + col];
-              if (!isfinite(v.x)) o_re[c][e] += pk * v.x;
-              if (!isfinite(v.y)) o_im[c][e] += pk * v.y;
-            }
-          }
-      }
+      if (!PRE) __builtin_amdgcn_sched_barrier(0);
     }
+    if (more) load_values(t + 16 * KG);
+    if (__ballot(!fine)) run.add_left_out(at, V, dh, t, s, vis);
   }
 
   // the waves of a node group, rescaled to their common maximum and added in order
-  l = xor32_sum(xor16_sum(l));
-  if (kq == 0) sm[wave][node] = m, sl[wave][node] = l;
+  run.l = xor32_sum(xor16_sum(run.l));
+  if (kq == 0) sm[wave][node] = run.m, sl[wave][node] = run.l;
   __syncthreads();  // and the queries' last read
   double M = -INFINITY;
 #pragma unroll
@@ -256,128 +294,283 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
   double Ls = 0.0;
 #pragma unroll
   for (int g = 0; g < KG; ++g) Ls += sl[g * NG + ng][node] * exp(sm[g * NG + ng][node] - base);
-  const double f = exp(m - base);
+  const double f = exp(run.m - base);
 #pragma unroll
-  for (int g = 0; g < KG; ++g) {
-    if (kg == g) {
+  for (int g = 0; g < KG; g += PARTS) {
+    if (kg / PARTS * PARTS == g && i < at.cnt) {
 #pragma unroll
       for (int c = 0; c < CT; ++c)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          double2* at = os + (16 * ng + node) * OSTR + 16 * c + 4 * e + kq;
-          const double2 v = make_double2(o_re[c][e] * f, o_im[c][e] * f);
-          *at = g ? cadd(*at, v) : v;
+          double2* to = os + ((kg - g) * NG * 16 + 16 * ng + node) * OSTR + 16 * c + 4 * e + kq;
+          const double2 v = make_double2(run.o_re[c][e] * f, run.o_im[c][e] * f);
+          *to = g ? cadd(*to, v) : v;
         }
     }
     __syncthreads();
   }
   if (kg == 0 && kq == 0) {
-    sl[ng][node] = Ls;
-    if (i < cnt && (p.nsplit > 1 || i < a.weigh)) {
-      const long at = ((long)bh * a.n + i) * p.nsplit + chunk;
-      p.ws.m[at] = M;
-      p.ws.l[at] = Ls;
-    }
+    sum[ng][node] = Ls;
+    tree_put_sum(a, p, ws, at, i, M, Ls);
   }
   __syncthreads();
-  for (int x = tid; x < 16 * NG * dh; x += 256) {
-    const int r = x / dh, e = x - r * dh, k = n0 + r;
-    if (k >= a.n) break;
-    const double2 v = os[r * OSTR + e];
-    if (p.nsplit == 1) {
-      const double w = sl[r >> 4][r & 15];
-      a.out[((long)b * a.n + k) * a.ldo + (long)h * dh + e] = k < cnt ? make_double2(v.x / w, v.y / w) : make_double2(0.0, 0.0);
-    } else if (k < cnt) {
-      p.ws.o[(((long)bh * a.n + k) * p.nsplit + chunk) * dh + e] = v;
-    } else if (chunk == 0) {
-      a.out[((long)b * a.n + k) * a.ldo + (long)h * dh + e] = make_double2(0.0, 0.0);
+  for (int x = tid; x < min(16 * NG, at.cnt - at.n0) * dh; x += 256) {
+    const int r = x / dh, e = x - r * dh;
+    double2 v = os[r * OSTR + e];
+#pragma unroll
+    for (int g = 1; g < PARTS; ++g) v = cadd(v, os[(g * NG * 16 + r) * OSTR + e]);
+    tree_put(a, p, ws, at, at.n0 + r, e, v, sum[r >> 4][r & 15]);
+  }
+}
+
+// 33 nodes and more: every wave has 16 nodes of its own and the block's tiles
+// are shared.  A wave requests a quarter of the tile after the next, in the
+// order the matrix cores take it, and leaves it in LDS once the products of the
+// current one are done: a load has a whole tile's time to arrive.  The queries
+// wait in registers.
+template <int DHP, bool FULL>
+__global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws) {
+  constexpr int U = DHP / 4, CT = DHP / 16;
+  constexpr int F = U + 4 * CT;    // 1 KB fragments of a tile: keys [U], values [4][CT]
+  constexpr int PER = F / 4;       // of each wave
+  constexpr int OSTR = DHP + 1;
+  constexpr size_t T_BYTES = 2 * (size_t)F * 64 * sizeof(double2), O_BYTES = (size_t)64 * OSTR * sizeof(double2);
+  __shared__ __align__(16) unsigned char lds[T_BYTES > O_BYTES ? T_BYTES : O_BYTES];
+  __shared__ double sum[64];
+  double2* tiles = (double2*)lds;  // [2][F][64], then outputs [64][OSTR]
+  double2* os = (double2*)lds;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int node = lane & 15, kq = lane >> 4, dh = a.dh;
+  const TreeAt at(a, p, 64);
+  at.clear(a, 64);
+  if (at.n0 >= at.cnt) return;
+  const int t0 = at.t0, t1 = at.t1;
+  const double2* K = a.kc + (long)at.bh * a.ctx * dh;
+  const double2* V = a.vc + (long)at.bh * a.ctx * dh;
+  const int i = at.n0 + 16 * wave + node;
+  // this wave's fragments of the tile at t: keys 4 u + kq of row lane % 16, then
+  // value columns 16 c + lane % 16 of row 4 q + kq (padding as in k_tree_split)
+  double2 next[PER];
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int j = 0; j < U / 4; ++j) {
+      const int u = wave * (U / 4) + j;
+      const uint32_t x = (uint32_t)min(node, t1 - 1 - t) * (uint32_t)dh + kq + 4 * u;
+      next[j] = FULL || 4 * u + kq < dh ? ld_glb(K + (long)t * dh + x) : make_double2(0.0, 0.0);
     }
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const uint32_t x = (uint32_t)min(4 * wave + kq, t1 - 1 - t) * (uint32_t)dh;
+      next[U / 4 + c] = ld_glb(V + (long)t * dh + (x + (FULL ? node + 16 * c : min(node + 16 * c, dh - 1))));
+    }
+  };
+  const auto leave = [&](int buf) {
+    double2* to = tiles + buf * F * 64 + lane;
+#pragma unroll
+    for (int j = 0; j < U / 4; ++j) to[(wave * (U / 4) + j) * 64] = next[j];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) to[(U + wave * CT + c) * 64] = next[U / 4 + c];
+  };
+  fetch(t0);
+  double2 qf[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = 4 * u + kq;
+    double2 q = make_double2(0.0, 0.0);
+    if (i < at.cnt && e < dh) q = a.q[((long)at.b * a.n + i) * a.ldq + (long)at.h * dh + e];
+    qf[u] = make_double2(q.x * a.scale, -q.y * a.scale);
+  }
+  leave(0);
+  if (t0 + 16 < t1) fetch(t0 + 16);
+  __syncthreads();
+
+  TreeRun<DHP> run;
+  int buf = 0;
+  for (int t = t0; t < t1; t += 16, buf ^= 1) {
+    const double2* tile = tiles + buf * F * 64 + lane;
+    double bf[4] = {0.0, 0.0, 0.0, 0.0};
+    tree_bias(a, at, t, kq, bf);
+    v4d s = {0.0, 0.0, 0.0, 0.0}, z = s;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const double2 k = tile[u * 64];
+      s = __builtin_amdgcn_mfma_f64_16x16x4f64(k.x, qf[u].x, s, 0, 0, 0);
+      z = __builtin_amdgcn_mfma_f64_16x16x4f64(k.y, qf[u].y, z, 0, 0, 0);
+      if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    const unsigned vis = tree_sees(a, at, t, kq, i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] = (vis >> e & 1) && t + 4 * e + kq < t1 ? s[e] + z[e] + bf[e] : -INFINITY;
+    tree_scores(a, p, ws, at, t, kq, i, s);
+    run.soften(s);
+    const bool drafted = t + 16 > at.L;
+    bool fine = true;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        double2 v = tile[(U + q * CT + c) * 64];
+        if (drafted) fine &= tree_finite(v);
+        run.output(s, q, c, v);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__ballot(!fine)) run.add_left_out(at, V, dh, t, s, vis);
+    if (t + 16 < t1) leave(buf ^ 1);  // read by nobody since the last barrier
+    if (t + 32 < t1) fetch(t + 32);
+    __syncthreads();
+  }
+  run.l = xor32_sum(xor16_sum(run.l));
+  if (kq == 0) {
+    sum[16 * wave + node] = run.l;
+    tree_put_sum(a, p, ws, at, i, run.m, run.l);
+  }
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      os[(16 * wave + node) * OSTR + 16 * c + 4 * e + kq] = make_double2(run.o_re[c][e], run.o_im[c][e]);
+  __syncthreads();
+  for (int x = tid; x < min(64, at.cnt - at.n0) * dh; x += 256) {
+    const int r = x / dh, e = x - r * dh;
+    tree_put(a, p, ws, at, at.n0 + r, e, os[r * OSTR + e], sum[r]);
   }
 }
 
 // Joins the chunks: blocks y < oparts the outputs, the others the weights of
-// 256 / 16 slots each (or 256 where few nodes are weighed).
-constexpr int TREE_FEW = 4;
-__global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, int oparts) {
+// the slots TREE_SLOTS y ..., 16 lanes to a slot where many nodes are weighed.
+constexpr int TREE_FEW = 4, TREE_SLOTS = 64;
+__global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeWs ws, int oparts) {
   const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, tid = threadIdx.x;
-  const int L = a.kv_len[b], cnt = a.count[b], T = cnt ? L + cnt : 0;
-  const int ns = (T + p.ch - 1) / p.ch;
+  const int L = a.kv_len[b], cnt = a.count[b], T = cnt ? L + cnt : 0, ns = p.splits[b];
   if ((int)blockIdx.y < oparts) {
     const int x = blockIdx.y * 256 + tid, i = x / a.dh, e = x - i * a.dh;
     if (i >= cnt) return;
     const long at = ((long)bh * a.n + i) * p.nsplit;
     double M = -INFINITY;
-    for (int s = 0; s < ns; ++s) M = fmax(M, p.ws.m[at + s]);
+    for (int s = 0; s < ns; ++s) M = fmax(M, ws.m[at + s]);
     const double base = M == -INFINITY ? 0.0 : M;
     double l = 0.0;
     double2 v = make_double2(0.0, 0.0);
     for (int s = 0; s < ns; ++s) {
-      const double f = exp(p.ws.m[at + s] - base);
-      const double2 o = p.ws.o[(at + s) * a.dh + e];
-      l += p.ws.l[at + s] * f;
+      const double f = exp(ws.m[at + s] - base);
+      const double2 o = ws.o[(at + s) * a.dh + e];
+      l += ws.l[at + s] * f;
       v = make_double2(v.x + o.x * f, v.y + o.y * f);
     }
     a.out[((long)b * a.n + i) * a.ldo + (long)h * a.dh + e] = make_double2(v.x / l, v.y / l);
     return;
   }
-  const int few = min(a.weigh, cnt);
+  const int few = min(a.weigh, cnt), part = blockIdx.y - oparts;
+  if (part * (a.weigh <= TREE_FEW ? 256 : TREE_SLOTS) >= T) return;
   __shared__ double sM[TREE_MAX_NODES], sL[TREE_MAX_NODES];
   for (int i = tid; i < few; i += 256) {
     const long at = ((long)bh * a.n + i) * p.nsplit;
     double M = -INFINITY, l = 0.0;
-    for (int s = 0; s < ns; ++s) M = fmax(M, p.ws.m[at + s]);
-    for (int s = 0; s < ns; ++s) l += p.ws.l[at + s] * exp(p.ws.m[at + s] - (M == -INFINITY ? 0.0 : M));
+    for (int s = 0; s < ns; ++s) M = fmax(M, ws.m[at + s]);
+    for (int s = 0; s < ns; ++s) l += ws.l[at + s] * exp(ws.m[at + s] - (M == -INFINITY ? 0.0 : M));
     sM[i] = M;
     sL[i] = l;
   }
   __syncthreads();
-  const int part = blockIdx.y - oparts;
   const auto add = [&](int t, double w) {
     double* to = a.weights + (long)bh * a.ctx + t;
     *to = t < L ? *to + w : w;
   };
   // a slot that a node does not see has score -inf; a node without any weight
   // (maximum -inf) is NaN at the slots it sees, as its output is
-  const auto weight = [&](int t, int i) {
-    const double x = p.ws.x[((long)bh * p.T + t) * a.weigh + i];
+  const auto weight = [&](int t, int i, double x) {
     if (x != -INFINITY || sM[i] != -INFINITY) return exp(x - sM[i]) / sL[i];
     const int j = t - L;
     const bool see = j < 0 || ((a.seen[((long)b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1);
     return see ? (double)NAN : 0.0;
   };
+  const double* xs = ws.x + (long)bh * p.T * a.weigh;
   if (a.weigh <= TREE_FEW) {
     const int t = part * 256 + tid;
     if (t >= T) return;
     double w = 0.0;
-    for (int i = 0; i < few; ++i) w += weight(t, i);
+    for (int i = 0; i < few; ++i) w += weight(t, i, xs[(long)t * a.weigh + i]);
     add(t, w);
-  } else {
-    const int t = part * 16 + (tid >> 4);
-    double w = 0.0;
-    if (t < T)
-      for (int i = tid & 15; i < few; i += 16) w += weight(t, i);
-    w = row16_sum(w);
-    if (t < T && (tid & 15) == 0) add(t, w);
+    return;
+  }
+  double w[TREE_SLOTS / 16] = {};
+  for (int i = tid & 15; i < few; i += 16) {
+    double x[TREE_SLOTS / 16];
+#pragma unroll
+    for (int k = 0; k < TREE_SLOTS / 16; ++k) {
+      const int t = part * TREE_SLOTS + 16 * k + (tid >> 4);
+      x[k] = xs[(long)min(t, T - 1) * a.weigh + i];
+    }
+#pragma unroll
+    for (int k = 0; k < TREE_SLOTS / 16; ++k) w[k] += weight(min(part * TREE_SLOTS + 16 * k + (tid >> 4), T - 1), i, x[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < TREE_SLOTS / 16; ++k) {
+    const int t = part * TREE_SLOTS + 16 * k + (tid >> 4);
+    const double all = row16_sum(w[k]);
+    if (t < T && (tid & 15) == 0) add(t, all);
   }
 }
 
-// Node groups per block: as many as there are nodes for, where LDS holds their
-// queries.  Chunks: as many as fill the chip twice over, of at least one tile
-// per wave.
-static TreePlan tree_plan(const TreeAttn& a) {
+// Chunks of c times 64 slots: the c of least estimated time.  The whole work at
+// the rates of a full chip (5.2 TB/s, 65 TFLOP/s), 2 us for each round of
+// blocks, and half of a block's time for the idle places of the last round.
+// Measured, us, head dim 64: 32 sequences of 144 to 512 slots and 16 nodes 64 in
+// chunks of 128, 52 of 256; 64 of 400 to 512 and one node 160 of 128, 147 of 256,
+// 157 of 512.
+TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& table) {
   TreePlan p;
-  const int most = a.dh <= 64 ? 4 : a.dh <= 128 ? 2 : 1;
-  p.ng = a.n <= 16 ? 1 : std::min(most, a.n <= 32 ? 2 : 4);
-  p.T = a.T_max;
-  const long blocks = (long)a.B * a.H * ((a.n + 16 * p.ng - 1) / (16 * p.ng));
-  const int tiles = std::max(1, (p.T + 63) / 64);
-  p.nsplit = (int)std::max<long>(1, std::min<long>(std::min(tiles, 64), (1024 + blocks - 1) / blocks));
-  p.ch = (tiles + p.nsplit - 1) / p.nsplit * 64;
-  p.nsplit = std::max(1, (p.T + p.ch - 1) / p.ch);
+  p.ng = a.n <= 16 ? 1 : a.n <= 32 ? 2 : a.dh <= 128 ? 4 : 1;
+  if (a.dh > 128) p.ng = 1;
+  const int groups = (a.n + 16 * p.ng - 1) / (16 * p.ng);
+  const double places = a.dh <= 64 || (a.dh <= 128 && p.ng < 4) ? 512.0 : 256.0;  // blocks the chip holds at once
+  double all = 0.0;  // 64-slot pieces of the call
+  for (int b = 0; b < a.B; ++b) {
+    const int T = count[b] ? kv_len[b] + count[b] : 0;
+    p.T = std::max(p.T, T);
+    all += (T + 63) / 64;
+  }
+  const double piece = std::max(64.0 * a.dh * 32 / 5.2e6 / groups, 64.0 * 16 * p.ng * 8 * a.dh / 65e6);  // us of the chip's time
+  int best = 1;
+  double least = 1e300;
+  const int most = (p.T + 63) / 64;
+  for (int c = 1; c <= std::max(1, most); ++c) {
+    double blocks = 0.0;
+    int widest = 0;
+    for (int b = 0; b < a.B; ++b) {
+      const int st = std::max(1, ((count[b] ? kv_len[b] + count[b] : 0) + 63) / 64), k = (st + c - 1) / c;
+      blocks += k;
+      widest = std::max(widest, (st + k - 1) / k);
+    }
+    blocks *= (double)a.H * groups;
+    const double rounds = std::ceil(blocks / places), busy = std::min(blocks, places);
+    const double block = 4.0 + widest * std::max(3.0, piece * busy);
+    const double cost = all * a.H * groups * piece + 2.0 * rounds + 0.5 * block * (1.0 - blocks / (rounds * places));
+    if (cost < least) least = cost, best = c;
+  }
+  std::vector<int> order, splits(a.B);
+  std::vector<int4> list;
+  for (int b = 0; b < a.B; ++b) {
+    const int T = count[b] ? kv_len[b] + count[b] : 0, st = std::max(1, (T + 63) / 64);
+    const int k = (st + best - 1) / best, each = (st + k - 1) / k * 64;
+    int s = 0;
+    for (int t0 = 0; s == 0 || t0 < T; t0 += each) list.push_back(make_int4(b, t0, std::min(T, t0 + each), s++));
+    splits[b] = s;
+    p.nsplit = std::max(p.nsplit, s);
+  }
+  std::stable_sort(list.begin(), list.end(), [](const int4& x, const int4& y) { return x.z - x.y > y.z - y.y; });
+  table.resize((table.size() + 3) & ~(size_t)3);
+  p.at = table.size();
+  p.entries = (int)list.size();
+  for (const int4& e : list) table.insert(table.end(), {e.x, e.y, e.z, e.w});
+  table.insert(table.end(), splits.begin(), splits.end());
   return p;
 }
 
-static size_t tree_layout(const TreeAttn& a, TreePlan& p, char* base) {
+static size_t tree_layout(const TreeAttn& a, const TreePlan& p, char* base, TreeWs& ws) {
   const size_t rows = (size_t)a.B * a.H * a.n * p.nsplit;
   size_t at = 0;
   const auto take = [&](size_t bytes) {
@@ -385,48 +578,43 @@ static size_t tree_layout(const TreeAttn& a, TreePlan& p, char* base) {
     at += (bytes + 255) & ~(size_t)255;
     return q;
   };
-  p.ws.m = (double*)take(rows * sizeof(double));
-  p.ws.l = (double*)take(rows * sizeof(double));
-  if (p.nsplit > 1) p.ws.o = (double2*)take(rows * a.dh * sizeof(double2));
-  if (a.weigh > 0) p.ws.x = (double*)take((size_t)a.B * a.H * p.T * a.weigh * sizeof(double));
+  ws.m = (double*)take(rows * sizeof(double));
+  ws.l = (double*)take(rows * sizeof(double));
+  if (p.nsplit > 1) ws.o = (double2*)take(rows * a.dh * sizeof(double2));
+  if (a.weigh > 0) ws.x = (double*)take((size_t)a.B * a.H * p.T * a.weigh * sizeof(double));
   return at;
 }
 
-size_t tree_ws_bytes(const TreeAttn& a) {
-  TreePlan p = tree_plan(a);
-  return tree_layout(a, p, nullptr);
+size_t tree_ws_bytes(const TreeAttn& a, const TreePlan& p) {
+  TreeWs ws;
+  return tree_layout(a, p, nullptr, ws);
 }
 
 template <int DHP, bool FULL>
-static void launch_split_of(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
-  const dim3 grid((unsigned)((long)a.B * a.H * p.nsplit), (a.n + 16 * p.ng - 1) / (16 * p.ng));
-  const auto go = [&](auto kern) { MITOK_LAUNCH(kern, grid, dim3(256), 0, st, a, p); };
-  if constexpr (DHP <= 64)
-    if (p.ng == 4) return go(k_tree_split<DHP, 4, FULL>);
-  if constexpr (DHP <= 128)
+static void launch_split(hipStream_t st, const TreeAttn& a, const TreePlan& p, const TreeWs& ws) {
+  const dim3 grid((unsigned)((long)p.entries * a.H), (a.n + 16 * p.ng - 1) / (16 * p.ng));
+  const auto go = [&](auto kern) { MITOK_LAUNCH(kern, grid, dim3(256), 0, st, a, p, ws); };
+  if constexpr (DHP <= 128) {
+    if (p.ng == 4) return go(k_tree_shared<DHP, FULL>);
     if (p.ng == 2) return go(k_tree_split<DHP, 2, FULL>);
+  }
   go(k_tree_split<DHP, 1, FULL>);
 }
 
-template <int DHP>
-static void launch_split(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
-  if (a.dh == DHP) launch_split_of<DHP, true>(st, a, p);
-  else launch_split_of<DHP, false>(st, a, p);
-}
-
-void tree_attention(hipStream_t st, const TreeAttn& a) {
-  TreePlan p = tree_plan(a);
-  tree_layout(a, p, (char*)a.ws);
-  if (a.dh <= 16) launch_split<16>(st, a, p);
-  else if (a.dh <= 32) launch_split<32>(st, a, p);
-  else if (a.dh <= 64) launch_split<64>(st, a, p);
-  else if (a.dh <= 128) launch_split<128>(st, a, p);
-  else launch_split<256>(st, a, p);
+void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
+  TreeWs ws;
+  tree_layout(a, p, (char*)a.ws, ws);
+  const auto width = [&](auto padded, auto whole, int dhp) { a.dh == dhp ? whole(st, a, p, ws) : padded(st, a, p, ws); };
+  if (a.dh <= 16) width(launch_split<16, false>, launch_split<16, true>, 16);
+  else if (a.dh <= 32) width(launch_split<32, false>, launch_split<32, true>, 32);
+  else if (a.dh <= 64) width(launch_split<64, false>, launch_split<64, true>, 64);
+  else if (a.dh <= 128) width(launch_split<128, false>, launch_split<128, true>, 128);
+  else width(launch_split<256, false>, launch_split<256, true>, 256);
   const int oparts = p.nsplit > 1 ? (a.n * a.dh + 255) / 256 : 0;
-  const int per = a.weigh <= TREE_FEW ? 256 : 16;
+  const int per = a.weigh <= TREE_FEW ? 256 : TREE_SLOTS;
   const int wparts = a.weights && a.weigh > 0 ? (p.T + per - 1) / per : 0;
   if (oparts + wparts)
-    hipLaunchKernelGGL(k_tree_join, dim3((unsigned)(a.B * a.H), oparts + wparts), dim3(256), 0, st, a, p, oparts);
+    hipLaunchKernelGGL(k_tree_join, dim3((unsigned)(a.B * a.H), oparts + wparts), dim3(256), 0, st, a, p, ws, oparts);
 }
 
 }  // namespace mitok
