@@ -74,23 +74,35 @@ __device__ __forceinline__ unsigned tree_sees(const TreeAttn& a, const TreeAt& a
   }
   return vis;
 }
-// the biases of slots t + 4 e + kq
+// the biases of slots t + 4 e + kq (0 without any)
 __device__ __forceinline__ void tree_bias(const TreeAttn& a, const TreeAt& at, int t, int kq, double (&bf)[4]) {
+  const double* bias = a.bias + (long)at.h * a.bias_stride;
   if (!a.bias) return;
+  if (t + 16 <= at.L) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bf[e] = ld_glb(bias + t + kq + 4 * e);
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     int col = min(t + 4 * e + kq, at.t1 - 1);
-    if (t + 16 > at.L && col >= at.L) col = at.L + a.depth[(long)at.b * a.n + col - at.L];
-    bf[e] = a.bias[(long)at.h * a.bias_stride + col];
+    if (col >= at.L) col = at.L + a.depth[(long)at.b * a.n + col - at.L];
+    bf[e] = bias[col];
   }
 }
 // the weighed nodes' scores, [slot][node]
 __device__ __forceinline__ void tree_scores(const TreeAttn& a, const TreePlan& p, const TreeWs& ws, const TreeAt& at,
                                             int t, int kq, int i, const v4d& s) {
   if (i >= a.weigh) return;
+  double* x = ws.x + ((long)at.bh * p.T + t) * a.weigh + (uint32_t)(kq * a.weigh + i);
+  if (t + 16 <= at.t1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) *(MITOK_GLOBAL double*)(x + 4 * e * (uint32_t)a.weigh) = s[e];
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (t + 4 * e + kq < at.t1) ws.x[((long)at.bh * p.T + t + 4 * e + kq) * a.weigh + i] = s[e];
+    if (t + 4 * e + kq < at.t1) x[4 * e * (uint32_t)a.weigh] = s[e];
 }
 
 // One wave's running softmax over 16-slot tiles for the node lane % 16, and
@@ -104,24 +116,30 @@ struct TreeRun {
 #pragma unroll
     for (int c = 0; c < CT; ++c) o_re[c] = o_im[c] = v4d{0.0, 0.0, 0.0, 0.0};
   }
-  // a tile's scores become its weights
+  // A tile's scores become its weights e^(s - m).  Any m near the largest score
+  // serves, so it moves only where a score passes it by 8 (weights up to e^8
+  // then), which after the first tiles hardly happens: no maximum across the
+  // lanes and no rescaling, which costs as much as 8 MFMAs (double arithmetic
+  // and double MFMAs take turns on a SIMD: 4 cycles an operation beside 64).
   __device__ __forceinline__ void soften(v4d& s) {
-    double x, y;
-    pair16_f64(fmax(fmax(s[0], s[1]), fmax(s[2], s[3])), x, y);
-    pair32_f64(fmax(x, y), x, y);
-    const double mn = fmax(m, fmax(x, y));
-    const double base = mn == -INFINITY ? 0.0 : mn;  // nothing seen yet: every weight e^-inf = 0
-    const double keep = exp(m - base);
-    m = mn;
-    double ls = 0.0;
+    const double top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
+    if (__ballot(top > m + 8.0)) {
+      double x, y;
+      pair16_f64(top, x, y);
+      pair32_f64(fmax(x, y), x, y);
+      const double mn = fmax(m, fmax(x, y));
+      const double keep = mn == -INFINITY ? 0.0 : exp(m - mn);
+      m = mn;
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o_re[c] *= keep, o_im[c] *= keep;
+    }
+    const double base = m == -INFINITY ? 0.0 : m;  // nothing seen yet: every weight e^-inf = 0
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       s[e] = exp(s[e] - base);
-      ls += s[e];
+      l += s[e];
     }
-    l = l * keep + ls;
-#pragma unroll
-    for (int c = 0; c < CT; ++c) o_re[c] *= keep, o_im[c] *= keep;
   }
   __device__ __forceinline__ void output(const v4d& s, int q, int c, double2 v) {
     o_re[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(v.x, s[q], o_re[c], 0, 0, 0);
@@ -324,9 +342,9 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 }
 
 // 33 nodes and more: every wave has 16 nodes of its own and the block's tiles
-// are shared.  A wave requests a quarter of the tile after the next, in the
-// order the matrix cores take it, and leaves it in LDS once the products of the
-// current one are done: a load has a whole tile's time to arrive.  The queries
+// are shared.  A wave requests a quarter of the next tile, in the order the
+// matrix cores take it, among the first products of the current one and leaves
+// it in LDS after the last: a load has most of a tile's time to arrive.  The queries
 // wait in registers.
 template <int DHP, bool FULL>
 __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws) {
@@ -337,6 +355,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
   constexpr size_t T_BYTES = 2 * (size_t)F * 64 * sizeof(double2), O_BYTES = (size_t)64 * OSTR * sizeof(double2);
   __shared__ __align__(16) unsigned char lds[T_BYTES > O_BYTES ? T_BYTES : O_BYTES];
   __shared__ double sum[64];
+  __shared__ int left_out;  // some value stayed out of a tile
   double2* tiles = (double2*)lds;  // [2][F][64], then outputs [64][OSTR]
   double2* os = (double2*)lds;
 
@@ -349,30 +368,42 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
   const double2* K = a.kc + (long)at.bh * a.ctx * dh;
   const double2* V = a.vc + (long)at.bh * a.ctx * dh;
   const int i = at.n0 + 16 * wave + node;
-  // this wave's fragments of the tile at t: keys 4 u + kq of row lane % 16, then
-  // value columns 16 c + lane % 16 of row 4 q + kq (padding as in k_tree_split)
+  // This wave's fragments of the tile at t: value columns 16 c + lane % 16 of row
+  // 4 q + kq, and keys, of which four lanes load 64 bytes of a row (a quarter
+  // wave then touches 4 lines, not 16) and leave them where the products' lanes
+  // read them; kq's rotation of the row keeps both sides off shared banks.
+  // Padding as in k_tree_split.
+  const int krow = lane >> 2, kcol = lane & 3;
+  const int kput = kcol * 16 + ((krow + 4 * kcol) & 15), kget = kq * 16 + ((node + 4 * kq) & 15);
   double2 next[PER];
-  const auto fetch = [&](int t) {
-#pragma unroll
-    for (int j = 0; j < U / 4; ++j) {
+  const auto fetch_one = [&](int t, int j) {
+    if (j < U / 4) {
       const int u = wave * (U / 4) + j;
-      const uint32_t x = (uint32_t)min(node, t1 - 1 - t) * (uint32_t)dh + kq + 4 * u;
-      next[j] = FULL || 4 * u + kq < dh ? ld_glb(K + (long)t * dh + x) : make_double2(0.0, 0.0);
-    }
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
+      const uint32_t x = (uint32_t)min(krow, t1 - 1 - t) * (uint32_t)dh + kcol + 4 * u;
+      next[j] = FULL || 4 * u + kcol < dh ? ld_glb(K + (long)t * dh + x) : make_double2(0.0, 0.0);
+    } else {
+      const int c = j - U / 4;
       const uint32_t x = (uint32_t)min(4 * wave + kq, t1 - 1 - t) * (uint32_t)dh;
-      next[U / 4 + c] = ld_glb(V + (long)t * dh + (x + (FULL ? node + 16 * c : min(node + 16 * c, dh - 1))));
+      next[j] = ld_glb(V + (long)t * dh + (x + (FULL ? node + 16 * c : min(node + 16 * c, dh - 1))));
     }
   };
-  const auto leave = [&](int buf) {
-    double2* to = tiles + buf * F * 64 + lane;
+  // into LDS; values of the nodes' own slots that are not finite stay out
+  const auto leave = [&](int buf, int t) {
+    if (t + 16 > at.L) {
+      bool fine = true;
 #pragma unroll
-    for (int j = 0; j < U / 4; ++j) to[(wave * (U / 4) + j) * 64] = next[j];
+      for (int c = 0; c < CT; ++c) fine &= tree_finite(next[U / 4 + c]);
+      if (!fine) left_out = 1;
+    }
+    double2* to = tiles + buf * F * 64;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) to[(U + wave * CT + c) * 64] = next[U / 4 + c];
+    for (int j = 0; j < U / 4; ++j) to[(wave * (U / 4) + j) * 64 + kput] = next[j];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) to[(U + wave * CT + c) * 64 + lane] = next[U / 4 + c];
   };
-  fetch(t0);
+  if (tid == 0) left_out = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) fetch_one(t0, j);
   double2 qf[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -381,45 +412,47 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
     if (i < at.cnt && e < dh) q = a.q[((long)at.b * a.n + i) * a.ldq + (long)at.h * dh + e];
     qf[u] = make_double2(q.x * a.scale, -q.y * a.scale);
   }
-  leave(0);
-  if (t0 + 16 < t1) fetch(t0 + 16);
+  __syncthreads();
+  leave(0, t0);
   __syncthreads();
 
   TreeRun<DHP> run;
   int buf = 0;
   for (int t = t0; t < t1; t += 16, buf ^= 1) {
-    const double2* tile = tiles + buf * F * 64 + lane;
+    const double2* tile = tiles + buf * F * 64;
     double bf[4] = {0.0, 0.0, 0.0, 0.0};
     tree_bias(a, at, t, kq, bf);
+    const int tn = min(t + 16, t1 - 1);  // the next tile's loads, spread over the products
     v4d s = {0.0, 0.0, 0.0, 0.0}, z = s;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const double2 k = tile[u * 64];
-      s = __builtin_amdgcn_mfma_f64_16x16x4f64(k.x, qf[u].x, s, 0, 0, 0);
-      z = __builtin_amdgcn_mfma_f64_16x16x4f64(k.y, qf[u].y, z, 0, 0, 0);
-      if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    for (int g = 0; g < U / 4; ++g) {
+#pragma unroll
+      for (int j = 0; j < PER / (U / 4); ++j) fetch_one(tn, g * (PER / (U / 4)) + j);
+      double2 k[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) k[j] = tile[(4 * g + j) * 64 + kget];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s = __builtin_amdgcn_mfma_f64_16x16x4f64(k[j].x, qf[4 * g + j].x, s, 0, 0, 0);
+        z = __builtin_amdgcn_mfma_f64_16x16x4f64(k[j].y, qf[4 * g + j].y, z, 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     const unsigned vis = tree_sees(a, at, t, kq, i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = (vis >> e & 1) && t + 4 * e + kq < t1 ? s[e] + z[e] + bf[e] : -INFINITY;
     tree_scores(a, p, ws, at, t, kq, i, s);
     run.soften(s);
-    const bool drafted = t + 16 > at.L;
-    bool fine = true;
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        double2 v = tile[(U + q * CT + c) * 64];
-        if (drafted) fine &= tree_finite(v);
-        run.output(s, q, c, v);
-      }
+      for (int c = 0; c < CT; ++c) run.output(s, q, c, tile[(U + q * CT + c) * 64 + lane]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (__ballot(!fine)) run.add_left_out(at, V, dh, t, s, vis);
-    if (t + 16 < t1) leave(buf ^ 1);  // read by nobody since the last barrier
-    if (t + 32 < t1) fetch(t + 32);
+    if (t + 16 > at.L && left_out) run.add_left_out(at, V, dh, t, s, vis);
+    leave(buf ^ 1, t + 16);  // read by nobody since the last barrier (after the last tile: by nobody at all)
     __syncthreads();
   }
   run.l = xor32_sum(xor16_sum(run.l));
@@ -450,10 +483,12 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
     if (i >= cnt) return;
     const long at = ((long)bh * a.n + i) * p.nsplit;
     double M = -INFINITY;
+#pragma unroll 4
     for (int s = 0; s < ns; ++s) M = fmax(M, ws.m[at + s]);
     const double base = M == -INFINITY ? 0.0 : M;
     double l = 0.0;
     double2 v = make_double2(0.0, 0.0);
+#pragma unroll 4
     for (int s = 0; s < ns; ++s) {
       const double f = exp(ws.m[at + s] - base);
       const double2 o = ws.o[(at + s) * a.dh + e];
@@ -465,14 +500,16 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
   }
   const int few = min(a.weigh, cnt), part = blockIdx.y - oparts;
   if (part * (a.weigh <= TREE_FEW ? 256 : TREE_SLOTS) >= T) return;
-  __shared__ double sM[TREE_MAX_NODES], sL[TREE_MAX_NODES];
+  __shared__ double sM[TREE_MAX_NODES], sR[TREE_MAX_NODES];  // maximum and 1 / sum
   for (int i = tid; i < few; i += 256) {
     const long at = ((long)bh * a.n + i) * p.nsplit;
     double M = -INFINITY, l = 0.0;
+#pragma unroll 4
     for (int s = 0; s < ns; ++s) M = fmax(M, ws.m[at + s]);
+#pragma unroll 4
     for (int s = 0; s < ns; ++s) l += ws.l[at + s] * exp(ws.m[at + s] - (M == -INFINITY ? 0.0 : M));
     sM[i] = M;
-    sL[i] = l;
+    sR[i] = 1.0 / l;
   }
   __syncthreads();
   const auto add = [&](int t, double w) {
@@ -482,7 +519,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
   // a slot that a node does not see has score -inf; a node without any weight
   // (maximum -inf) is NaN at the slots it sees, as its output is
   const auto weight = [&](int t, int i, double x) {
-    if (x != -INFINITY || sM[i] != -INFINITY) return exp(x - sM[i]) / sL[i];
+    if (x != -INFINITY || sM[i] != -INFINITY) return exp(x - sM[i]) * sR[i];
     const int j = t - L;
     const bool see = j < 0 || ((a.seen[((long)b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1);
     return see ? (double)NAN : 0.0;
@@ -515,49 +552,56 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
   }
 }
 
-// Chunks of c times 64 slots: the c of least estimated time.  The whole work at
-// the rates of a full chip (5.2 TB/s, 65 TFLOP/s), 2 us for each round of
-// blocks, and half of a block's time for the idle places of the last round.
-// Measured, us, head dim 64: 32 sequences of 144 to 512 slots and 16 nodes 64 in
-// chunks of 128, 52 of 256; 64 of 400 to 512 and one node 160 of 128, 147 of 256,
-// 157 of 512.
+// Chunks of the least estimated time.  A block's tile takes 2.3 us of a SIMD at
+// head dim 64 (64 MFMAs and the softmax), half as much again alone, or its
+// bytes' time at 5.2 TB/s where every place of the chip is busy; 8 us go to a
+// block's start and end, and the parts of a split pass through memory twice.
+// Whole rounds run at the average length, the last at its longest.  Measured,
+// us, head dim 64: 32 sequences of 144 to 512 slots and 16 nodes 69 in chunks of
+// 64, 57 of 128, 47 of 256, 50 whole; 64 of 400 to 512 and one node 157 of 128,
+// 146 of 256, 149 whole.
 TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& table) {
   TreePlan p;
-  p.ng = a.n <= 16 ? 1 : a.n <= 32 ? 2 : a.dh <= 128 ? 4 : 1;
-  if (a.dh > 128) p.ng = 1;
-  const int groups = (a.n + 16 * p.ng - 1) / (16 * p.ng);
+  p.ng = a.n <= 16 || a.dh > 128 ? 1 : a.n <= 32 ? 2 : 4;
+  const int groups = (a.n + 16 * p.ng - 1) / (16 * p.ng), unit = 64 / p.ng;  // slots that its waves take at a time
   const double places = a.dh <= 64 || (a.dh <= 128 && p.ng < 4) ? 512.0 : 256.0;  // blocks the chip holds at once
-  double all = 0.0;  // 64-slot pieces of the call
+  std::vector<int> len(a.B);
+  double all = 0.0;  // units of the call
   for (int b = 0; b < a.B; ++b) {
-    const int T = count[b] ? kv_len[b] + count[b] : 0;
-    p.T = std::max(p.T, T);
-    all += (T + 63) / 64;
+    len[b] = count[b] ? kv_len[b] + count[b] : 0;
+    p.T = std::max(p.T, len[b]);
+    all += (len[b] + unit - 1) / unit;
   }
-  const double piece = std::max(64.0 * a.dh * 32 / 5.2e6 / groups, 64.0 * 16 * p.ng * 8 * a.dh / 65e6);  // us of the chip's time
-  int best = 1;
-  double least = 1e300;
-  const int most = (p.T + 63) / 64;
-  for (int c = 1; c <= std::max(1, most); ++c) {
-    double blocks = 0.0;
-    int widest = 0;
-    for (int b = 0; b < a.B; ++b) {
-      const int st = std::max(1, ((count[b] ? kv_len[b] + count[b] : 0) + 63) / 64), k = (st + c - 1) / c;
-      blocks += k;
-      widest = std::max(widest, (st + k - 1) / k);
+  const double row = (double)a.H * groups, tile = 0.7 + 1.6 * a.dh / 64;
+  const double unit_mb_us = unit * a.dh * 32 / 5.2e6 / groups;
+  const int most = std::max(1, (p.T + unit - 1) / unit);
+  int each = 1;  // units of a chunk
+  if (all * row > places) {
+    double least = 1e300;
+    int last = 0;
+    for (int k : {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 32}) {
+      const int c = (most + k - 1) / k, slots = c * unit;
+      if (c == last) continue;
+      last = c;
+      double blocks = 0.0;
+      for (int b = 0; b < a.B; ++b) blocks += std::max(1, (len[b] + slots - 1) / slots);
+      const bool split = blocks > a.B;
+      blocks *= row;
+      const double full = std::floor(blocks / places), rest = blocks - full * places;
+      const double work = all * row / blocks;  // units of a block, on average
+      double cost = full * (8.0 + work * std::max(2.0 * tile * places / 512.0, places * unit_mb_us));
+      if (rest > 0.0) cost += 8.0 + std::max(c * tile * (rest > 256.0 ? 2.0 : 1.45), rest * work * unit_mb_us);
+      if (split) cost += blocks * 16 * std::min(p.ng * 16, a.n) * a.dh * 2 / 5.2e6;
+      if (cost < least) least = cost, each = c;
     }
-    blocks *= (double)a.H * groups;
-    const double rounds = std::ceil(blocks / places), busy = std::min(blocks, places);
-    const double block = 4.0 + widest * std::max(3.0, piece * busy);
-    const double cost = all * a.H * groups * piece + 2.0 * rounds + 0.5 * block * (1.0 - blocks / (rounds * places));
-    if (cost < least) least = cost, best = c;
   }
-  std::vector<int> order, splits(a.B);
+  std::vector<int> splits(a.B);
   std::vector<int4> list;
   for (int b = 0; b < a.B; ++b) {
-    const int T = count[b] ? kv_len[b] + count[b] : 0, st = std::max(1, (T + 63) / 64);
-    const int k = (st + best - 1) / best, each = (st + k - 1) / k * 64;
+    const int units = std::max(1, (len[b] + unit - 1) / unit), k = (units + each - 1) / each;
+    const int slots = (units + k - 1) / k * unit;
     int s = 0;
-    for (int t0 = 0; s == 0 || t0 < T; t0 += each) list.push_back(make_int4(b, t0, std::min(T, t0 + each), s++));
+    for (int t0 = 0; s == 0 || t0 < len[b]; t0 += slots) list.push_back(make_int4(b, t0, std::min(len[b], t0 + slots), s++));
     splits[b] = s;
     p.nsplit = std::max(p.nsplit, s);
   }
