@@ -129,6 +129,12 @@ def _ptr(a):
     return None if a is None else a.ctypes.data_as(C.c_void_p)
 
 
+def _at(a):
+    """_ptr as a plain address, in a third of the time: for an array that the
+    caller's frame keeps alive through the call."""
+    return None if a is None else a.__array_interface__["data"][0]
+
+
 def _dev(p):
     return None if p is None else C.c_void_p(p.ptr if isinstance(p, DeviceBuffer) else int(p))
 
@@ -583,7 +589,7 @@ class Network:
         lens = _u32_vec(kv_lens, B, "kv_lens")
         cnt = None if counts is None else _u32_vec(counts, B, "counts")
         _check(self._lib.mitok_tree_attention_device(self._h, _dev(d_q), _dev(d_k_cache), _dev(d_v_cache), _dev(bias),
-                                                     int(bias_stride), _ptr(lens), _ptr(par), _ptr(cnt), B, nodes,
+                                                     int(bias_stride), _at(lens), _at(par), _at(cnt), B, nodes,
                                                      heads, head_dim, max_ctx, int(weigh_nodes), _dev(weights),
                                                      _dev(d_out)))
 
@@ -598,8 +604,8 @@ class Network:
         cnt = None if counts is None else _u32_vec(counts, B, "counts")
         out = np.empty((B, nodes), np.uint32)
         logits = np.empty((B, nodes, self.vocab), np.float64) if want_logits else None
-        _check(self._lib.mitok_tree_step(self._h, _ptr(ids), _ptr(par), _ptr(cnt), B, nodes, int(weigh_nodes),
-                                         _ptr(out), _ptr(logits)))
+        _check(self._lib.mitok_tree_step(self._h, _at(ids), _at(par), _at(cnt), B, nodes, int(weigh_nodes),
+                                         _at(out), _at(logits)))
         return (out, logits) if want_logits else out
 
     def tree_step_device(self, ids, parents, d_logits, counts=None, weigh_nodes=0):
@@ -608,7 +614,7 @@ class Network:
         B, nodes = ids.shape
         par = _u32_rows(parents, "parents", (B, nodes))
         cnt = None if counts is None else _u32_vec(counts, B, "counts")
-        _check(self._lib.mitok_tree_step_device(self._h, _ptr(ids), _ptr(par), _ptr(cnt), B, nodes, int(weigh_nodes),
+        _check(self._lib.mitok_tree_step_device(self._h, _at(ids), _at(par), _at(cnt), B, nodes, int(weigh_nodes),
                                                 _dev(d_logits)))
 
     def tree_accept(self, path, path_lens=None):
@@ -617,7 +623,7 @@ class Network:
         path = _u32_rows(path, "path")
         B, most = path.shape
         lens = np.full(B, most, np.uint32) if path_lens is None else _u32_vec(path_lens, B, "path_lens")
-        _check(self._lib.mitok_tree_accept(self._h, _ptr(path), _ptr(lens), B, most))
+        _check(self._lib.mitok_tree_accept(self._h, _at(path), _at(lens), B, most))
 
     def evict_rows_device(self, d_k_cache, d_v_cache, d_weights, kv_lens, heads, head_dim, max_ctx, keep, sinks, recent,
                           d_k_out, d_v_out, d_weights_out, out_ctx, kept=None):
@@ -629,10 +635,10 @@ class Network:
         if lens.ndim != 1:
             raise ValueError(f"kv_lens: shape {lens.shape}, expected (batch,)")
         out = np.empty(lens.shape, np.uint32)
-        _check(self._lib.mitok_evict_rows_device(self._h, _dev(d_k_cache), _dev(d_v_cache), _dev(d_weights), _ptr(lens),
+        _check(self._lib.mitok_evict_rows_device(self._h, _dev(d_k_cache), _dev(d_v_cache), _dev(d_weights), _at(lens),
                                                  len(lens), heads, head_dim, max_ctx, keep, sinks, recent,
                                                  _dev(d_k_out), _dev(d_v_out), _dev(d_weights_out), out_ctx,
-                                                 _dev(kept), _ptr(out)))
+                                                 _dev(kept), _at(out)))
         return out
 
     def evict_rows(self, batch, keep, sinks=0, recent=0):
@@ -640,7 +646,7 @@ class Network:
         that tree_step(weigh_nodes > 0) kept (mitok_evict_rows).  Returns the
         rows left per sequence."""
         out = np.empty(int(batch), np.uint32)
-        _check(self._lib.mitok_evict_rows(self._h, int(batch), int(keep), int(sinks), int(recent), _ptr(out)))
+        _check(self._lib.mitok_evict_rows(self._h, int(batch), int(keep), int(sinks), int(recent), _at(out)))
         return out
 
     def process_logits_device(self, d_logits, rows, vocab, out=None, ids=None, history=None, max_history=0,
@@ -683,9 +689,9 @@ class Network:
             al = np.ascontiguousarray(np.packbits(bits, axis=1, bitorder="little")).view("<u4")
         out = np.empty_like(x) if want_logits else None
         ids = np.empty(R, np.uint32)
-        _check(self._lib.mitok_process_logits(self._h, _ptr(x), R, V, _ptr(h), 0 if h is None else h.shape[1], _ptr(p),
-                                              _ptr(bi), _ptr(bv), 0 if bi is None else bi.shape[1], _ptr(al),
-                                              _ptr(out), _ptr(ids)))
+        _check(self._lib.mitok_process_logits(self._h, _at(x), R, V, _at(h), 0 if h is None else h.shape[1], _at(p),
+                                              _at(bi), _at(bv), 0 if bi is None else bi.shape[1], _at(al),
+                                              _at(out), _at(ids)))
         return out, ids
 
     # ---- measurement ----

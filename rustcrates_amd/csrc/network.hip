@@ -3614,6 +3614,8 @@ int mitok_greedy_decoding_noalloc(mitok_network* n, const double* logits, uint32
 // ===========================================================================
 // operators of a serving loop (serving.hpp)
 // ===========================================================================
+constexpr uint32_t OP_MAX_CTX = 1u << 30;  // the kernels count a sequence's slots in 32 bits, and a tile past them
+
 // a x b x ..., or SIZE_MAX where that passes 64 bits
 static size_t times(std::initializer_list<size_t> f) {
   size_t p = 1;
@@ -3793,7 +3795,7 @@ int mitok_tree_attention_device(mitok_network* n, const double* d_q, const doubl
                                 double* d_out) {
   if (!n || !d_q || !d_k || !d_v || !kv_lens || !parents || !d_out) return fail(ERR_ARG, "tree attention: null argument");
   TRY(check_tree(parents, counts, B, nodes));
-  if (!heads || !dh || !ctx || ctx > (uint32_t)INT32_MAX) return fail(ERR_ARG, "tree attention: bad shape");
+  if (!heads || !dh || !ctx || ctx > OP_MAX_CTX) return fail(ERR_ARG, "tree attention: bad shape");
   if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "tree attention: head dim %u > %d unsupported", dh, TREE_MAX_DH);
   if (B > 65535 || heads > 65535) return fail(ERR_ARG, "tree attention: batch and heads at most 65535");
   if (weigh_nodes && !d_weights) return fail(ERR_ARG, "tree attention: weigh_nodes without weights");
@@ -4056,7 +4058,7 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
                             double* d_weights_out, uint32_t out_ctx, uint32_t* d_kept, uint32_t* out_lens) {
   if (!n || !d_k || !d_v || !d_weights || !kv_lens || !d_k_out || !d_v_out || !d_weights_out || !out_lens)
     return fail(ERR_ARG, "evict: null argument");
-  if (!B || !heads || !dh || !ctx || ctx > (uint32_t)INT32_MAX || B > 65535 || heads > 65535)
+  if (!B || !heads || !dh || !ctx || ctx > OP_MAX_CTX || out_ctx > OP_MAX_CTX || B > 65535 || heads > 65535)
     return fail(ERR_ARG, "evict: bad shape");
   if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "evict: head dim %u > %d unsupported", dh, TREE_MAX_DH);
   TRY(check_evict(keep, sinks, recent));
@@ -4098,7 +4100,10 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
     kv[b] = (int)kv_lens[b];
     rows[b] = (int)std::min(kv_lens[b], keep);
   }
-  if (!d_kept) TRY(alloc(n, n->op_ws, kb));
+  if (!d_kept) {  // no more than there are to list
+    keep = std::max(1u, stay);
+    TRY(alloc(n, n->op_ws, times({B, heads, keep, sizeof(uint32_t)})));
+  }
   TRY(op_upload(n, 2 * (size_t)B * sizeof(int)));
   EvictSelect e;
   e.w = d_weights;

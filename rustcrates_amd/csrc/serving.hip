@@ -17,17 +17,17 @@ __device__ __forceinline__ unsigned long long order_key(double w) {
   return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
 
-// One block per (head, sequence).  The least key that stays is found by
-// bisection between the smallest and the largest: each round counts the keys at
-// or above the middle (a compare and a ballot per key, held in registers), and
-// ends early once that is as many as have to stay: about 20 rounds of 0.1 us
-// for weights that differ, 64 at most.  Of equal least keys the lowest slots
+// One block per (head, sequence).  The least key that stays is sought between
+// the smallest and the largest: each round counts the keys at or above three
+// values that quarter the range (a compare and a ballot per key, held in
+// registers), and the search ends once as many as have to stay lie above one:
+// about 10 rounds for weights that differ, 33 at most.  Of equal least keys the lowest slots
 // stay; scans over the slots give ranks and places.  NK: slots per thread, 0:
 // any number, read again each round.
 template <int NK>
 __global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
   __shared__ unsigned long long ext[2][4];
-  __shared__ int part[2][4];
+  __shared__ int4 part[2][4];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int L = e.kv_len[b];
   const double* w = e.w + ((long)b * e.H + h) * e.ctx;
@@ -51,15 +51,22 @@ __global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
     for (int k = 0; k < NK; ++k) held[k] = load(k);
   }
   int round = 0;
-  const auto count = [&](unsigned long long least) {  // keys >= least, in the whole block
-    int c = 0;
+  // keys at or above each of three values, in the whole block
+  const auto count = [&](const unsigned long long (&least)[3], int (&c)[3]) {
+    c[0] = c[1] = c[2] = 0;
 #pragma unroll NK ? NK : 1
-    for (int k = 0; k < nk; ++k) c += __popcll(__ballot(key(k) >= least));
-    if (lane == 0) part[round & 1][wave] = c;
+    for (int k = 0; k < nk; ++k)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) c[j] += __popcll(__ballot(key(k) >= least[j]));
+    if (lane == 0) part[round & 1][wave] = make_int4(c[0], c[1], c[2], 0);
     __syncthreads();
-    c = part[round & 1][0] + part[round & 1][1] + part[round & 1][2] + part[round & 1][3];
+    c[0] = c[1] = c[2] = 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int4 q = part[round & 1][v];
+      c[0] += q.x, c[1] += q.y, c[2] += q.z;
+    }
     ++round;
-    return c;
   };
   // count(>= low) >= most > count(>= high)
   unsigned long long low = ~0ull, high = 0;
@@ -82,39 +89,84 @@ __global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
     low = ~0ull;
   } else {
     bool found = false;
-    while (high - low > 1) {
-      const unsigned long long mid = low + (high - low) / 2;
-      const int c = count(mid);
-      if (c >= most) low = mid;
-      else high = mid;
-      if (c == most) {
-        found = true;
-        break;
+    while (!found && high - low > 1) {
+      const unsigned long long q = (high - low) / 4;
+      const unsigned long long at[3] = {low + q, low + 2 * q, low + 3 * q + (high - low) % 4 / 2};
+      int c[3];
+      count(at, c);
+      unsigned long long next = low;
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        if (c[j] >= most) next = at[j];
+        else high = min(high, at[j]);
+        if (c[j] == most) found = true;  // and low is the largest such, so none below it stays
       }
+      low = next;
     }
-    equal = found ? L : most - count(low + 1);
+    equal = L;
+    if (!found) {
+      const unsigned long long above[3] = {low + 1, low + 1, low + 1};
+      int c[3];
+      count(above, c);
+      equal = most - c[0];
+    }
   }
-  // places, 256 slots at a time
-  int before = 0, ties = 0;
-  __syncthreads();  // the last count has been read
-#pragma unroll NK ? NK : 1
-  for (int k = 0; k < nk; ++k) {
+  const unsigned long long below = (1ull << lane) - 1;
+  // a running number over the slots, whose 256 of step k vote `v`: what comes
+  // before this lane's, given the waves' votes of the step, and the total so far
+  const auto before = [&](const int4& votes, unsigned long long v, int& so_far) {
+    const int w[4] = {votes.x, votes.y, votes.z, votes.w};
+    int at = so_far + __popcll(v & below);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (x < wave) at += w[x];
+      so_far += w[x];
+    }
+    return at;
+  };
+  const auto certain = [&](int k) {  // stays whatever the ties
     const int t = 256 * k + tid;
-    const unsigned long long x = key(k);
-    const unsigned long long eq = __ballot(x == low), below = (1ull << lane) - 1;
-    if (lane == 0) part[0][wave] = __popcll(eq);
+    return t < L && (t < lo || t >= hi || key(k) > low);
+  };
+  int ties = 0, all = 0;
+  if constexpr (NK > 0) {
+    __shared__ int4 eq[NK], st[NK];
+    unsigned stays = 0;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int n = __popcll(__ballot(held[k] == low));
+      if (lane == 0) ((int*)&eq[k])[wave] = n;
+    }
     __syncthreads();
-    int rank = ties + __popcll(eq & below);
-    for (int v = 0; v < wave; ++v) rank += part[0][v];
-    ties += part[0][0] + part[0][1] + part[0][2] + part[0][3];
-    const bool stay = t < L && (t < lo || t >= hi || x > low || (x == low && rank < equal));
-    const unsigned long long st = __ballot(stay);
-    if (lane == 0) part[1][wave] = __popcll(st);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const bool tied = held[k] == low;
+      const int rank = before(eq[k], __ballot(tied), ties);
+      if (certain(k) || (tied && rank < equal)) stays |= 1u << k;
+      const int n = __popcll(__ballot(stays >> k & 1));
+      if (lane == 0) ((int*)&st[k])[wave] = n;
+    }
     __syncthreads();
-    int at = before + __popcll(st & below);
-    for (int v = 0; v < wave; ++v) at += part[1][v];
-    before += part[1][0] + part[1][1] + part[1][2] + part[1][3];
-    if (stay) kept[at] = (uint32_t)t;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int at = before(st[k], __ballot(stays >> k & 1), all);
+      if (stays >> k & 1) kept[at] = (uint32_t)(256 * k + tid);
+    }
+  } else {
+    __shared__ int4 eq, st;
+    for (int k = 0; k < nk; ++k) {
+      const bool tied = key(k) == low;
+      const unsigned long long v = __ballot(tied);
+      if (lane == 0) ((int*)&eq)[wave] = __popcll(v);
+      __syncthreads();
+      const int rank = before(eq, v, ties);
+      const bool stay = certain(k) || (tied && rank < equal);
+      const unsigned long long w2 = __ballot(stay);
+      if (lane == 0) ((int*)&st)[wave] = __popcll(w2);
+      __syncthreads();
+      const int at = before(st, w2, all);
+      if (stay) kept[at] = (uint32_t)(256 * k + tid);
+    }
   }
 }
 
@@ -349,7 +401,7 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
 }
 
 void logit_rules(hipStream_t st, const LogitRules& r) {
-  const bool wide = (long)((r.V + LR_WIDE - 1) / LR_WIDE) * r.rows >= 512;
+  const bool wide = (long)((r.V + LR_WIDE - 1) / LR_WIDE) * r.rows >= 256;
   const int chunks = wide ? (r.V + LR_WIDE - 1) / LR_WIDE : logit_chunks(r.V);
   for (int row0 = 0; row0 < r.rows; row0 += 32768) {  // a counter per row of a launch
     const dim3 grid(chunks, std::min(r.rows - row0, 32768));

@@ -121,9 +121,10 @@ struct TreeRun {
   // then), which after the first tiles hardly happens: no maximum across the
   // lanes and no rescaling, which costs as much as 8 MFMAs (double arithmetic
   // and double MFMAs take turns on a SIMD: 4 cycles an operation beside 64).
+  template <bool LAZY>
   __device__ __forceinline__ void soften(v4d& s) {
     const double top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
-    if (__ballot(top > m + 8.0)) {
+    if (!LAZY || __ballot(top > m + 8.0)) {
       double x, y;
       pair16_f64(top, x, y);
       pair32_f64(fmax(x, y), x, y);
@@ -277,7 +278,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
     tree_scores(a, p, ws, at, t, kq, i, s);
     const bool more = t + 16 * KG < t1;
     if (more) load_keys(t + 16 * KG);
-    run.soften(s);
+    run.template soften<true>(s);
     const bool drafted = t + 16 > at.L;
     bool fine = true;
     if (PRE && drafted) {
@@ -443,7 +444,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = (vis >> e & 1) && t + 4 * e + kq < t1 ? s[e] + z[e] + bf[e] : -INFINITY;
     tree_scores(a, p, ws, at, t, kq, i, s);
-    run.soften(s);
+    run.template soften<true>(s);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -473,8 +474,9 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 }
 
 // Joins the chunks: blocks y < oparts the outputs, the others the weights of
-// the slots TREE_SLOTS y ..., 16 lanes to a slot where many nodes are weighed.
-constexpr int TREE_FEW = 4, TREE_SLOTS = 64;
+// 256 slots, or of TREE_SLOTS and 16 lanes to a slot where many nodes are
+// weighed; a grid of at most TREE_PARTS such blocks walks a longer cache.
+constexpr int TREE_FEW = 4, TREE_SLOTS = 64, TREE_PARTS = 16384;
 __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeWs ws, int oparts) {
   const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, tid = threadIdx.x;
   const int L = a.kv_len[b], cnt = a.count[b], T = cnt ? L + cnt : 0, ns = p.splits[b];
@@ -498,8 +500,8 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
     a.out[((long)b * a.n + i) * a.ldo + (long)h * a.dh + e] = make_double2(v.x / l, v.y / l);
     return;
   }
-  const int few = min(a.weigh, cnt), part = blockIdx.y - oparts;
-  if (part * (a.weigh <= TREE_FEW ? 256 : TREE_SLOTS) >= T) return;
+  const int few = min(a.weigh, cnt), per = a.weigh <= TREE_FEW ? 256 : TREE_SLOTS, step = gridDim.y - oparts;
+  if ((long)(blockIdx.y - oparts) * per >= T) return;
   __shared__ double sM[TREE_MAX_NODES], sR[TREE_MAX_NODES];  // maximum and 1 / sum
   for (int i = tid; i < few; i += 256) {
     const long at = ((long)bh * a.n + i) * p.nsplit;
@@ -525,30 +527,29 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
     return see ? (double)NAN : 0.0;
   };
   const double* xs = ws.x + (long)bh * p.T * a.weigh;
-  if (a.weigh <= TREE_FEW) {
-    const int t = part * 256 + tid;
-    if (t >= T) return;
-    double w = 0.0;
-    for (int i = 0; i < few; ++i) w += weight(t, i, xs[(long)t * a.weigh + i]);
-    add(t, w);
-    return;
-  }
-  double w[TREE_SLOTS / 16] = {};
-  for (int i = tid & 15; i < few; i += 16) {
-    double x[TREE_SLOTS / 16];
+  for (int from = (blockIdx.y - oparts) * per; from < T; from += step * per) {
+    if (a.weigh <= TREE_FEW) {
+      const int t = from + tid;
+      if (t >= T) return;
+      double w = 0.0;
+      for (int i = 0; i < few; ++i) w += weight(t, i, xs[(long)t * a.weigh + i]);
+      add(t, w);
+      continue;
+    }
+    double w[TREE_SLOTS / 16] = {};
+    for (int i = tid & 15; i < few; i += 16) {
+      double x[TREE_SLOTS / 16];
 #pragma unroll
-    for (int k = 0; k < TREE_SLOTS / 16; ++k) {
-      const int t = part * TREE_SLOTS + 16 * k + (tid >> 4);
-      x[k] = xs[(long)min(t, T - 1) * a.weigh + i];
+      for (int k = 0; k < TREE_SLOTS / 16; ++k) x[k] = xs[(long)min(from + 16 * k + (tid >> 4), T - 1) * a.weigh + i];
+#pragma unroll
+      for (int k = 0; k < TREE_SLOTS / 16; ++k) w[k] += weight(min(from + 16 * k + (tid >> 4), T - 1), i, x[k]);
     }
 #pragma unroll
-    for (int k = 0; k < TREE_SLOTS / 16; ++k) w[k] += weight(min(part * TREE_SLOTS + 16 * k + (tid >> 4), T - 1), i, x[k]);
-  }
-#pragma unroll
-  for (int k = 0; k < TREE_SLOTS / 16; ++k) {
-    const int t = part * TREE_SLOTS + 16 * k + (tid >> 4);
-    const double all = row16_sum(w[k]);
-    if (t < T && (tid & 15) == 0) add(t, all);
+    for (int k = 0; k < TREE_SLOTS / 16; ++k) {
+      const int t = from + 16 * k + (tid >> 4);
+      const double all = row16_sum(w[k]);
+      if (t < T && (tid & 15) == 0) add(t, all);
+    }
   }
 }
 
@@ -589,7 +590,7 @@ TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::
       blocks *= row;
       const double full = std::floor(blocks / places), rest = blocks - full * places;
       const double work = all * row / blocks;  // units of a block, on average
-      double cost = full * (8.0 + work * std::max(2.0 * tile * places / 512.0, places * unit_mb_us));
+      double cost = full * (3.0 + work * std::max(2.0 * tile * places / 512.0, places * unit_mb_us));
       if (rest > 0.0) cost += 8.0 + std::max(c * tile * (rest > 256.0 ? 2.0 : 1.45), rest * work * unit_mb_us);
       if (split) cost += blocks * 16 * std::min(p.ng * 16, a.n) * a.dh * 2 / 5.2e6;
       if (cost < least) least = cost, each = c;
@@ -656,7 +657,7 @@ void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
   else width(launch_split<256, false>, launch_split<256, true>, 256);
   const int oparts = p.nsplit > 1 ? (a.n * a.dh + 255) / 256 : 0;
   const int per = a.weigh <= TREE_FEW ? 256 : TREE_SLOTS;
-  const int wparts = a.weights && a.weigh > 0 ? (p.T + per - 1) / per : 0;
+  const int wparts = a.weights && a.weigh > 0 ? std::min((p.T + per - 1) / per, TREE_PARTS) : 0;
   if (oparts + wparts)
     hipLaunchKernelGGL(k_tree_join, dim3((unsigned)(a.B * a.H), oparts + wparts), dim3(256), 0, st, a, p, ws, oparts);
 }

@@ -265,7 +265,8 @@ def test_refusals(net):
     go("null", q=None)
     go("not device memory", q=c["q"].ctypes.data)
     go("exceed its allocation", H=3)
-    go("64 bits|exceed its", H=65535, dh=256, ctx=2 ** 31 - 1)
+    go("exceed its", H=65535, dh=256, ctx=2 ** 30, weigh=1)
+    go("bad shape", ctx=2 ** 30 + 1)
     go("aligned", q=qb.ptr + 8)
     go("overlap", o=qb)
     go("overlap", o=vb)
