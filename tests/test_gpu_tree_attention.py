@@ -133,6 +133,14 @@ CASES = [
     (2, 3, 5, 1, 40, [5, 33], None, "tree", 3, True),        # one complex number a head
     (1, 2, 2, 7, 20, [9], None, "chain", 2, True),
     (2, 20, 12, 64, 2048, [2028, 1500], None, "tree", 1, True),
+    (1, 40, 2, 24, 90, [33], None, "tree", 7, True),         # 33 nodes and more, odd widths
+    (2, 50, 1, 100, 120, [61, 8], [50, 37], "forest", 50, True),
+    (1, 70, 3, 7, 200, [127], None, "tree", 1, False),
+    (3, 34, 2, 128, 600, [566, 300, 16], None, "tree", 5, True),
+    (1, 20, 2, 200, 100, [70], None, "tree", 20, True),
+    (2, 24, 3, 128, 1100, [1076, 513], None, "tree", 24, True),
+    (9, 64, 12, 64, 1200, [1100, 1136, 5, 700, 300, 64, 0, 999, 1000], None, "tree", 64, True),  # several chunks each
+    (33, 16, 8, 32, 600, [(37 * b) % 584 for b in range(33)], None, "tree", 2, True),
     (70, 2, 1, 16, 40, [(7 * b) % 38 for b in range(70)], None, "chain", 2, True),
 ]
 
@@ -233,6 +241,97 @@ def test_weights_add_up_over_calls(net):
         assert np.allclose(w2[b, :, :L] - w1[b, :, :L], w1[b, :, :L] - c["w"][b, :, :L], rtol=0, atol=1e-12)
         assert np.array_equal(w2[b, :, L:], w1[b, :, L:])  # drafted slots are set, the rest left
         assert abs((w1 - c["w"])[b, :, :L].sum() + w1[b, :, L:L + c["counts"][b]].sum() - 2 * c["counts"][b]) < 1e-10
+
+
+def test_offsets_past_32_bits(net):
+    """A cache of 6.4 GB of keys: the last sequence's heads begin past 2^32 bytes."""
+    c = make(21, 2, 5, 3, 64, 60, [0, 50], [0, 5])
+    ctx = 1 << 20
+    q, o, w = ra.DeviceBuffer(c["q"].nbytes), ra.DeviceBuffer(c["q"].nbytes), ra.DeviceBuffer(2 * 3 * ctx * 8)
+    k, v, b = ra.DeviceBuffer(2 * 3 * ctx * 64 * 16), ra.DeviceBuffer(2 * 3 * ctx * 64 * 16), ra.DeviceBuffer(c["bias"].nbytes)
+
+    def part(buf, row, a):
+        x = ra.DeviceBuffer.__new__(ra.DeviceBuffer)
+        x._hip, x.nbytes, x.device = buf._hip, a.nbytes, 0
+        x._p = type(buf._p)(buf.ptr + row * a.itemsize * (a.shape[-1] if a.ndim > 1 else 1))
+        return x
+
+    q.upload(c["q"])
+    b.upload(c["bias"])
+    for h in range(3):
+        part(k, (3 + h) * ctx, c["k"][1, h]).upload(c["k"][1, h])
+        part(v, (3 + h) * ctx, c["v"][1, h]).upload(c["v"][1, h])
+        part(w, (3 + h) * ctx, c["w"][1, h]).upload(c["w"][1, h])
+    net.tree_attention_device(q, k, v, c["lens"], c["par"], 3, 64, ctx, o, counts=c["counts"], bias=b, bias_stride=60,
+                              weights=w, weigh_nodes=5)
+    want, tol, w_want, w_tol = formula(c, 5)
+    close(o.download(c["q"].shape, complex), want, tol)
+    for h in range(3):
+        close(part(w, (3 + h) * ctx, c["w"][1, h]).download((60,), float), w_want[1, h], w_tol[1, h])
+    # and an eviction of the same rows, to a small cache and in place
+    ko, vo, wo = ra.DeviceBuffer(2 * 3 * 20 * 64 * 16), ra.DeviceBuffer(2 * 3 * 20 * 64 * 16), ra.DeviceBuffer(2 * 3 * 20 * 8)
+    kept = ra.DeviceBuffer(2 * 3 * 20 * 4)
+    assert net.evict_rows_device(k, v, w, [0, 55], 3, 64, ctx, 20, 2, 6, ko, vo, wo, 20, kept=kept).tolist() == [0, 20]
+    rows = kept.download((2, 3, 20), np.uint32)[1]
+    assert net.evict_rows_device(k, v, w, [0, 55], 3, 64, ctx, 20, 2, 6, k, v, w, ctx).tolist() == [0, 20]
+    for h in range(3):
+        x = ko.download((2, 3, 20, 64), complex)[1, h]
+        assert np.array_equal(x, c["k"][1, h, rows[h]])
+        assert np.array_equal(part(k, (3 + h) * ctx, x).download(x.shape, complex), x)
+        y = vo.download((2, 3, 20, 64), complex)[1, h]
+        assert np.array_equal(part(v, (3 + h) * ctx, y).download(y.shape, complex), y)
+    for x in (q, o, w, k, v, b, ko, vo, wo, kept):
+        x.free()
+
+
+def test_work_queued_on_the_default_stream_comes_first(net):
+    """The queries arrive by a copy that the default stream still has before it
+    when the call is made."""
+    c = make(22, 2, 5, 3, 64, 200, [150, 40])
+    want, _ = call(net, c)
+    big = [ra.DeviceBuffer(1 << 30) for _ in range(2)]
+    bufs = {x: ra.DeviceBuffer(c[x].nbytes) for x in ("q", "k", "v", "bias")}
+    late, o = ra.DeviceBuffer(c["q"].nbytes), ra.DeviceBuffer(c["q"].nbytes)
+    for x in bufs:
+        bufs[x].upload(c[x])
+    late.upload(np.zeros_like(c["q"]))
+    hip = late._hip
+    size = __import__("ctypes").c_size_t
+    for i in range(16):  # about 6 ms of copies
+        assert hip.hipMemcpyAsync(big[i % 2]._p, big[1 - i % 2]._p, size(1 << 30), 3, None) == 0
+    assert hip.hipMemcpyAsync(late._p, bufs["q"]._p, size(c["q"].nbytes), 3, None) == 0
+    net.tree_attention_device(late, bufs["k"], bufs["v"], c["lens"], c["par"], 3, 64, 200, o, bias=bufs["bias"], bias_stride=200)
+    assert np.array_equal(o.download(c["q"].shape, complex), want)
+    for x in [*big, *bufs.values(), late, o]:
+        x.free()
+
+
+def test_two_networks_at_once():
+    """Two threads, each with a network of its own: every call gives its own result."""
+    import threading
+
+    cases = [make(30 + i, 3, 9 + 30 * i, 4, 64, 400, [300, 200 + i, 17]) for i in range(2)]
+    wants, bad = [None, None], []
+    with ra.Network(0) as one:
+        for i, c in enumerate(cases):
+            wants[i] = call(one, c, 2)
+
+    def loop(i):
+        try:
+            with ra.Network(0) as n:
+                for _ in range(10):
+                    o, w = call(n, cases[i], 2)
+                    if not (np.array_equal(o, wants[i][0]) and np.array_equal(w, wants[i][1])):
+                        bad.append(i)
+        except Exception as e:  # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def test_refusals(net):

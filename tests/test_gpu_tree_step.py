@@ -258,6 +258,38 @@ def test_a_drafting_loop_with_rules_and_evictions(model):
     assert evicted >= 2 and len(prompt) + committed > cfg.max_ctx
 
 
+def test_trees_on_a_cache_that_predict_filled_with_launches_timed(model):
+    """A forward_only predict leaves the caches too; attention launches are timed
+    like the others."""
+    cfg, t, build = model
+    prompt = seeded.prompts(9, [12, 8], cfg.vocab)
+    with build(ra.Network(0)) as g:
+        g.prefill(prompt, lens=[12, 8])
+        want, lg = g.tree_step([[5, 6], [7, 8]], [[-1, 0], [-1, -1]], want_logits=True)
+        g.reset()
+        g.predict(prompt, lens=[12, 8])
+        g.timing_enable(ra.TIME_ATTENTION)
+        got, lg2 = g.tree_step([[5, 6], [7, 8]], [[-1, 0], [-1, -1]], want_logits=True)
+        timed = g.timing_read()
+        g.timing_enable(0)
+        assert np.array_equal(got, want) and np.array_equal(lg, lg2)
+        assert timed["launches"] == cfg.layers and timed["total_ms"] > 0
+        g.tree_accept([[0, 1], [1, 0]], [2, 1])
+        assert np.array_equal(g.decode_step([3, 4]), g_steps(build, prompt, [12, 8], [[5, 6], [8]], [3, 4]))
+
+
+def g_steps(build, prompt, lens, fed, last):
+    """The same tokens one step at a time, each sequence in a network of its own: the ids after the last."""
+    out = []
+    for b in range(2):
+        with build(ra.Network(0)) as g:
+            g.prefill(prompt[b:b + 1, :lens[b]])
+            for tok in fed[b]:
+                g.decode_step([tok])
+            out.append(int(g.decode_step([last[b]])[0]))
+    return np.array(out, np.uint32)
+
+
 def test_refusals(model):
     cfg, t, build = model
 
