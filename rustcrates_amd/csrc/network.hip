@@ -285,6 +285,7 @@ enum RunMode { MODE_PREFILL = 0, MODE_CACHED = 1, MODE_STATELESS = 2 };
 struct TreePass {
   TreeAttn a;
   std::vector<TreePlan> plans;
+  OpTable own;
 };
 
 struct Spec {
@@ -927,7 +928,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
           t.out = cat;
           {
             TimeScope ts(n, MITOK_TIME_ATTENTION, 0.0);
-            tree_attention(st, t, sp.tree->plans[ti++]);
+            tree_attention(st, t, sp.tree->plans[ti++], sp.tree->own);
           }
           layernorm(st, cat, cur, nxt, rows, d, A->eps, A->gamma.as<double2>(), A->beta.as<double2>());
         } else if (sp.mode == MODE_CACHED && S == 1) {
@@ -3678,6 +3679,17 @@ static int op_upload(Net* n, size_t bytes) {
   HIP_TRY(hipMemcpyAsync(n->op_tab.p, n->op_host, bytes, hipMemcpyHostToDevice, n->stream));
   return OK;
 }
+// The staged table for kernels: in their arguments (*tab null) where it fits, else uploaded.
+static int op_hand_over(Net* n, size_t bytes, OpTable& own, const char** tab) {
+  *tab = nullptr;
+  if (bytes <= OpTable::ROOM) {
+    memcpy(own.at, n->op_host, bytes);
+    return OK;
+  }
+  TRY(op_upload(n, bytes));
+  *tab = (const char*)n->op_tab.p;
+  return OK;
+}
 
 // Waits for the network's stream and turns the operators' error words into a code.
 static int op_finish(Net* n) {
@@ -3725,8 +3737,8 @@ static int check_tree(const uint32_t* parents, const uint32_t* counts, uint32_t 
 }
 
 // Lengths, counts, depths, ancestor bits and the plans of `layers` (heads and
-// head dims; one plan each, in order), staged and uploaded to op_tab; fills
-// the pass's pointers and sizes and reserves its workspace.  *depth: the nodes'
+// head dims; one plan each, in order), staged and handed over; fills the
+// pass's offsets and sizes and reserves its workspace.  *depth: the nodes'
 // depths [B][nodes] in the staging.
 static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, const uint32_t* counts, uint32_t B,
                       uint32_t nodes, uint32_t weigh, const std::vector<std::pair<int, int>>& layers, TreePass& pass,
@@ -3774,16 +3786,15 @@ static int stage_tree(Net* n, const uint32_t* kv_lens, const uint32_t* parents, 
       s[i >> 6] |= 1ull << (i & 63);
     }
   if (depth) *depth = dep;
-  TRY(op_upload(n, bytes));
-  const char* t = (const char*)n->op_tab.p;
-  a.seen = (const unsigned long long*)t;
+  TRY(op_hand_over(n, bytes, pass.own, &a.tab));
+  a.seen = 0;
   a.words = words;
-  a.kv_len = (const int*)(t + seen_b);
-  a.count = a.kv_len + B;
-  a.depth = a.count + B;
+  a.kv_len = (uint32_t)seen_b;
+  a.count = (uint32_t)(seen_b + B * sizeof(int));
+  a.depth = (uint32_t)(seen_b + 2 * B * sizeof(int));
   for (TreePlan& p : pass.plans) {
-    p.chunks = (const int4*)(t + lists_at) + p.at / 4;
-    p.splits = (const int*)(p.chunks + p.entries);
+    p.chunks += (uint32_t)lists_at;
+    p.splits += (uint32_t)lists_at;
   }
   return OK;
 }
@@ -3838,7 +3849,7 @@ int mitok_tree_attention_device(mitok_network* n, const double* d_q, const doubl
   a.out = (double2*)d_out;
   TRY(behind_default_stream(n));
   TRY(stage_tree(n, kv_lens, parents, counts, B, nodes, weigh_nodes, {{(int)heads, (int)dh}}, pass));
-  tree_attention(n->stream, a, pass.plans[0]);
+  tree_attention(n->stream, a, pass.plans[0], pass.own);
   return op_finish(n);
 }
 
@@ -4013,7 +4024,7 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
   }
   TRY(op_upload(n, (bp + 4 * (size_t)B) * sizeof(int)));
   const uint32_t* dp = n->op_tab.as<uint32_t>();
-  const int* dm = (const int*)(dp + bp);
+  const OpTable none = {};
   for (auto& L : n->layers) {
     if (L->kind != K_SELF_ATTENTION || !most) continue;
     auto* A = (SelfAttentionLayer*)L.get();
@@ -4025,14 +4036,16 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
     m.H = (int)A->heads;
     m.dh = (int)A->dh;
     m.ctx = m.ctx_out = A->max_ctx;
-    m.base = dm + B;
+    m.tab = (const char*)dp;
+    m.based = true;
+    m.base = (uint32_t)((bp + B) * sizeof(int));
     m.idx = dp;
     m.idx_b = max_path;
-    m.rows = dm;
+    m.rows = (uint32_t)(bp * sizeof(int));
     m.rows_max = most;
-    cache_move(st, m);
+    cache_move(st, m, none);
   }
-  pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, dm + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
+  pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, (const int*)(dp + bp) + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
   HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, then, B * sizeof(int), hipMemcpyHostToDevice, st));  // decode steps read it
   TRY(op_finish(n));
   const bool weighed = !n->aw_len.empty();
@@ -4104,10 +4117,10 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
     keep = std::max(1u, stay);
     TRY(alloc(n, n->op_ws, times({B, heads, keep, sizeof(uint32_t)})));
   }
-  TRY(op_upload(n, 2 * (size_t)B * sizeof(int)));
+  OpTable own;
   EvictSelect e;
+  TRY(op_hand_over(n, 2 * (size_t)B * sizeof(int), own, &e.tab));
   e.w = d_weights;
-  e.kv_len = n->op_tab.as<int>();
   e.B = (int)B;
   e.H = (int)heads;
   e.ctx = ctx;
@@ -4116,8 +4129,9 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
   e.sinks = (int)sinks;
   e.recent = (int)recent;
   e.kept = d_kept ? d_kept : n->op_ws.as<uint32_t>();
-  evict_select(n->stream, e);
+  evict_select(n->stream, e, own);
   CacheMove m;
+  m.tab = e.tab;
   m.k = (const double2*)d_k;
   m.v = (const double2*)d_v;
   m.w = d_weights;
@@ -4132,9 +4146,9 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
   m.idx = e.kept;
   m.idx_b = (long)heads * keep;
   m.idx_h = keep;
-  m.rows = e.kv_len + B;
+  m.rows = (uint32_t)(B * sizeof(int));
   m.rows_max = (int)stay;
-  cache_move(n->stream, m);
+  cache_move(n->stream, m, own);
   TRY(op_finish(n));
   for (uint32_t b = 0; b < B; ++b) out_lens[b] = std::min(kv_lens[b], keep);
   return OK;
@@ -4171,13 +4185,14 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
     TRY(alloc(n, n->op_ws, kb));
     TRY(op_upload(n, 4 * (size_t)B * sizeof(int)));
     const int* t = n->op_tab.as<int>();
+    const OpTable none = {};
     for (auto& L : n->layers) {
       if (L->kind != K_SELF_ATTENTION) continue;
       auto* A = (SelfAttentionLayer*)L.get();
       zero_weights(st, A->aw.as<double>(), (int)B, (int)A->heads, A->max_ctx, t + 2 * B, t, most);
       EvictSelect e;
       e.w = A->aw.as<double>();
-      e.kv_len = t;
+      e.tab = (const char*)t;
       e.B = (int)B;
       e.H = (int)A->heads;
       e.ctx = A->max_ctx;
@@ -4186,8 +4201,9 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
       e.sinks = (int)sinks;
       e.recent = (int)recent;
       e.kept = n->op_ws.as<uint32_t>();
-      evict_select(st, e);
+      evict_select(st, e, none);
       CacheMove m;
+      m.tab = e.tab;
       m.k = m.ko = A->kc.as<double2>();
       m.v = m.vo = A->vc.as<double2>();
       m.w = m.wo = A->aw.as<double>();
@@ -4198,9 +4214,9 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
       m.idx = e.kept;
       m.idx_b = (long)A->heads * keep;
       m.idx_h = keep;
-      m.rows = t + B;
+      m.rows = (uint32_t)(B * sizeof(int));
       m.rows_max = std::min(longest, (int)keep);
-      cache_move(st, m);
+      cache_move(st, m, none);
     }
     // later tokens stand where they would without the eviction
     if (!n->pos_off) drop_graph(n);

@@ -25,11 +25,11 @@ __device__ __forceinline__ unsigned long long order_key(double w) {
 // stay; scans over the slots give ranks and places.  NK: slots per thread, 0:
 // any number, read again each round.
 template <int NK>
-__global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
+__global__ __launch_bounds__(256) void k_evict_select(EvictSelect e, OpTable own) {
   __shared__ unsigned long long ext[2][4];
   __shared__ int4 part[2][4];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int L = e.kv_len[b];
+  const int L = op_int(e.tab, own, e.kv_len, b);
   const double* w = e.w + ((long)b * e.H + h) * e.ctx;
   uint32_t* kept = e.kept + ((long)b * e.H + h) * e.keep;
   for (int r = min(L, e.keep) + tid; r < e.keep; r += 256) kept[r] = NO_ROW;
@@ -172,8 +172,8 @@ __global__ __launch_bounds__(256) void k_evict_select(EvictSelect e) {
 
 // keys in registers up to the widest context of a layer (6144); the smallest
 // variant that holds the call's slots
-void evict_select(hipStream_t st, const EvictSelect& e) {
-  const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(e.H, e.B), dim3(256), 0, st, e); };
+void evict_select(hipStream_t st, const EvictSelect& e, const OpTable& own) {
+  const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(e.H, e.B), dim3(256), 0, st, e, own); };
   if (e.T_max <= 512) go(k_evict_select<2>);
   else if (e.T_max <= 2048) go(k_evict_select<8>);
   else if (e.T_max <= 6144) go(k_evict_select<24>);
@@ -188,9 +188,9 @@ __device__ __forceinline__ void st_stream(double2* p, double2 v) {
 
 // To another cache: 256 * MV_PER elements of one (head, sequence)'s keys (y 0)
 // or values (y 1) per block, each read once and written once.
-__global__ __launch_bounds__(256) void k_cache_copy(CacheMove m, int parts) {
+__global__ __launch_bounds__(256) void k_cache_copy(CacheMove m, int parts, OpTable own) {
   const int bh = blockIdx.x / parts, part = blockIdx.x % parts, b = bh / m.H, h = bh - b * m.H, dh = m.dh;
-  const int base = m.base ? m.base[b] : 0, rows = m.rows[b];
+  const int base = m.based ? op_int(m.tab, own, m.base, b) : 0, rows = op_int(m.tab, own, m.rows, b);
   const uint32_t* idx = m.idx + b * m.idx_b + h * m.idx_h;
   if (blockIdx.y == 2) {
     for (int r = part * 256 + threadIdx.x; r < rows; r += parts * 256)
@@ -221,9 +221,9 @@ __global__ __launch_bounds__(256) void k_cache_copy(CacheMove m, int parts) {
 // (head, sequence)'s keys or values, 32 * MV_PER rows at a time: all read, then
 // all written.  The slots ascend, so a row moves to a place at or before its
 // own, and no write reaches a row that a later step reads.
-__global__ __launch_bounds__(256) void k_cache_pack(CacheMove m, int slices) {
+__global__ __launch_bounds__(256) void k_cache_pack(CacheMove m, int slices, OpTable own) {
   const int bh = blockIdx.x / slices, sl = blockIdx.x % slices, b = bh / m.H, h = bh - b * m.H, dh = m.dh;
-  const int base = m.base ? m.base[b] : 0, rows = m.rows[b];
+  const int base = m.based ? op_int(m.tab, own, m.base, b) : 0, rows = op_int(m.tab, own, m.rows, b);
   const uint32_t* idx = m.idx + b * m.idx_b + h * m.idx_h;
   if (blockIdx.y == 2) {
     if (sl) return;
@@ -261,15 +261,15 @@ __global__ __launch_bounds__(256) void k_cache_pack(CacheMove m, int slices) {
   }
 }
 
-void cache_move(hipStream_t st, const CacheMove& m) {
+void cache_move(hipStream_t st, const CacheMove& m, const OpTable& own) {
   if (m.rows_max <= 0) return;
   const unsigned y = m.w ? 3 : 2;
   if (m.ko == m.k) {
     const int slices = (m.dh + 7) / 8;
-    hipLaunchKernelGGL(k_cache_pack, dim3((unsigned)(m.B * m.H * slices), y), dim3(256), 0, st, m, slices);
+    hipLaunchKernelGGL(k_cache_pack, dim3((unsigned)(m.B * m.H * slices), y), dim3(256), 0, st, m, slices, own);
   } else {
     const int parts = (int)(((long)m.rows_max * m.dh + 256 * MV_PER - 1) / (256 * MV_PER));
-    hipLaunchKernelGGL(k_cache_copy, dim3((unsigned)((long)m.B * m.H * parts), y), dim3(256), 0, st, m, parts);
+    hipLaunchKernelGGL(k_cache_copy, dim3((unsigned)((long)m.B * m.H * parts), y), dim3(256), 0, st, m, parts, own);
   }
 }
 

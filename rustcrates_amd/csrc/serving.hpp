@@ -16,6 +16,14 @@ namespace mitok {
 // memory: no copy back).  Plain stores of 1, so any number of lanes may set one.
 enum OpErrWord : int { OE_BAD_TOKEN = 0, OE_NAN = 1, OE_BAD_PENALTY = 2, OE_WORDS = 4 };
 
+// The host's small arrays of a call (lengths, trees, lists), at byte offsets of
+// one table: in the kernels' own arguments where they fit, which saves the
+// upload's 3 us, else in device memory (`tab` of the operator's struct).
+struct OpTable {
+  static constexpr size_t ROOM = 2032;
+  alignas(16) unsigned char at[ROOM];
+};
+
 constexpr int TREE_MAX_NODES = 256;
 constexpr int TREE_WORDS = TREE_MAX_NODES / 64;
 constexpr int TREE_MAX_DH = 256;
@@ -35,10 +43,11 @@ struct TreeAttn {
   const double2* vc = nullptr;
   const double* bias = nullptr;  // [H][bias_stride] or null
   long bias_stride = 0;
-  const int* kv_len = nullptr;         // [B]
-  const int* count = nullptr;          // [B] nodes used; rows past them are zero
-  const int* depth = nullptr;          // [B][n]
-  const unsigned long long* seen = nullptr;  // [B][n][words]: bit j of a node: itself or an ancestor
+  const char* tab = nullptr;  // the table, or null: the kernels' arguments
+  uint32_t seen = 0;          // 64-bit [B][n][words]: bit j of a node: itself or an ancestor
+  uint32_t kv_len = 0;        // int [B]
+  uint32_t count = 0;         // int [B] nodes used; rows past them are zero
+  uint32_t depth = 0;         // int [B][n]
   int words = 1;
   int B = 0, n = 0, H = 0, dh = 0, ctx = 0;
   double scale = 1.0;
@@ -49,20 +58,19 @@ struct TreeAttn {
   void* ws = nullptr;  // tree_ws_bytes
 };
 // How a call's work is cut up, from its lengths (host arrays): each sequence's
-// slots in chunks, the longest first.  The lists are appended to `table`;
-// chunks and splits are set to them once they are on the device.
+// slots in chunks, the longest first.  The lists are appended to `lists`;
+// chunks and splits are their offsets, once the lists' own place is known.
 struct TreePlan {
   int ng = 1;      // groups of 16 nodes per block
   int entries = 0; // chunks of all sequences
   int nsplit = 1;  // the most of one sequence
   int T = 0;       // the most slots of one sequence
-  size_t at = 0;   // first word of the lists in the table
-  const int4* chunks = nullptr;  // [entries]: sequence, first slot, end, index in the sequence
-  const int* splits = nullptr;   // [B] chunks of each sequence
+  uint32_t chunks = 0;  // int4 [entries]: sequence, first slot, end, index in the sequence
+  uint32_t splits = 0;  // int [B] chunks of each sequence
 };
-TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& table);
+TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& lists);
 size_t tree_ws_bytes(const TreeAttn& a, const TreePlan& p);
-void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p);
+void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p, const OpTable& own);
 
 // ---- rows of a cache moved to its front, or to another cache's ----
 struct CacheMove {
@@ -74,13 +82,15 @@ struct CacheMove {
   double* wo = nullptr;
   int B = 0, H = 0, dh = 0;
   long ctx = 0, ctx_out = 0;
-  const int* base = nullptr;      // [B] slot that both sides count from, or null: 0
+  const char* tab = nullptr;      // the table, or null: the kernels' arguments
+  uint32_t base = 0;              // int [B] slot that both sides count from
+  bool based = false;             // (else 0)
   const uint32_t* idx = nullptr;  // row r of (b, h) comes from slot base + idx[b * idx_b + h * idx_h + r]; ascending
   long idx_b = 0, idx_h = 0;
-  const int* rows = nullptr;  // [B] rows moved
+  uint32_t rows = 0;  // int [B] rows moved
   int rows_max = 0;
 };
-void cache_move(hipStream_t st, const CacheMove& m);
+void cache_move(hipStream_t st, const CacheMove& m, const OpTable& own);
 
 // ---- which rows an eviction keeps ----
 // Of kv_len[b] rows, `keep` stay where there are more: the first `sinks`, the
@@ -90,14 +100,15 @@ void cache_move(hipStream_t st, const CacheMove& m);
 constexpr uint32_t NO_ROW = 0xFFFFFFFFu;
 struct EvictSelect {
   const double* w = nullptr;  // [B][H][ctx]
-  const int* kv_len = nullptr;
+  const char* tab = nullptr;
+  uint32_t kv_len = 0;  // int [B] in the table
   int B = 0, H = 0;
   long ctx = 0;
   int T_max = 0;
   int keep = 0, sinks = 0, recent = 0;
   uint32_t* kept = nullptr;
 };
-void evict_select(hipStream_t st, const EvictSelect& e);
+void evict_select(hipStream_t st, const EvictSelect& e, const OpTable& own);
 
 // w[b][h][from[b] .. to[b]) = 0
 void zero_weights(hipStream_t st, double* w, int B, int H, long ctx, const int* from, const int* to, int most);
@@ -126,5 +137,14 @@ struct LogitRules {
 };
 int logit_chunks(int V);
 void logit_rules(hipStream_t st, const LogitRules& r);
+
+// an array of the table; the same value for every lane of a wave where `i` is
+template <class T>
+__device__ __forceinline__ const T* op_array(const char* tab, const OpTable& own, uint32_t at) {
+  return (const T*)((tab ? tab : (const char*)own.at) + at);
+}
+__device__ __forceinline__ int op_int(const char* tab, const OpTable& own, uint32_t at, int i) {
+  return __builtin_amdgcn_readfirstlane(op_array<int>(tab, own, at)[i]);
+}
 
 }  // namespace mitok

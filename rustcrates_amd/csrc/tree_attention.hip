@@ -42,14 +42,21 @@ struct TreeWs {
 // A block's place: chunk entry * H + head, and its first node.
 struct TreeAt {
   int b, h, bh, L, cnt, t0, t1, s, n0;
-  __device__ __forceinline__ TreeAt(const TreeAttn& a, const TreePlan& p, int nodes) {
+  const unsigned long long* seen;  // of the sequence's nodes
+  const int* depth;
+  __device__ __forceinline__ TreeAt(const TreeAttn& a, const TreePlan& p, const OpTable& own, int nodes) {
     const int e = blockIdx.x / a.H;
-    const int4 c = p.chunks[e];
-    b = c.x, t0 = c.y, t1 = c.z, s = c.w;
+    const int4 c = op_array<int4>(a.tab, own, p.chunks)[e];
+    b = __builtin_amdgcn_readfirstlane(c.x);
+    t0 = __builtin_amdgcn_readfirstlane(c.y);
+    t1 = __builtin_amdgcn_readfirstlane(c.z);
+    s = __builtin_amdgcn_readfirstlane(c.w);
     h = blockIdx.x - e * a.H;
     bh = b * a.H + h;
-    L = a.kv_len[b];
-    cnt = a.count[b];
+    L = op_int(a.tab, own, a.kv_len, b);
+    cnt = op_int(a.tab, own, a.count, b);
+    seen = op_array<unsigned long long>(a.tab, own, a.seen) + (long)b * a.n * a.words;
+    depth = op_array<int>(a.tab, own, a.depth) + (long)b * a.n;
     n0 = blockIdx.y * nodes;
   }
   // rows of nodes [n0, n0 + nodes) that are not used: zero, by the sequence's first chunk
@@ -69,7 +76,7 @@ __device__ __forceinline__ unsigned tree_sees(const TreeAttn& a, const TreeAt& a
   for (int e = 0; e < 4; ++e) {
     const int j = t + 4 * e + kq - at.L;
     bool see = j < 0;
-    if (j >= 0 && j < at.cnt && i < at.cnt) see = (a.seen[((long)at.b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1;
+    if (j >= 0 && j < at.cnt && i < at.cnt) see = (at.seen[i * a.words + (j >> 6)] >> (j & 63)) & 1;
     if (see) vis |= 1u << e;
   }
   return vis;
@@ -86,7 +93,7 @@ __device__ __forceinline__ void tree_bias(const TreeAttn& a, const TreeAt& at, i
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     int col = min(t + 4 * e + kq, at.t1 - 1);
-    if (col >= at.L) col = at.L + a.depth[(long)at.b * a.n + col - at.L];
+    if (col >= at.L) col = at.L + at.depth[col - at.L];
     bf[e] = bias[col];
   }
 }
@@ -191,7 +198,7 @@ __device__ __forceinline__ void tree_put_sum(const TreeAttn& a, const TreePlan& 
 }
 
 template <int DHP, int NG, bool FULL>
-__global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p, TreeWs ws) {
+__global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int KG = 4 / NG;       // waves that share a node group's slots
   constexpr int U = DHP / 4;       // 16-byte key loads of a lane per tile, two MFMAs each
   constexpr int CT = DHP / 16;     // 16-column tiles of the values
@@ -208,7 +215,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ng = wave % NG, kg = wave / NG;
   const int node = lane & 15, kq = lane >> 4, dh = a.dh;
-  const TreeAt at(a, p, 16 * NG);
+  const TreeAt at(a, p, own, 16 * NG);
   at.clear(a, 16 * NG);
   if (at.n0 >= at.cnt) return;
   const int t0 = at.t0, t1 = at.t1;
@@ -348,7 +355,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 // it in LDS after the last: a load has most of a tile's time to arrive.  The queries
 // wait in registers.
 template <int DHP, bool FULL>
-__global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws) {
+__global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int U = DHP / 4, CT = DHP / 16;
   constexpr int F = U + 4 * CT;    // 1 KB fragments of a tile: keys [U], values [4][CT]
   constexpr int PER = F / 4;       // of each wave
@@ -362,7 +369,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int node = lane & 15, kq = lane >> 4, dh = a.dh;
-  const TreeAt at(a, p, 64);
+  const TreeAt at(a, p, own, 64);
   at.clear(a, 64);
   if (at.n0 >= at.cnt) return;
   const int t0 = at.t0, t1 = at.t1;
@@ -477,9 +484,10 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 // 256 slots, or of TREE_SLOTS and 16 lanes to a slot where many nodes are
 // weighed; a grid of at most TREE_PARTS such blocks walks a longer cache.
 constexpr int TREE_FEW = 4, TREE_SLOTS = 64, TREE_PARTS = 16384;
-__global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeWs ws, int oparts) {
+__global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeWs ws, int oparts, OpTable own) {
   const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, tid = threadIdx.x;
-  const int L = a.kv_len[b], cnt = a.count[b], T = cnt ? L + cnt : 0, ns = p.splits[b];
+  const int L = op_int(a.tab, own, a.kv_len, b), cnt = op_int(a.tab, own, a.count, b), T = cnt ? L + cnt : 0;
+  const int ns = op_int(a.tab, own, p.splits, b);
   if ((int)blockIdx.y < oparts) {
     const int x = blockIdx.y * 256 + tid, i = x / a.dh, e = x - i * a.dh;
     if (i >= cnt) return;
@@ -523,7 +531,8 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
   const auto weight = [&](int t, int i, double x) {
     if (x != -INFINITY || sM[i] != -INFINITY) return exp(x - sM[i]) * sR[i];
     const int j = t - L;
-    const bool see = j < 0 || ((a.seen[((long)b * a.n + i) * a.words + (j >> 6)] >> (j & 63)) & 1);
+    const auto* seen = op_array<unsigned long long>(a.tab, own, a.seen) + ((long)b * a.n + i) * a.words;
+    const bool see = j < 0 || ((seen[j >> 6] >> (j & 63)) & 1);
     return see ? (double)NAN : 0.0;
   };
   const double* xs = ws.x + (long)bh * p.T * a.weigh;
@@ -561,7 +570,7 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
 // us, head dim 64: 32 sequences of 144 to 512 slots and 16 nodes 69 in chunks of
 // 64, 57 of 128, 47 of 256, 50 whole; 64 of 400 to 512 and one node 157 of 128,
 // 146 of 256, 149 whole.
-TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& table) {
+TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& lists) {
   TreePlan p;
   p.ng = a.n <= 16 || a.dh > 128 ? 1 : a.n <= 32 ? 2 : 4;
   const int groups = (a.n + 16 * p.ng - 1) / (16 * p.ng), unit = 64 / p.ng;  // slots that its waves take at a time
@@ -607,11 +616,12 @@ TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::
     p.nsplit = std::max(p.nsplit, s);
   }
   std::stable_sort(list.begin(), list.end(), [](const int4& x, const int4& y) { return x.z - x.y > y.z - y.y; });
-  table.resize((table.size() + 3) & ~(size_t)3);
-  p.at = table.size();
+  lists.resize((lists.size() + 3) & ~(size_t)3);
   p.entries = (int)list.size();
-  for (const int4& e : list) table.insert(table.end(), {e.x, e.y, e.z, e.w});
-  table.insert(table.end(), splits.begin(), splits.end());
+  p.chunks = (uint32_t)(lists.size() * sizeof(int));
+  for (const int4& e : list) lists.insert(lists.end(), {e.x, e.y, e.z, e.w});
+  p.splits = (uint32_t)(lists.size() * sizeof(int));
+  lists.insert(lists.end(), splits.begin(), splits.end());
   return p;
 }
 
@@ -636,9 +646,9 @@ size_t tree_ws_bytes(const TreeAttn& a, const TreePlan& p) {
 }
 
 template <int DHP, bool FULL>
-static void launch_split(hipStream_t st, const TreeAttn& a, const TreePlan& p, const TreeWs& ws) {
+static void launch_split(hipStream_t st, const TreeAttn& a, const TreePlan& p, const TreeWs& ws, const OpTable& own) {
   const dim3 grid((unsigned)((long)p.entries * a.H), (a.n + 16 * p.ng - 1) / (16 * p.ng));
-  const auto go = [&](auto kern) { MITOK_LAUNCH(kern, grid, dim3(256), 0, st, a, p, ws); };
+  const auto go = [&](auto kern) { MITOK_LAUNCH(kern, grid, dim3(256), 0, st, a, p, ws, own); };
   if constexpr (DHP <= 128) {
     if (p.ng == 4) return go(k_tree_shared<DHP, FULL>);
     if (p.ng == 2) return go(k_tree_split<DHP, 2, FULL>);
@@ -646,10 +656,10 @@ static void launch_split(hipStream_t st, const TreeAttn& a, const TreePlan& p, c
   go(k_tree_split<DHP, 1, FULL>);
 }
 
-void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
+void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p, const OpTable& own) {
   TreeWs ws;
   tree_layout(a, p, (char*)a.ws, ws);
-  const auto width = [&](auto padded, auto whole, int dhp) { a.dh == dhp ? whole(st, a, p, ws) : padded(st, a, p, ws); };
+  const auto width = [&](auto padded, auto whole, int dhp) { a.dh == dhp ? whole(st, a, p, ws, own) : padded(st, a, p, ws, own); };
   if (a.dh <= 16) width(launch_split<16, false>, launch_split<16, true>, 16);
   else if (a.dh <= 32) width(launch_split<32, false>, launch_split<32, true>, 32);
   else if (a.dh <= 64) width(launch_split<64, false>, launch_split<64, true>, 64);
@@ -659,7 +669,7 @@ void tree_attention(hipStream_t st, const TreeAttn& a, const TreePlan& p) {
   const int per = a.weigh <= TREE_FEW ? 256 : TREE_SLOTS;
   const int wparts = a.weights && a.weigh > 0 ? std::min((p.T + per - 1) / per, TREE_PARTS) : 0;
   if (oparts + wparts)
-    hipLaunchKernelGGL(k_tree_join, dim3((unsigned)(a.B * a.H), oparts + wparts), dim3(256), 0, st, a, p, ws, oparts);
+    hipLaunchKernelGGL(k_tree_join, dim3((unsigned)(a.B * a.H), oparts + wparts), dim3(256), 0, st, a, p, ws, oparts, own);
 }
 
 }  // namespace mitok
