@@ -328,7 +328,8 @@ int mitok_greedy_decoding_noalloc(mitok_network* net, const double* logits, uint
  * row that a node does not see has no part in its output, finite or not; rows
  * past counts[b] are zero.
  *   d_q, d_out [batch][nodes][heads * head_dim] complex
- *   d_k_cache, d_v_cache [batch][heads][max_ctx][head_dim] complex, head_dim <= 256, max_ctx <= 2^30
+ *   d_k_cache, d_v_cache [batch][heads][max_ctx][head_dim] complex, head_dim <= 256, max_ctx <= 2^30,
+ *     batch * heads <= 2^18 (here and in an eviction)
  *   d_bias [heads] rows of real numbers, bias_stride apart, or NULL
  *   d_weights [batch][heads][max_ctx] or NULL: the softmax weights that the
  *     first weigh_nodes nodes give each slot are summed; committed slots are

@@ -3616,6 +3616,13 @@ int mitok_greedy_decoding_noalloc(mitok_network* n, const double* logits, uint32
 // operators of a serving loop (serving.hpp)
 // ===========================================================================
 constexpr uint32_t OP_MAX_CTX = 1u << 30;  // the kernels count a sequence's slots in 32 bits, and a tile past them
+constexpr uint32_t OP_MAX_BH = 1u << 18;   // batch x heads: with 32 blocks of 256 threads for each, a launch has 2^31 threads
+
+static int check_heads(const char* what, uint32_t B, uint32_t heads) {
+  if (B > 65535 || heads > 65535 || (uint64_t)B * heads > OP_MAX_BH)
+    return fail(ERR_ARG, "%s: batch and heads at most 65535, and their product %u", what, OP_MAX_BH);
+  return OK;
+}
 
 // a x b x ..., or SIZE_MAX where that passes 64 bits
 static size_t times(std::initializer_list<size_t> f) {
@@ -3808,7 +3815,7 @@ int mitok_tree_attention_device(mitok_network* n, const double* d_q, const doubl
   TRY(check_tree(parents, counts, B, nodes));
   if (!heads || !dh || !ctx || ctx > OP_MAX_CTX) return fail(ERR_ARG, "tree attention: bad shape");
   if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "tree attention: head dim %u > %d unsupported", dh, TREE_MAX_DH);
-  if (B > 65535 || heads > 65535) return fail(ERR_ARG, "tree attention: batch and heads at most 65535");
+  TRY(check_heads("tree attention", B, heads));
   if (weigh_nodes && !d_weights) return fail(ERR_ARG, "tree attention: weigh_nodes without weights");
   if (weigh_nodes > nodes) return fail(ERR_ARG, "tree attention: weigh_nodes %u above %u nodes", weigh_nodes, nodes);
   uint32_t longest = 0;
@@ -3889,6 +3896,7 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
   for (auto& L : n->layers)
     if (L->kind == K_SELF_ATTENTION) {
       auto* A = (SelfAttentionLayer*)L.get();
+      TRY(check_heads("tree step", B, (uint32_t)A->heads));
       shapes.push_back({(int)A->heads, (int)A->dh});
     }
   TRY(stage_tree(n, n->kv_len_h.data(), parents, counts, B, nodes, weigh, shapes, tree, &depth));
@@ -4071,8 +4079,8 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
                             double* d_weights_out, uint32_t out_ctx, uint32_t* d_kept, uint32_t* out_lens) {
   if (!n || !d_k || !d_v || !d_weights || !kv_lens || !d_k_out || !d_v_out || !d_weights_out || !out_lens)
     return fail(ERR_ARG, "evict: null argument");
-  if (!B || !heads || !dh || !ctx || ctx > OP_MAX_CTX || out_ctx > OP_MAX_CTX || B > 65535 || heads > 65535)
-    return fail(ERR_ARG, "evict: bad shape");
+  if (!B || !heads || !dh || !ctx || ctx > OP_MAX_CTX || out_ctx > OP_MAX_CTX) return fail(ERR_ARG, "evict: bad shape");
+  TRY(check_heads("evict", B, heads));
   if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "evict: head dim %u > %d unsupported", dh, TREE_MAX_DH);
   TRY(check_evict(keep, sinks, recent));
   uint32_t longest = 0;

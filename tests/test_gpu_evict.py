@@ -120,6 +120,16 @@ def test_evicting_twice(net):
     check(again, 90, 4, 50, *call(net, again, 90, 4, 50, in_place=True))
 
 
+@pytest.mark.parametrize("B,H", [(5, 65535), (65536, 1), (1, 65536), (513, 512)])
+def test_batches_and_heads_that_a_launch_cannot_hold(net, B, H):
+    b = [ra.DeviceBuffer(256) for _ in range(6)]
+    with pytest.raises(ra.MitokError, match="their product 262144") as e:
+        net.evict_rows_device(*b[:3], np.zeros(B, np.uint32), H, 1, 1, 1, 0, 0, *b[3:], 1)
+    assert e.value.code == 1
+    for x in b:
+        x.free()
+
+
 def test_refusals(net):
     c = make(1, 2, 2, 8, 40, [40, 30])
     dev = {x: ra.DeviceBuffer(c[x].nbytes) for x in "kvw"}

@@ -334,6 +334,14 @@ def test_two_networks_at_once():
     assert not bad
 
 
+@pytest.mark.parametrize("B,H", [(5, 65535), (65536, 1), (1, 65536), (513, 512)])
+def test_batches_and_heads_that_a_launch_cannot_hold(net, B, H):
+    with ra.DeviceBuffer(4096) as x, ra.DeviceBuffer(4096) as y:
+        with pytest.raises(ra.MitokError, match="their product 262144") as e:
+            net.tree_attention_device(x, x, x, np.zeros(B, np.uint32), np.full((B, 1), -1), H, 1, 1, y)
+        assert e.value.code == 1
+
+
 def test_refusals(net):
     c = make(1, 2, 4, 2, 16, 32, [3, 28])
     good = dict(par=c["par"], lens=c["lens"], H=2, dh=16, ctx=32, counts=None, weigh=0, stride=32)

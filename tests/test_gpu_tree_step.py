@@ -11,7 +11,7 @@ import pytest
 import oracle
 import rustcrates_amd as ra
 from conftest import REL_TOL, build_explicit, max_rel_err, seeded_tensors
-from plain_stack import Sequence, apply_rules
+from plain_stack import Sequence, apply_rules, kept_rows
 from rustcrates_amd import configs, seeded
 
 pytestmark = pytest.mark.gpu
@@ -172,6 +172,46 @@ def test_eviction_in_a_stack(model, steps):
             for b, s in enumerate(seqs):
                 want = s.step(int(tok[b]))
                 assert max_rel_err(lg[b], want) < REL_TOL and i[b] == np.argmax(want)
+
+
+def test_weights_of_an_accepted_path_move_with_its_rows(model):
+    """Several nodes weigh, a rejected one among them, and the path's rows do not
+    lie together: each keeps its own weight, which the next eviction goes by."""
+    cfg, t, build = model
+    lens, path, weigh = [11, 17], [0, 2, 4, 5], 5
+    par = np.array([[-1, 0, 0, 1, 2, 4]] * 2)
+    prompt = seeded.prompts(41, lens, cfg.vocab)
+    ids = np.random.default_rng(19).integers(2, cfg.vocab, (2, 6)).astype(np.uint32)
+    keep, seqs, unmoved = 10, [], False
+    for b, L in enumerate(lens):
+        s = Sequence(cfg, t)
+        s.prompt(prompt[b, :L])
+        slots = np.zeros((cfg.layers, cfg.heads, L + 6))  # committed rows, then nodes
+        for i in range(weigh):
+            f, way = s.fork(), path_to(par[b], i)
+            for j in way:
+                f.step(int(ids[b, j]), weigh=j == i)
+            slots[:, :, [*range(L), *(L + j for j in way)]] += np.array(f.weights)
+        for j in path:
+            s.step(int(ids[b, j]))
+        for layer in range(cfg.layers):
+            for h in range(cfg.heads):
+                own = slots[layer, h, [*range(L), *(L + j for j in path)]]
+                s.weights[layer][h] = list(own)
+                unmoved |= kept_rows(list(slots[layer, h, :L + 4]), keep, 0, 0) != kept_rows(list(own), keep, 0, 0)
+        seqs.append(s)
+    assert unmoved  # weights left where they were would keep other rows
+    with build(ra.Network(0)) as g:
+        g.prefill(prompt, lens=lens)
+        g.tree_step(ids, par, weigh_nodes=weigh)
+        g.tree_accept([path] * 2)
+        assert g.evict_rows(2, keep, 0, 0).tolist() == [keep, keep]
+        for s in seqs:
+            s.evict(keep, 0, 0)
+        for tok in (7, 12):
+            _, lg = g.decode_step(np.array([tok, tok + 1], np.uint32), want_logits=True)
+            for b, s in enumerate(seqs):
+                assert max_rel_err(lg[b], s.step(tok + b)) < REL_TOL, (tok, b)
 
 
 def test_a_prompt_starts_weights_anew_and_generate_is_what_it_was(model):
