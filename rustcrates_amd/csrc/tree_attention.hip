@@ -197,6 +197,12 @@ __device__ __forceinline__ void tree_put_sum(const TreeAttn& a, const TreePlan& 
   ws.l[x] = l;
 }
 
+// What bounds it: the bytes of keys and values where a tile has one or few
+// nodes (64 sequences of 12 heads and 400 to 511 rows, head dim 64, one node:
+// 725 MB in 140 us, 5.1 TB/s, as a large copy runs); with 16 nodes 182 MB in 51
+// us, a block's start and end (8 us of its 50) and the longest sequence.  One
+// node takes the matrix instructions too: the 15 unused rows cost nothing that
+// the memory does not hide.
 template <int DHP, int NG, bool FULL>
 __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int KG = 4 / NG;       // waves that share a node group's slots
@@ -353,7 +359,11 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 // are shared.  A wave requests a quarter of the next tile, in the order the
 // matrix cores take it, among the first products of the current one and leaves
 // it in LDS after the last: a load has most of a tile's time to arrive.  The queries
-// wait in registers.
+// wait in registers.  Bound by double MFMAs and the softmax's double arithmetic,
+// which take turns on a SIMD: 4 sequences of 12 heads, 1964 to 2048 slots and 64
+// nodes at head dim 64 take 92 us, 47% of it MFMAs (the padded products alone
+// are 44 us).  Tiles of a wave's own would be read four
+// times through the caches.
 template <int DHP, bool FULL>
 __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int U = DHP / 4, CT = DHP / 16;
@@ -483,6 +493,11 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 // Joins the chunks: blocks y < oparts the outputs, the others the weights of
 // 256 slots, or of TREE_SLOTS and 16 lanes to a slot where many nodes are
 // weighed; a grid of at most TREE_PARTS such blocks walks a longer cache.
+// Bound by its launch where little was split (4 us), else by the parts and
+// scores it reads: 23 us for 64 weighed nodes of 48 heads and 2000 slots (49 MB
+// of scores) and their parts of ten chunks (32 MB).  Joining in the
+// last chunk's block instead was slower throughout (one token 28 -> 30 us a
+// call, 64 sequences 164 -> 175): the parts then pass the XCD's own cache.
 constexpr int TREE_FEW = 4, TREE_SLOTS = 64, TREE_PARTS = 16384;
 __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeWs ws, int oparts, OpTable own) {
   const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, tid = threadIdx.x;
