@@ -309,21 +309,26 @@ __device__ __forceinline__ void set_err(uint32_t* err, int word) {
   __hip_atomic_store(err + word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 
-// tokens per block: 4096, or 1024 where that leaves most of the chip idle
-constexpr int LR_WIDE = 4096, LR_NARROW = 1024;
+// tokens per block: 2048, or 1024 where that leaves most of the chip idle
+constexpr int LR_WIDE = 2048, LR_NARROW = 1024;
 int logit_chunks(int V) { return (V + LR_NARROW - 1) / LR_NARROW; }
+
+// two logits of a row, whose start is aligned to one
+typedef double v2row __attribute__((ext_vector_type(2), aligned(8)));
 
 // One block per (chunk of the vocabulary, row).  Its logits are requested first;
 // the chunk's occurrences in the history and its last bias entry are gathered
 // in LDS meanwhile (integer atomics, so their order does not show); then each
 // logit is changed, written and compared, so it is read once and written once.
 // The row's last block joins the chunks' maxima.  Bound by HBM on many rows
-// (512 rows of 50280, 512 tokens of history: 412 MB in 99 us, 4.2 TB/s; each of
-// a row's 13 blocks reads the row's history), by its chain of loads, LDS
-// atomics and the join on few (one row of 4096 6.8 us, 7 of 31999 9.8).
+// (512 rows of 50280, 512 tokens of history: 412 MB in 86 us, 4.8 TB/s; each of
+// a row's 25 blocks reads the row's history), by its chain of loads, LDS
+// atomics and the join on few (one row of 4096 6.4 us, 7 of 31999 9.5).  Of 4096
+// tokens a block, half as many of which a CU holds, 92 us; one logit to a load
+// and store 99 us at either size.
 template <int CH>
 __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
-  constexpr int PER = CH / 256;
+  constexpr int PER = CH / 512;  // pairs of a thread
   __shared__ __align__(16) uint32_t count[CH], entry[CH];
   __shared__ uint32_t words[CH / 32];
   __shared__ double sv[4];
@@ -335,9 +340,14 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
     return;
   }
   const double* x = r.x + (long)row * V + c0;
-  double y[PER];
+  v2row y[PER];
 #pragma unroll
-  for (int k = 0; k < PER; ++k) y[k] = tid + 256 * k < len ? x[tid + 256 * k] : 0.0;
+  for (int k = 0; k < PER; ++k) {
+    const int i = 2 * (tid + 256 * k);
+    y[k] = v2row{0.0, 0.0};
+    if (i + 1 < len) y[k] = __builtin_nontemporal_load((const MITOK_GLOBAL v2row*)(x + i));
+    else if (i < len) y[k].x = x[i];
+  }
   double theta = 1.0, presence = 0.0, frequency = 0.0;
   if (r.penalties) {
     theta = r.penalties[3 * (long)row];
@@ -371,21 +381,31 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
   bool nan = false;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
-    const int i = tid + 256 * k;
+    const int i = 2 * (tid + 256 * k);
     if (i >= len) break;
-    if (ruled) {
-      const uint32_t c = count[i], en = entry[i];
-      if (c) {
-        y[k] = y[k] > 0.0 ? y[k] / theta : y[k] * theta;
-        y[k] -= frequency * (double)c + presence;
+    uint2 c = make_uint2(0, 0), en = c;
+    if (ruled) c = *(const uint2*)(count + i), en = *(const uint2*)(entry + i);
+    const uint32_t ok = r.allowed ? words[i >> 5] >> (i & 31) : 3u;
+    const auto change = [&](double v, uint32_t times, uint32_t at, bool may) {
+      if (times) {
+        v = v > 0.0 ? v / theta : v * theta;
+        v -= frequency * (double)times + presence;
       }
-      if (en) y[k] += r.bias[(long)row * r.nb + en - 1];
+      if (at) v += r.bias[(long)row * r.nb + at - 1];
+      return may ? v : -INFINITY;
+    };
+    y[k].x = change(y[k].x, c.x, en.x, ok & 1);
+    nan |= isnan(y[k].x);
+    argmax_combine(bv, bi, y[k].x, c0 + i);
+    double* out = r.out + (long)row * V + c0 + i;
+    if (i + 1 < len) {
+      y[k].y = change(y[k].y, c.y, en.y, ok & 2);
+      nan |= isnan(y[k].y);
+      argmax_combine(bv, bi, y[k].y, c0 + i + 1);
+      if (r.out) __builtin_nontemporal_store(y[k], (MITOK_GLOBAL v2row*)out);
+    } else if (r.out) {
+      *out = y[k].x;
     }
-    const bool ok = !r.allowed || ((words[i >> 5] >> (i & 31)) & 1);
-    if (!ok) y[k] = -INFINITY;
-    nan |= isnan(y[k]);
-    argmax_combine(bv, bi, y[k], c0 + i);
-    if (r.out) __builtin_nontemporal_store(y[k], (MITOK_GLOBAL double*)(r.out + (long)row * V + c0 + i));
   }
   if (__ballot(nan) && lane == 0) set_err(r.err, OE_NAN);
   if (!r.ids) return;
@@ -413,8 +433,8 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
 }
 
 void logit_rules(hipStream_t st, const LogitRules& r) {
-  // us a call, narrow / wide: 32 rows of 32000 (256 wide blocks) 28.8 / 24.9
-  const bool wide = (long)((r.V + LR_WIDE - 1) / LR_WIDE) * r.rows >= 256;
+  // us a call, narrow / wide: 32 rows of 32000 (512 wide blocks) 28.8 / 24.6
+  const bool wide = (long)((r.V + LR_WIDE - 1) / LR_WIDE) * r.rows >= 512;
   const int chunks = wide ? (r.V + LR_WIDE - 1) / LR_WIDE : logit_chunks(r.V);
   for (int row0 = 0; row0 < r.rows; row0 += 32768) {  // a counter per row of a launch
     const dim3 grid(chunks, std::min(r.rows - row0, 32768));

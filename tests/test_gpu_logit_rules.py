@@ -98,6 +98,29 @@ def test_formula(net, R, V, H, nb, mask):
     assert none is None and np.array_equal(ids, ids2)
 
 
+@pytest.mark.parametrize("R,V,H,nb,mask", [(600, 2001, 9, 5, True), (300, 4097, 30, 3, True), (40, 27001, 300, 0, False)])
+def test_many_rows_of_odd_sizes(net, R, V, H, nb, mask):
+    """Rows that start between two 16-byte words, chunks that end in one token."""
+    test_formula(net, R, V, H, nb, mask)
+
+
+@pytest.mark.parametrize("R,V", [(2, 5000), (200, 6001)])
+def test_logits_that_start_between_two_words(net, R, V):
+    c = make(R, R, V, 20)
+    want = formula(c)
+    host = [np.concatenate([[7.0], c["x"].ravel(), [7.0]]), c["hist"].astype(np.int32), c["pen"]]
+    d = [ra.DeviceBuffer(a.nbytes) for a in host]
+    ids = ra.DeviceBuffer(4 * R)
+    for b, a in zip(d, host):
+        b.upload(a)
+    net.process_logits_device(d[0].ptr + 8, R, V, out=d[0].ptr + 8, ids=ids, history=d[1], max_history=20, penalties=d[2])
+    got = d[0].download(R * V + 2, float)
+    assert got[0] == got[-1] == 7.0
+    check(c, got[1:-1].reshape(R, V), ids.download(R, np.uint32), want)
+    for b in [*d, ids]:
+        b.free()
+
+
 def test_no_rules_is_greedy_decoding(net):
     x = np.round(np.random.default_rng(1).standard_normal((40, 5003)) * 4) / 4  # ties: the last one
     out, ids = net.process_logits(x)
