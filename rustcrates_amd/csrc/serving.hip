@@ -27,6 +27,7 @@ __device__ __forceinline__ unsigned long long order_key(double w) {
 // each, not by the 8 bytes of a slot: 48 heads of 2048 slots 11.5 us, 256 of
 // up to 512 7.5, 4 of 320 5.3.  Sorting would order what only has to be
 // divided; quartering the range instead of halving it saves half the barriers.
+// Blocks of 8 waves take 6.2 us for the 320, of 16 waves 18.6 for the 2048.
 template <int NK>
 __global__ __launch_bounds__(256) void k_evict_select(EvictSelect e, OpTable own) {
   __shared__ unsigned long long ext[2][4];
