@@ -372,7 +372,7 @@ int mitok_tree_accept(mitok_network* net, const uint32_t* path, const uint32_t* 
  * order, to slots 0, 1, ... of the output arrays [batch][heads][out_ctx]...;
  * slots behind them stay as they were.  In place: d_k_out == d_k_cache,
  * d_v_out == d_v_cache, d_weights_out == d_weights and out_ctx == max_ctx.
- * d_kept [batch][heads][keep] or NULL: the slots kept, then MITOK_NO_ROW.
+ * d_kept [batch][heads][keep] (keep <= 2^30) or NULL: the slots kept, then MITOK_NO_ROW.
  * out_lens (host) [batch]: rows kept. */
 int mitok_evict_rows_device(mitok_network* net, const double* d_k_cache, const double* d_v_cache,
                             const double* d_weights, const uint32_t* kv_lens, uint32_t batch, uint32_t heads,
@@ -395,6 +395,7 @@ int mitok_evict_rows(mitok_network* net, uint32_t batch, uint32_t keep, uint32_t
  *     presence, frequency); max_history 0: neither is read
  *   d_bias_ids, d_bias [rows][max_bias]: of equal ids the last entry counts
  *   d_allowed [rows][(vocab + 31) / 32] bits (t at bit t % 32 of word t / 32) or NULL
+ *   each size at most 2^30
  * MITOK_NO_TOKEN entries of the history and the ids are skipped; another id
  * >= vocab is MITOK_ERR_ARG.  d_out [rows][vocab] or NULL: the logits after
  * the rules (d_logits itself: in place).  d_out_ids [rows] or NULL: the last

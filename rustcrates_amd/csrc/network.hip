@@ -4089,6 +4089,7 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
     longest = std::max(longest, kv_lens[b]);
   }
   const uint32_t stay = std::min(longest, keep);
+  if (d_kept && keep > OP_MAX_CTX) return fail(ERR_ARG, "evict: %u kept slots of a head to list, at most 2^30", keep);
   if (stay > out_ctx) return fail(ERR_ARG, "evict: %u rows do not fit out_ctx %u", stay, out_ctx);
   TRY(set_device(n));
   const size_t cb = times({B, heads, ctx, dh, sizeof(double2)}), co = times({B, heads, out_ctx, dh, sizeof(double2)});
@@ -4252,9 +4253,9 @@ int mitok_process_logits_device(mitok_network* n, const double* d_logits, uint32
                                 const uint32_t* d_allowed, double* d_out, uint32_t* d_out_ids) {
   if (!n || !d_logits || !rows || !V) return fail(ERR_ARG, "process_logits: bad arguments");
   if (!d_out && !d_out_ids) return fail(ERR_ARG, "process_logits: neither logits nor ids wanted");
-  if (rows > (uint32_t)INT32_MAX || V > (uint32_t)INT32_MAX - 64 || max_history > (uint32_t)INT32_MAX ||
-      max_bias > (uint32_t)INT32_MAX)
-    return fail(ERR_ARG, "process_logits: a size beyond 31 bits");
+  // a block's next step behind the last row, token or entry still fits the kernel's 31 bits
+  if (std::max({rows, V, max_history, max_bias}) > 1u << 30)
+    return fail(ERR_ARG, "process_logits: a size above 2^30 (indices have 31 bits)");
   if (max_history && (!d_history || !d_penalties)) return fail(ERR_ARG, "process_logits: a history needs its tokens and penalties");
   if (max_bias && (!d_bias_ids || !d_bias)) return fail(ERR_ARG, "process_logits: biases need their ids and values");
   TRY(set_device(n));

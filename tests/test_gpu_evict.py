@@ -130,6 +130,12 @@ def test_batches_and_heads_that_a_launch_cannot_hold(net, B, H):
         x.free()
 
 
+def test_a_list_of_kept_slots_past_the_kernels_indices(net):
+    with ra.DeviceBuffer(4096) as x, pytest.raises(ra.MitokError, match="2\\^30") as e:
+        net.evict_rows_device(x, x, x, [1], 1, 1, 1, 2 ** 30 + 1, 0, 0, x, x, x, 1, kept=x)
+    assert e.value.code == 1
+
+
 def test_refusals(net):
     c = make(1, 2, 2, 8, 40, [40, 30])
     dev = {x: ra.DeviceBuffer(c[x].nbytes) for x in "kvw"}

@@ -177,6 +177,15 @@ def test_repeated_entries(net):
     assert np.count_nonzero(out) == 3
 
 
+@pytest.mark.parametrize("big", ["rows", "vocab", "max_history", "max_bias"])
+def test_sizes_past_the_kernels_indices(net, big):
+    """A step past the last entry would wrap 31 bits: refused before any array is looked at."""
+    with ra.DeviceBuffer(64) as d:
+        with pytest.raises(ra.MitokError, match="2\\^30") as e:
+            net.process_logits_device(d, ids=d.ptr + 32, **{**dict(rows=1, vocab=2), big: 2 ** 30 + 1})
+        assert e.value.code == 1
+
+
 def test_refusals(net):
     c = make(2, 2, 50, 4, 3, True)
 
