@@ -461,6 +461,16 @@ static void drop_graph(Net* n) {
   n->graph = nullptr;
 }
 
+// The caches' rows no longer count, nor what hangs on them: lengths, weights
+// and a pending tree.
+static void drop_caches(Net* n) {
+  n->cache_valid = false;
+  n->cache_B = 0;
+  n->kv_len_h.clear();
+  n->tree_valid = false;
+  n->aw_len.clear();
+}
+
 // Gives up the saved forward products; the bytes they held.
 static size_t drop_saved(Net* n) {
   size_t held = 0;
@@ -1980,7 +1990,7 @@ static int upload_c(Net* n, DevBuf& b, const double* src, size_t count, double2 
 
 static int add_layer(Net* n, Layer* L) {
   n->layers.emplace_back(L);
-  n->cache_valid = false;
+  drop_caches(n);
   drop_graph(n);
   return OK;
 }
@@ -2183,7 +2193,7 @@ int mitok_init_seeded(mitok_network* n, uint64_t seed) {
   }
   HIP_TRY(hipGetLastError());
   HIP_TRY(hipStreamSynchronize(st));
-  n->cache_valid = false;
+  drop_caches(n);
   return OK;
 }
 
@@ -2203,7 +2213,7 @@ int mitok_init_embedding_wavelet(mitok_network* n, uint32_t layer, uint64_t seed
                                         stream_key(seed, stream_id(layer, 0xFFF)), kern.as<double2>(), 64);
   if (rc == ERR_HIP) return fail(ERR_HIP, "embedding wavelet init: %s", hipGetErrorString(hipGetLastError()));
   if (rc) return fail(rc, "embedding wavelet init: the CMOR integral");
-  n->cache_valid = false;
+  drop_caches(n);
   return check_err_word(n);
 }
 
@@ -2263,11 +2273,7 @@ int mitok_get_tensor(mitok_network* n, uint32_t layer, uint32_t slot, double* ou
 
 int mitok_reset(mitok_network* n) {
   if (!n) return fail(ERR_ARG, "null network");
-  n->cache_valid = false;
-  n->cache_B = 0;
-  n->kv_len_h.clear();
-  n->tree_valid = false;
-  n->aw_len.clear();
+  drop_caches(n);
   return OK;
 }
 

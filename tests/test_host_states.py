@@ -1,0 +1,33 @@
+"""What the serving calls do on caches that are gone, and where a runtime call
+fails half way (host_runtime.py): no GPU."""
+from __future__ import annotations
+
+import pytest
+
+from host_runtime import run
+
+TREE = """
+net = stack()
+prompt = np.arange(2, 12, dtype=np.uint32).reshape(2, 5)
+net.prefill(prompt)
+net.tree_step([[3, 4, 5]] * 2, [[-1, 0, 0]] * 2, weigh_nodes=1)
+"""
+
+
+def test_the_host_runtime_stands_in_for_the_gpu():
+    run(TREE + """
+net.tree_accept([[0, 2]] * 2)  # a gap: rows move
+assert launches("k_cache_pack") == 1 and launches("k_tree_split") == 1 and calls("hipMalloc") > 10
+assert net.evict_rows(2, 4, 1, 1).tolist() == [4, 4]
+""")
+
+
+@pytest.mark.parametrize("drop", ["net.add_self_attention(2, 16, 40, 1e-12)", "net.init_seeded(2)"])
+def test_dropped_caches_take_the_pending_tree_with_them(drop):
+    run(TREE + drop + """
+moved = launches("k_cache_pack")
+refused(3, "without a tree_step", lambda: net.tree_accept([[0, 2]] * 2))
+assert launches("k_cache_pack") == moved
+refused(3, "no KV cache", lambda: net.evict_rows(2, 4))
+refused(3, "no KV cache", lambda: net.decode_step())
+""")
