@@ -541,10 +541,11 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
     double* to = a.weights + (long)bh * a.ctx + t;
     *to = t < L ? *to + w : w;
   };
-  // a slot that a node does not see has score -inf; a node without any weight
-  // (maximum -inf) is NaN at the slots it sees, as its output is
+  // a slot that a node does not see has score -inf; a node without a softmax
+  // (a score NaN or infinite, its sum NaN, or none above -inf, its sum 0) is NaN
+  // at the slots it sees, as its output is
   const auto weight = [&](int t, int i, double x) {
-    if (x != -INFINITY || sM[i] != -INFINITY) return exp(x - sM[i]) * sR[i];
+    if (x != -INFINITY || isfinite(sR[i])) return exp(x - sM[i]) * sR[i];
     const int j = t - L;
     const auto* seen = op_array<unsigned long long>(a.tab, own, a.seen) + ((long)b * a.n + i) * a.words;
     const bool see = j < 0 || ((seen[j >> 6] >> (j & 63)) & 1);
