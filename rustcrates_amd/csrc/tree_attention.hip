@@ -128,15 +128,15 @@ struct TreeRun {
   // then), which after the first tiles hardly happens: no maximum across the
   // lanes and no rescaling, which costs as much as 8 MFMAs (double arithmetic
   // and double MFMAs take turns on a SIMD: 4 cycles an operation beside 64).
-  template <bool LAZY>
+  // Each node goes by its own scores, so its bits do not depend on the others'.
   __device__ __forceinline__ void soften(v4d& s) {
     const double top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
-    if (!LAZY || __ballot(top > m + 8.0)) {
+    if (__ballot(top > m + 8.0)) {
       double x, y;
       pair16_f64(top, x, y);
       pair32_f64(fmax(x, y), x, y);
-      const double mn = fmax(m, fmax(x, y));
-      const double keep = mn == -INFINITY ? 0.0 : exp(m - mn);
+      const double most = fmax(x, y), mn = most > m + 8.0 ? most : m;
+      const double keep = mn == m ? 1.0 : exp(m - mn);
       m = mn;
       l *= keep;
 #pragma unroll
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
     tree_scores(a, p, ws, at, t, kq, i, s);
     const bool more = t + 16 * KG < t1;
     if (more) load_keys(t + 16 * KG);
-    run.template soften<true>(s);
+    run.soften(s);
     const bool drafted = t + 16 > at.L;
     bool fine = true;
     if (PRE && drafted) {
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
 #pragma unroll
     for (int e = 0; e < 4; ++e) s[e] = (vis >> e & 1) && t + 4 * e + kq < t1 ? s[e] + z[e] + bf[e] : -INFINITY;
     tree_scores(a, p, ws, at, t, kq, i, s);
-    run.template soften<true>(s);
+    run.soften(s);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
