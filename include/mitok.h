@@ -202,9 +202,10 @@ int mitok_generate(mitok_network* net, const uint32_t* prompt, const uint32_t* l
  *   greedy id of each sequence's last prompt row; out_logits [batch][vocab]
  *   Re-logits of that row, or NULL.
  * mitok_decode_step: feeds ids [batch] (NULL: the ids the previous prefill or
- *   step returned, already on the device) at position = each sequence's KV
- *   length, appends to the caches; out_ids [batch] = the next greedy ids;
- *   out_logits [batch][vocab] or NULL.  batch must equal the prefill's.
+ *   step returned, already on the device; MITOK_ERR_STATE where a mitok_predict
+ *   used the caches last) at position = each sequence's KV length, appends to
+ *   the caches; out_ids [batch] = the next greedy ids; out_logits
+ *   [batch][vocab] or NULL.  batch must equal the prefill's.
  * On error the caches are dropped (prefill again). */
 int mitok_prefill(mitok_network* net, const uint32_t* prompt, const uint32_t* lens, uint32_t batch, uint32_t seq,
                   uint32_t* out_ids, double* out_logits);

@@ -398,6 +398,9 @@ struct mitok_network {
   mitok::DevBuf pos_off_d;
   bool pos_off = false;
   std::vector<int> pos_off_h;  // the same on the host, while pos_off
+  // whether kv_len_d holds kv_len_h, and dec_ids_d each sequence's next id: a
+  // predict on the caches sets neither
+  bool lens_on_device = false, ids_on_device = false;
   // the last mitok_tree_step's nodes behind the committed rows, until another
   // call uses the cache: nodes per sequence, their parents and counts
   bool tree_valid = false;
@@ -502,6 +505,21 @@ static int reserve(Net* n, DevBuf& b, size_t bytes) {
     n->ws_generation++;
     drop_graph(n);
   }
+  return OK;
+}
+
+// Room in a buffer whose contents belong to the caches and outlast calls: they
+// move along.
+static int reserve_kept(Net* n, DevBuf& b, size_t bytes) {
+  if (!b.p || bytes <= b.bytes) return reserve(n, b, bytes);
+  DevBuf wide;
+  TRY(alloc(n, wide, bytes));
+  HIP_TRY(hipMemcpyAsync(wide.p, b.p, b.bytes, hipMemcpyDeviceToDevice, n->stream));
+  HIP_TRY(hipStreamSynchronize(n->stream));
+  std::swap(b.p, wide.p);
+  std::swap(b.bytes, wide.bytes);
+  n->ws_generation++;
+  drop_graph(n);
   return OK;
 }
 
@@ -741,10 +759,11 @@ static int prepare(Net* n, const Spec& sp) {
     TRY(reserve(n, n->dp0, 8 * B * dm.dmax * c16));
     TRY(reserve(n, n->dp1, 8 * B * dm.dmax * c16));
   }
-  TRY(reserve(n, n->kv_len_d, (size_t)sp.B * sizeof(int)));
-  if (n->pos_off) TRY(reserve(n, n->pos_off_d, (size_t)sp.B * sizeof(int)));
+  // a stateless pass of any batch leaves the caches' lengths, offsets and next ids
+  TRY(reserve_kept(n, n->kv_len_d, (size_t)sp.B * sizeof(int)));
+  if (n->pos_off) TRY(reserve_kept(n, n->pos_off_d, (size_t)sp.B * sizeof(int)));
   TRY(reserve(n, n->ones_d, std::max<size_t>(rows, sp.B) * sizeof(uint32_t)));
-  TRY(reserve(n, n->dec_ids_d, (size_t)sp.B * sizeof(uint32_t)));
+  TRY(reserve_kept(n, n->dec_ids_d, (size_t)sp.B * sizeof(uint32_t)));
   return OK;
 }
 
@@ -2462,6 +2481,7 @@ static void end_call(Net* n, const Spec& sp, const uint32_t* lens) {
   } else if (sp.mode == MODE_CACHED) {
     for (uint32_t b = 0; b < (uint32_t)sp.B; ++b) n->kv_len_h[b] += 1;
   }
+  if (sp.mode != MODE_STATELESS) n->lens_on_device = n->ids_on_device = false;
 }
 
 // out may be null only for a stateless pass of every row (mitok_predict_targets
@@ -2762,6 +2782,7 @@ static int run_prompt(Net* n, const uint32_t* prompt, const uint32_t* lens, uint
   const void* kvsrc = n->wstages.empty() ? n->lens_d.p : n->wstages.back()->lens.p;
   HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, kvsrc, B * sizeof(int), hipMemcpyDeviceToDevice, st));
   end_call(n, pre, lens);
+  n->lens_on_device = n->ids_on_device = true;
   return OK;
 }
 
@@ -2928,6 +2949,8 @@ static int decode_step_impl(Net* n, const uint32_t* ids, uint32_t B, uint32_t* o
   if (want_logits) TRY(reserve(n, n->logit_hist_d, (size_t)B * V * sizeof(double)));
   TRY(ensure_rope_for(n, 0, dec.last, (int)std::max<uint32_t>(rope_positions_needed(n), kv_max + 1)));
   bind_decode_inputs(n, dec);
+  if (!n->lens_on_device)
+    HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, n->kv_len_h.data(), B * sizeof(int), hipMemcpyHostToDevice, st));
   if (ids) {
     // the caller's ids are staged in ids_d (a stream-ordered copy of a host buffer
     // that the call holds until its synchronisation below), then moved into place
@@ -2953,6 +2976,7 @@ static int decode_step_impl(Net* n, const uint32_t* ids, uint32_t B, uint32_t* o
   collect_timing(n);
   TRY(check_err_word(n));
   for (uint32_t b = 0; b < B; ++b) n->kv_len_h[b] += 1;
+  n->lens_on_device = n->ids_on_device = true;
   return OK;
 }
 
@@ -2970,6 +2994,7 @@ int mitok_decode_step(mitok_network* n, const uint32_t* ids, uint32_t B, uint32_
     for (uint32_t b = 0; b < B; ++b)
       if (ids[b] >= V0) return fail(ERR_ARG, "No token embedding found: token id %u >= vocab %u (embedding_layer.rs:305)", ids[b], V0);
   }
+  if (!ids && !n->ids_on_device) return fail(ERR_STATE, "decode_step without ids: no call has left any on these caches");
   const int rc = decode_step_impl(n, ids, B, out_ids, out_logits);
   if (rc) (void)mitok_reset(n);
   return rc;
@@ -3922,8 +3947,8 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
   TRY(upload(n, n->ids_d, padded.data(), rows * sizeof(uint32_t)));
   TRY(upload(n, n->mask_d, mask.data(), rows * sizeof(uint32_t)));
   TRY(upload(n, n->pos_d, pos.data(), rows * sizeof(int)));
-  std::vector<int> kv(n->kv_len_h.begin(), n->kv_len_h.end());
-  TRY(upload(n, n->kv_len_d, kv.data(), B * sizeof(int)));
+  TRY(upload(n, n->kv_len_d, n->kv_len_h.data(), B * sizeof(int)));
+  n->lens_on_device = true;
   if (weigh && most > 0) {
     HIP_TRY(hipMemcpyAsync(n->tree_rng.p, from.data(), B * sizeof(int), hipMemcpyHostToDevice, st));
     HIP_TRY(hipMemcpyAsync(n->tree_rng.as<int>() + B, to.data(), B * sizeof(int), hipMemcpyHostToDevice, st));
@@ -4062,6 +4087,8 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
   pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, (const int*)(dp + bp) + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
   HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, then, B * sizeof(int), hipMemcpyHostToDevice, st));  // decode steps read it
   TRY(op_finish(n));
+  n->lens_on_device = true;
+  if (std::all_of(path_lens, path_lens + B, [](uint32_t len) { return len > 0; })) n->ids_on_device = true;
   const bool weighed = !n->aw_len.empty();
   for (uint32_t b = 0; b < B; ++b) {
     const bool whole = weighed && n->aw_len[b] == n->kv_len_h[b];
@@ -4246,6 +4273,7 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
     }
     n->pos_off_h.assign(off, off + B);
     for (uint32_t b = 0; b < B; ++b) n->kv_len_h[b] = (uint32_t)rows[b];
+    n->lens_on_device = true;
     n->aw_len = n->kv_len_h;
   }
   if (out_lens) memcpy(out_lens, n->kv_len_h.data(), B * sizeof(uint32_t));
