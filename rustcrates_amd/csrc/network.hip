@@ -3729,15 +3729,17 @@ static int op_hand_over(Net* n, size_t bytes, OpTable& own, const char** tab) {
   return OK;
 }
 
-// Waits for the network's stream and turns the operators' error words into a code.
+// Waits for the network's stream and turns the operators' error words into a
+// code.  Whatever comes first, the stream is idle and the words are clear.
 static int op_finish(Net* n) {
-  HIP_TRY(hipGetLastError());
-  HIP_TRY(hipStreamSynchronize(n->stream));
+  const hipError_t launch = hipGetLastError(), wait = hipStreamSynchronize(n->stream);
   uint32_t w[OE_WORDS];
   for (int i = 0; i < OE_WORDS; ++i) {
     w[i] = __atomic_load_n(&n->op_err[i], __ATOMIC_ACQUIRE);
     if (w[i]) __atomic_store_n(&n->op_err[i], 0u, __ATOMIC_RELEASE);
   }
+  HIP_TRY(launch);
+  HIP_TRY(wait);
   if (w[OE_BAD_TOKEN]) return fail(ERR_ARG, "a token id of the history or the biases is outside the vocabulary");
   if (w[OE_BAD_PENALTY]) return fail(ERR_ARG, "penalties must be finite and the repetition penalty above 0");
   if (w[OE_NAN]) return fail(ERR_NAN, "greedy_decoding: NaN in logits (sampling_methods.rs:12)");
