@@ -456,6 +456,7 @@ static const int* rope_offsets(const Net* n) { return n->pos_off ? n->pos_off_d.
 
 static int set_device(Net* n) {
   HIP_TRY(hipSetDevice(n->device));
+  (void)hipGetLastError();  // what the thread's earlier calls left is not this call's
   return OK;
 }
 

@@ -31,3 +31,21 @@ assert launches("k_cache_pack") == moved
 refused(3, "no KV cache", lambda: net.evict_rows(2, 4))
 refused(3, "no KV cache", lambda: net.decode_step())
 """)
+
+
+def test_an_error_of_the_threads_earlier_calls_is_not_a_calls_own():
+    """The runtime keeps the last error of a thread, of whatever made the call, until it is read."""
+    run(TREE + """
+def stale(f):
+    assert hip.hipSetDevice(5) != 0
+    return f()
+stale(lambda: net.tree_step([[3, 4, 5]] * 2, [[-1, 0, 0]] * 2, weigh_nodes=1))
+stale(lambda: net.tree_accept([[0, 2]] * 2))
+stale(lambda: net.decode_step())
+stale(lambda: net.evict_rows(2, 4, 1, 1))
+stale(lambda: net.process_logits(np.zeros((2, 50))))
+stale(lambda: net.predict(prompt, forward_only=False))
+stale(lambda: net.prefill(prompt))
+a = [device(65536) for _ in range(4)]
+stale(lambda: net.tree_attention_device(*a[:3], [3], [[-1]], 1, 4, 8, a[3]))
+""")
