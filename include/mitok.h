@@ -361,7 +361,9 @@ int mitok_tree_step_device(mitok_network* net, const uint32_t* ids, const uint32
 /* Commits the nodes path[b][0 .. path_lens[b]) of the last mitok_tree_step, a
  * chain from a node without a parent downwards (path [batch][max_path]; 0
  * nodes: none): their rows become the cache's next ones.  A following
- * mitok_decode_step(NULL) feeds the greedy id after the last of them. */
+ * mitok_decode_step(NULL) feeds the greedy id after the last of them.  Where
+ * the runtime fails once rows move (here and in mitok_evict_rows) the caches
+ * are dropped. */
 int mitok_tree_accept(mitok_network* net, const uint32_t* path, const uint32_t* path_lens, uint32_t batch,
                       uint32_t max_path);
 

@@ -3730,21 +3730,36 @@ static int op_hand_over(Net* n, size_t bytes, OpTable& own, const char** tab) {
   return OK;
 }
 
+// The operators' error words, cleared; the stream is idle.
+static void take_words(Net* n, uint32_t (&w)[OE_WORDS]) {
+  for (int i = 0; i < OE_WORDS; ++i) {
+    w[i] = __atomic_load_n(&n->op_err[i], __ATOMIC_ACQUIRE);
+    if (w[i]) __atomic_store_n(&n->op_err[i], 0u, __ATOMIC_RELEASE);
+  }
+}
+
 // Waits for the network's stream and turns the operators' error words into a
 // code.  Whatever comes first, the stream is idle and the words are clear.
 static int op_finish(Net* n) {
   const hipError_t launch = hipGetLastError(), wait = hipStreamSynchronize(n->stream);
   uint32_t w[OE_WORDS];
-  for (int i = 0; i < OE_WORDS; ++i) {
-    w[i] = __atomic_load_n(&n->op_err[i], __ATOMIC_ACQUIRE);
-    if (w[i]) __atomic_store_n(&n->op_err[i], 0u, __ATOMIC_RELEASE);
-  }
+  take_words(n, w);
   HIP_TRY(launch);
   HIP_TRY(wait);
   if (w[OE_BAD_TOKEN]) return fail(ERR_ARG, "a token id of the history or the biases is outside the vocabulary");
   if (w[OE_BAD_PENALTY]) return fail(ERR_ARG, "penalties must be finite and the repetition penalty above 0");
   if (w[OE_NAN]) return fail(ERR_NAN, "greedy_decoding: NaN in logits (sampling_methods.rs:12)");
   return OK;
+}
+
+// A call that failed once it had queued work on the caches: waits for what is
+// queued, and the caches, part-way moved, no longer count.
+static int drop_moved(Net* n, int rc) {
+  uint32_t w[OE_WORDS];
+  (void)hipStreamSynchronize(n->stream);
+  take_words(n, w);
+  drop_caches(n);
+  return rc;
 }
 
 // per-chunk argmax partials of `rows` logit rows (in am_v, am_i)
@@ -3894,9 +3909,16 @@ int mitok_tree_attention_device(mitok_network* n, const double* d_q, const doubl
   return op_finish(n);
 }
 
+// host arrays that the pass's copies read: they live until the stream is idle
+struct TreeStaged {
+  std::vector<uint32_t> padded, mask;
+  std::vector<int> pos, from, to;
+};
+
 // The next tokens' tree through every layer (mitok_tree_step).
 static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts, uint32_t B,
-                          uint32_t nodes, uint32_t weigh, uint32_t* out_ids, double* out_logits, double* d_logits) {
+                          uint32_t nodes, uint32_t weigh, uint32_t* out_ids, double* out_logits, double* d_logits,
+                          TreeStaged& staged) {
   hipStream_t st = n->stream;
   const uint32_t V = n->layers[n->layers.size() - 2]->d_out;
   const size_t rows = (size_t)B * nodes;
@@ -3912,7 +3934,9 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
   TreePass tree;
   const int* depth = nullptr;
   // the rows whose weights are kept so far, zero for those appended since
-  std::vector<int> from(B), to(B);
+  std::vector<int>&from = staged.from, &to = staged.to;
+  from.resize(B);
+  to.resize(B);
   int most = 0;
   if (weigh) {
     for (auto& L : n->layers)
@@ -3934,8 +3958,11 @@ static int tree_step_impl(Net* n, const uint32_t* ids, const uint32_t* parents, 
       shapes.push_back({(int)A->heads, (int)A->dh});
     }
   TRY(stage_tree(n, n->kv_len_h.data(), parents, counts, B, nodes, weigh, shapes, tree, &depth));
-  std::vector<uint32_t> padded(rows), mask(rows);
-  std::vector<int> pos(rows);
+  std::vector<uint32_t>&padded = staged.padded, &mask = staged.mask;
+  std::vector<int>& pos = staged.pos;
+  padded.resize(rows);
+  mask.resize(rows);
+  pos.resize(rows);
   int maxpos = 0;
   for (uint32_t b = 0; b < B; ++b)
     for (uint32_t i = 0; i < nodes; ++i) {
@@ -4017,9 +4044,9 @@ static int tree_step_checked(Net* n, const uint32_t* ids, const uint32_t* parent
     TRY(check_device_array(n, d_logits, times({B, nodes, V, sizeof(double)}), 8, "logits"));
     TRY(behind_default_stream(n));
   }
-  const int rc = tree_step_impl(n, ids, parents, counts, B, nodes, weigh, out_ids, out_logits, d_logits);
-  if (rc) (void)mitok_reset(n);
-  return rc;
+  TreeStaged staged;
+  const int rc = tree_step_impl(n, ids, parents, counts, B, nodes, weigh, out_ids, out_logits, d_logits, staged);
+  return rc ? drop_moved(n, rc) : OK;
 }
 
 int mitok_tree_step(mitok_network* n, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts, uint32_t B,
@@ -4031,6 +4058,38 @@ int mitok_tree_step_device(mitok_network* n, const uint32_t* ids, const uint32_t
                            uint32_t B, uint32_t nodes, uint32_t weigh_nodes, double* d_logits) {
   if (!d_logits) return fail(ERR_ARG, "null argument");
   return tree_step_checked(n, ids, parents, counts, B, nodes, weigh_nodes, nullptr, nullptr, d_logits);
+}
+
+// Moves the paths' rows together in every layer's cache and sets the device's
+// lengths and next ids (`tab`: mitok_tree_accept's table on the device, `then`:
+// its lengths on the host).
+static int move_paths(Net* n, uint32_t B, uint32_t cols, int most, const uint32_t* tab, const int* then) {
+  hipStream_t st = n->stream;
+  const size_t bp = (size_t)B * cols;
+  const OpTable none = {};
+  for (auto& L : n->layers) {
+    if (L->kind != K_SELF_ATTENTION || !most) continue;
+    auto* A = (SelfAttentionLayer*)L.get();
+    CacheMove m;
+    m.k = m.ko = A->kc.as<double2>();
+    m.v = m.vo = A->vc.as<double2>();
+    if (!n->aw_len.empty()) m.w = m.wo = A->aw.as<double>();
+    m.B = (int)B;
+    m.H = (int)A->heads;
+    m.dh = (int)A->dh;
+    m.ctx = m.ctx_out = A->max_ctx;
+    m.tab = (const char*)tab;
+    m.based = true;
+    m.base = (uint32_t)((bp + B) * sizeof(int));
+    m.idx = tab;
+    m.idx_b = cols;
+    m.rows = (uint32_t)(bp * sizeof(int));
+    m.rows_max = most;
+    cache_move(st, m, none);
+  }
+  pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, (const int*)(tab + bp) + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
+  HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, then, B * sizeof(int), hipMemcpyHostToDevice, st));  // decode steps read it
+  return op_finish(n);
 }
 
 int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* path_lens, uint32_t B, uint32_t max_path) {
@@ -4049,7 +4108,6 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
     }
   }
   TRY(set_device(n));
-  hipStream_t st = n->stream;
   // [path | rows moved | committed rows | last node | rows then]; a path without gaps stays where it is
   const size_t bp = (size_t)B * max_path;
   TRY(op_staging(n, (bp + 4 * (size_t)B) * sizeof(int)));
@@ -4065,31 +4123,7 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
     most = std::max(most, moved[b]);
   }
   TRY(op_upload(n, (bp + 4 * (size_t)B) * sizeof(int)));
-  const uint32_t* dp = n->op_tab.as<uint32_t>();
-  const OpTable none = {};
-  for (auto& L : n->layers) {
-    if (L->kind != K_SELF_ATTENTION || !most) continue;
-    auto* A = (SelfAttentionLayer*)L.get();
-    CacheMove m;
-    m.k = m.ko = A->kc.as<double2>();
-    m.v = m.vo = A->vc.as<double2>();
-    if (!n->aw_len.empty()) m.w = m.wo = A->aw.as<double>();
-    m.B = (int)B;
-    m.H = (int)A->heads;
-    m.dh = (int)A->dh;
-    m.ctx = m.ctx_out = A->max_ctx;
-    m.tab = (const char*)dp;
-    m.based = true;
-    m.base = (uint32_t)((bp + B) * sizeof(int));
-    m.idx = dp;
-    m.idx_b = max_path;
-    m.rows = (uint32_t)(bp * sizeof(int));
-    m.rows_max = most;
-    cache_move(st, m, none);
-  }
-  pick_ids(st, n->tree_ids.as<uint32_t>(), (int)n->tree_n, (const int*)(dp + bp) + 2 * B, (int)B, n->dec_ids_d.as<uint32_t>());
-  HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, then, B * sizeof(int), hipMemcpyHostToDevice, st));  // decode steps read it
-  TRY(op_finish(n));
+  if (const int rc = move_paths(n, B, max_path, most, n->op_tab.as<uint32_t>(), then)) return drop_moved(n, rc);
   n->lens_on_device = true;
   if (std::all_of(path_lens, path_lens + B, [](uint32_t len) { return len > 0; })) n->ids_on_device = true;
   const bool weighed = !n->aw_len.empty();
@@ -4199,6 +4233,50 @@ int mitok_evict_rows_device(mitok_network* n, const double* d_k, const double* d
   return OK;
 }
 
+// Evicts from every layer's cache and sets the device's lengths and position
+// offsets (`t`: mitok_evict_rows' table on the device, `rows` and `off`: their
+// host arrays).
+static int evict_layers(Net* n, uint32_t B, uint32_t keep, uint32_t sinks, uint32_t recent, int most, int longest, const int* t,
+                        const int* rows, const int* off) {
+  hipStream_t st = n->stream;
+  const OpTable none = {};
+  for (auto& L : n->layers) {
+    if (L->kind != K_SELF_ATTENTION) continue;
+    auto* A = (SelfAttentionLayer*)L.get();
+    zero_weights(st, A->aw.as<double>(), (int)B, (int)A->heads, A->max_ctx, t + 2 * B, t, most);
+    EvictSelect e;
+    e.w = A->aw.as<double>();
+    e.tab = (const char*)t;
+    e.B = (int)B;
+    e.H = (int)A->heads;
+    e.ctx = A->max_ctx;
+    e.T_max = longest;
+    e.keep = (int)keep;
+    e.sinks = (int)sinks;
+    e.recent = (int)recent;
+    e.kept = n->op_ws.as<uint32_t>();
+    evict_select(st, e, none);
+    CacheMove m;
+    m.tab = e.tab;
+    m.k = m.ko = A->kc.as<double2>();
+    m.v = m.vo = A->vc.as<double2>();
+    m.w = m.wo = A->aw.as<double>();
+    m.B = (int)B;
+    m.H = (int)A->heads;
+    m.dh = (int)A->dh;
+    m.ctx = m.ctx_out = A->max_ctx;
+    m.idx = e.kept;
+    m.idx_b = (long)A->heads * keep;
+    m.idx_h = keep;
+    m.rows = (uint32_t)(B * sizeof(int));
+    m.rows_max = std::min(longest, (int)keep);
+    cache_move(st, m, none);
+  }
+  HIP_TRY(hipMemcpyAsync(n->pos_off_d.p, off, B * sizeof(int), hipMemcpyHostToDevice, st));
+  HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, rows, B * sizeof(int), hipMemcpyHostToDevice, st));
+  return op_finish(n);
+}
+
 int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks, uint32_t recent, uint32_t* out_lens) {
   if (!n) return fail(ERR_ARG, "null network");
   TRY(check_evict(keep, sinks, recent));
@@ -4206,7 +4284,6 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
   if (n->aw_len.empty()) return fail(ERR_STATE, "evict: no tree_step has weighed attention since the prompt");
   if (B != n->cache_B) return fail(ERR_STATE, "cached batch %u != %u", n->cache_B, B);
   TRY(set_device(n));
-  hipStream_t st = n->stream;
   // rows appended by other calls since the last weighed step have no weight yet
   TRY(op_staging(n, 4 * (size_t)B * sizeof(int)));
   int *kv = (int*)n->op_host, *rows = kv + B, *from = rows + B, *off = from + B, most = 0, longest = 0;
@@ -4228,52 +4305,13 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
       if (L->kind == K_SELF_ATTENTION)
         kb = std::max(kb, times({B, ((SelfAttentionLayer*)L.get())->heads, keep, sizeof(uint32_t)}));
     TRY(alloc(n, n->op_ws, kb));
+    TRY(reserve_kept(n, n->pos_off_d, (size_t)B * sizeof(int)));
     TRY(op_upload(n, 4 * (size_t)B * sizeof(int)));
-    const int* t = n->op_tab.as<int>();
-    const OpTable none = {};
-    for (auto& L : n->layers) {
-      if (L->kind != K_SELF_ATTENTION) continue;
-      auto* A = (SelfAttentionLayer*)L.get();
-      zero_weights(st, A->aw.as<double>(), (int)B, (int)A->heads, A->max_ctx, t + 2 * B, t, most);
-      EvictSelect e;
-      e.w = A->aw.as<double>();
-      e.tab = (const char*)t;
-      e.B = (int)B;
-      e.H = (int)A->heads;
-      e.ctx = A->max_ctx;
-      e.T_max = longest;
-      e.keep = (int)keep;
-      e.sinks = (int)sinks;
-      e.recent = (int)recent;
-      e.kept = n->op_ws.as<uint32_t>();
-      evict_select(st, e, none);
-      CacheMove m;
-      m.tab = e.tab;
-      m.k = m.ko = A->kc.as<double2>();
-      m.v = m.vo = A->vc.as<double2>();
-      m.w = m.wo = A->aw.as<double>();
-      m.B = (int)B;
-      m.H = (int)A->heads;
-      m.dh = (int)A->dh;
-      m.ctx = m.ctx_out = A->max_ctx;
-      m.idx = e.kept;
-      m.idx_b = (long)A->heads * keep;
-      m.idx_h = keep;
-      m.rows = (uint32_t)(B * sizeof(int));
-      m.rows_max = std::min(longest, (int)keep);
-      cache_move(st, m, none);
-    }
+    if (const int rc = evict_layers(n, B, keep, sinks, recent, most, longest, n->op_tab.as<int>(), rows, off))
+      return drop_moved(n, rc);
     // later tokens stand where they would without the eviction
     if (!n->pos_off) drop_graph(n);
     n->pos_off = true;
-    TRY(reserve(n, n->pos_off_d, (size_t)B * sizeof(int)));
-    HIP_TRY(hipMemcpyAsync(n->pos_off_d.p, off, B * sizeof(int), hipMemcpyHostToDevice, st));
-    HIP_TRY(hipMemcpyAsync(n->kv_len_d.p, rows, B * sizeof(int), hipMemcpyHostToDevice, st));
-    const int rc = op_finish(n);
-    if (rc) {
-      (void)mitok_reset(n);
-      return rc;
-    }
     n->pos_off_h.assign(off, off + B);
     for (uint32_t b = 0; b < B; ++b) n->kv_len_h[b] = (uint32_t)rows[b];
     n->lens_on_device = true;

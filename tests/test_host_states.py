@@ -49,3 +49,52 @@ stale(lambda: net.prefill(prompt))
 a = [device(65536) for _ in range(4)]
 stale(lambda: net.tree_attention_device(*a[:3], [3], [[-1]], 1, 4, 8, a[3]))
 """)
+
+
+MEND = """
+def state():
+    try:
+        net.decode_step([3, 4])
+    except ra.MitokError as e:
+        assert e.code == 3, e  # dropped
+        return "dropped"
+    return "there"
+"""
+
+
+@pytest.mark.parametrize("name", ["hipMemcpyAsync", "launch", "hipMalloc", "hipStreamSynchronize"])
+@pytest.mark.parametrize("call, moved", [
+    ("net.tree_accept([[0, 2], [0, 1]])", "k_cache_pack"),
+    ("net.evict_rows(2, 4, 1, 1)", "k_cache_pack"),
+    ("net.tree_step([[5, 6]] * 2, [[-1, 0]] * 2, weigh_nodes=2)", "k_tree_split"),
+])
+def test_a_runtime_call_that_fails_half_way(name, call, moved):
+    """Caches that a call may have touched are dropped where it fails, never half
+    moved and still in use; where it finds no room before, they go on as they were."""
+    run(MEND + f"""
+for k in range(1, 60):
+""" + "".join("    " + line + "\n" for line in TREE.strip().splitlines()) + f"""
+    if "evict" in {call!r}:
+        net.tree_accept([[0], [0]])
+        net._lib.mitok_set_graph_mode(net._h, 0)
+    before, lens = launches({moved!r}), calls({name!r})
+    fail({name!r}, k)
+    try:
+        {call}
+    except ra.MitokError as e:
+        fail({name!r}, 0)
+        assert e.code in (2, 5), e
+        if launches({moved!r}) > before or "tree_step" in {call!r}:
+            assert state() == "dropped", k
+        elif {name!r} == "hipMalloc":
+            {call}  # the same call again
+            assert state() == "there"
+        net.close()
+        continue
+    fail({name!r}, 0)
+    assert calls({name!r}) - lens < k
+    break
+else:
+    raise AssertionError("the call never ended well")
+assert k > 1 or {name!r} == "hipMalloc"
+""")
