@@ -4109,21 +4109,22 @@ int mitok_tree_accept(mitok_network* n, const uint32_t* path, const uint32_t* pa
   }
   TRY(set_device(n));
   // [path | rows moved | committed rows | last node | rows then]; a path without gaps stays where it is
-  const size_t bp = (size_t)B * max_path;
+  const uint32_t cols = std::max(1u, *std::max_element(path_lens, path_lens + B));  // of max_path; no more than nodes
+  const size_t bp = (size_t)B * cols;
   TRY(op_staging(n, (bp + 4 * (size_t)B) * sizeof(int)));
   uint32_t* p = (uint32_t*)n->op_host;
   int *moved = (int*)(p + bp), *base = moved + B, *last = base + B, *then = last + B, most = 0;
-  memcpy(p, path, bp * sizeof(uint32_t));
   for (uint32_t b = 0; b < B; ++b) {
-    const uint32_t len = path_lens[b];
-    moved[b] = len && path[(size_t)b * max_path + len - 1] != len - 1 ? (int)len : 0;
+    const uint32_t len = path_lens[b], *from = path + (size_t)b * max_path;
+    std::copy(from, from + cols, p + (size_t)b * cols);
+    moved[b] = len && from[len - 1] != len - 1 ? (int)len : 0;
     base[b] = (int)n->kv_len_h[b];
-    last[b] = len ? (int)path[(size_t)b * max_path + len - 1] : -1;
+    last[b] = len ? (int)from[len - 1] : -1;
     then[b] = base[b] + (int)len;
     most = std::max(most, moved[b]);
   }
   TRY(op_upload(n, (bp + 4 * (size_t)B) * sizeof(int)));
-  if (const int rc = move_paths(n, B, max_path, most, n->op_tab.as<uint32_t>(), then)) return drop_moved(n, rc);
+  if (const int rc = move_paths(n, B, cols, most, n->op_tab.as<uint32_t>(), then)) return drop_moved(n, rc);
   n->lens_on_device = true;
   if (std::all_of(path_lens, path_lens + B, [](uint32_t len) { return len > 0; })) n->ids_on_device = true;
   const bool weighed = !n->aw_len.empty();

@@ -98,3 +98,14 @@ else:
     raise AssertionError("the call never ended well")
 assert k > 1 or {name!r} == "hipMalloc"
 """)
+
+
+def test_a_path_array_wider_than_any_path():
+    """Only the columns in use are staged: offsets into the table keep their 32 bits whatever max_path is."""
+    run(TREE + """
+path = np.zeros((2, 100000), np.uint32)
+path[:, 1] = 2
+host = calls("hipHostMalloc")
+net.tree_accept(path, [2, 1])
+assert calls("hipHostMalloc") == host and launches("k_cache_pack") == 1
+""")
