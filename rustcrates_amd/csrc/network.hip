@@ -791,19 +791,26 @@ static int launch_rc(int rc, const char* what) {
 }
 
 // RoPE table: (cos, sin) of clamp(pos / base^(2i/d), -1, 1) with the host libm,
-// exactly as positional_encoding_layer.rs:188-198 evaluates it.
+// exactly as positional_encoding_layer.rs:188-198 evaluates it.  A table that
+// grows grows to twice its rows at least and computes the new ones: positions
+// go on past max_ctx after evictions, one with every token, and each growth
+// also costs the captured step (3.5 ms for 512 rows of 256 angles on the host,
+// beside a step of 0.25 ms).
 static int ensure_rope_table(Net* n, PositionalEncodingLayer* P, int positions) {
-  if (P->positions >= positions) return OK;
+  const int had = P->positions;
+  if (had >= positions) return OK;
+  positions = (int)std::max<long>(positions, std::min<long>(2L * had, INT32_MAX));
   const uint32_t d = P->d_in, half = d / 2;
-  std::vector<double2> cs((size_t)positions * half);
-  for (int p = 0; p < positions; ++p)
+  std::vector<double2> cs((size_t)(positions - had) * half);
+  for (int p = had; p < positions; ++p)
     for (uint32_t i = 0; i < half; ++i) {
       double theta = (double)p / pow(P->base * 1.0, 2.0 * (double)i / (double)d);
       theta = std::min(1.0, std::max(-1.0, theta));
-      cs[(size_t)p * half + i] = make_double2(cos(theta), sin(theta));
+      cs[(size_t)(p - had) * half + i] = make_double2(cos(theta), sin(theta));
     }
-  TRY(reserve(n, P->cs, cs.size() * sizeof(double2)));
-  HIP_TRY(hipMemcpy(P->cs.p, cs.data(), cs.size() * sizeof(double2), hipMemcpyHostToDevice));
+  TRY(reserve_kept(n, P->cs, (size_t)positions * half * sizeof(double2)));
+  HIP_TRY(hipMemcpy(P->cs.as<double2>() + (size_t)had * half, cs.data(), cs.size() * sizeof(double2), hipMemcpyHostToDevice));
+  if (had) n->ws_generation++, drop_graph(n);  // a captured step holds the number of rows
   P->positions = positions;
   return OK;
 }

@@ -109,3 +109,29 @@ host = calls("hipHostMalloc")
 net.tree_accept(path, [2, 1])
 assert calls("hipHostMalloc") == host and launches("k_cache_pack") == 1
 """)
+
+
+@pytest.mark.parametrize("step", ["net.decode_step([3])", "net.tree_step([[3]], [[-1]]); net.tree_accept([[0]])"])
+def test_positions_past_the_rope_table(step):
+    """A session that evicts and goes on: the table of angles grows a few times,
+    not with every token, and the captured step with it."""
+    run(f"""
+net = stack(rope=True)
+net.prefill(np.arange(2, 32, dtype=np.uint32)[None])
+def evict():
+    net.tree_step([[3]], [[-1]], weigh_nodes=1)
+    net.tree_accept([[0]])
+    net.evict_rows(1, 20, 2, 4)
+pos, before, grown = 30, None, 0
+while pos < 1300:
+    evict()
+    pos += 1
+    for _ in range(15):
+        if pos > 600:  # past the first growth
+            now = calls("hipMalloc"), calls("hipGraphInstantiate")
+            grown += before is not None and now != before
+            before = now
+        {step}
+        pos += 1
+assert 1 <= grown <= 2, grown
+""")
