@@ -403,7 +403,9 @@ int mitok_evict_rows(mitok_network* net, uint32_t batch, uint32_t keep, uint32_t
  * >= vocab is MITOK_ERR_ARG.  d_out [rows][vocab] or NULL: the logits after
  * the rules (d_logits itself: in place).  d_out_ids [rows] or NULL: the last
  * index of the largest one, MITOK_NO_TOKEN if none is above -inf.  A NaN that
- * is allowed is MITOK_ERR_NAN, as in greedy_decoding (sampling_methods.rs:5-18). */
+ * is allowed is MITOK_ERR_NAN, as in greedy_decoding (sampling_methods.rs:5-18).
+ * On an error the outputs have no meaning; logits in place are as they were
+ * where ids or penalties are refused, and changed on MITOK_ERR_NAN. */
 int mitok_process_logits_device(mitok_network* net, const double* d_logits, uint32_t rows, uint32_t vocab,
                                 const uint32_t* d_history, uint32_t max_history, const double* d_penalties,
                                 const uint32_t* d_bias_ids, const double* d_bias, uint32_t max_bias,

@@ -417,6 +417,8 @@ struct mitok_network {
   size_t op_host_bytes = 0;
   mitok::DevBuf op_tab, op_ws;
   uint32_t* op_err = nullptr;
+  mitok::DevBuf op_refused;  // the number of the last call whose logits in place stayed (LogitRules)
+  uint32_t op_calls = 0;
   hipEvent_t op_event = nullptr;
   // the last stateless pass's vocab Linear input rows [head_B * head_S][d]
   // (in act0/act1) and its softmax output (probs), which mitok_backward_head
@@ -1976,9 +1978,11 @@ int mitok_network_create(int device, mitok_network** out) {
   if (!rc && hipEventCreateWithFlags(&n->op_event, hipEventDisableTiming) != hipSuccess)
     rc = fail(ERR_HIP, "hipEventCreate failed");
   if (!rc) rc = n->err_d.reserve(2 * sizeof(uint32_t));
+  if (!rc) rc = n->op_refused.reserve(sizeof(uint32_t));
   if (!rc) rc = n->sync_cnt.reserve((size_t)SYNC_COUNTERS * sizeof(uint32_t));
   if (!rc) {
     fill_u32(n->stream, n->err_d.as<uint32_t>(), 2, 0);
+    fill_u32(n->stream, n->op_refused.as<uint32_t>(), 1, 0);
     fill_u32(n->stream, n->sync_cnt.as<uint32_t>(), SYNC_COUNTERS, 0);
     if (hipStreamSynchronize(n->stream) != hipSuccess) rc = fail(ERR_HIP, "stream sync failed");
   }
@@ -4330,10 +4334,11 @@ int mitok_evict_rows(mitok_network* n, uint32_t B, uint32_t keep, uint32_t sinks
 }
 
 // ---- logits to a token ----
-int mitok_process_logits_device(mitok_network* n, const double* d_logits, uint32_t rows, uint32_t V,
-                                const uint32_t* d_history, uint32_t max_history, const double* d_penalties,
-                                const uint32_t* d_bias_ids, const double* d_bias, uint32_t max_bias,
-                                const uint32_t* d_allowed, double* d_out, uint32_t* d_out_ids) {
+// `keep`: a refusal leaves logits in place as they were
+static int process_logits_impl(Net* n, const double* d_logits, uint32_t rows, uint32_t V, const uint32_t* d_history,
+                               uint32_t max_history, const double* d_penalties, const uint32_t* d_bias_ids,
+                               const double* d_bias, uint32_t max_bias, const uint32_t* d_allowed, double* d_out,
+                               uint32_t* d_out_ids, bool keep) {
   if (!n || !d_logits || !rows || !V) return fail(ERR_ARG, "process_logits: bad arguments");
   if (!d_out && !d_out_ids) return fail(ERR_ARG, "process_logits: neither logits nor ids wanted");
   // a block's next step behind the last row, token or entry still fits the kernel's 31 bits
@@ -4377,8 +4382,22 @@ int mitok_process_logits_device(mitok_network* n, const double* d_logits, uint32
   r.out = d_out;
   r.ids = d_out_ids;
   bind_rules(n, r);
+  if (keep && d_out == d_logits && (hist || bias)) {
+    if (++n->op_calls == 0) n->op_calls = 1;  // the word starts at 0
+    r.refused = n->op_refused.as<uint32_t>();
+    r.call = n->op_calls;
+    logit_check(n->stream, r);
+  }
   logit_rules(n->stream, r);
   return op_finish(n);
+}
+
+int mitok_process_logits_device(mitok_network* n, const double* d_logits, uint32_t rows, uint32_t V,
+                                const uint32_t* d_history, uint32_t max_history, const double* d_penalties,
+                                const uint32_t* d_bias_ids, const double* d_bias, uint32_t max_bias,
+                                const uint32_t* d_allowed, double* d_out, uint32_t* d_out_ids) {
+  return process_logits_impl(n, d_logits, rows, V, d_history, max_history, d_penalties, d_bias_ids, d_bias, max_bias,
+                             d_allowed, d_out, d_out_ids, true);
 }
 
 int mitok_process_logits(mitok_network* n, const double* logits, uint32_t rows, uint32_t V, const uint32_t* history,
@@ -4405,10 +4424,9 @@ int mitok_process_logits(mitok_network* n, const double* logits, uint32_t rows, 
   TRY(put(bv, bias, times({rows, max_bias, sizeof(double)})));
   TRY(put(al, allowed, times({rows, ((size_t)V + 31) / 32, sizeof(uint32_t)})));
   if (out_ids) TRY(alloc(n, id, rows * sizeof(uint32_t)));
-  const int rc = mitok_process_logits_device(n, x.as<double>(), rows, V, h.as<uint32_t>(), max_history, p.as<double>(),
-                                             bi.as<uint32_t>(), bv.as<double>(), max_bias, al.as<uint32_t>(),
-                                             out ? x.as<double>() : nullptr, id.as<uint32_t>());
-  TRY(rc);
+  TRY(process_logits_impl(n, x.as<double>(), rows, V, h.as<uint32_t>(), max_history, p.as<double>(), bi.as<uint32_t>(),
+                          bv.as<double>(), max_bias, al.as<uint32_t>(), out ? x.as<double>() : nullptr, id.as<uint32_t>(),
+                          false));  // in place in a copy
   if (out) HIP_TRY(hipMemcpyAsync(out, x.p, (size_t)rows * V * sizeof(double), hipMemcpyDeviceToHost, n->stream));
   if (out_ids) HIP_TRY(hipMemcpyAsync(out_ids, id.p, rows * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
   HIP_TRY(hipStreamSynchronize(n->stream));

@@ -134,8 +134,14 @@ struct LogitRules {
   int* part_i = nullptr;
   uint32_t* counters = nullptr;  // SYNC_COUNTERS words, zero
   uint32_t* err = nullptr;       // OpErrWord
+  // in place: a device word that holds `call` where logit_check refused the
+  // rules; no logit is changed then
+  uint32_t* refused = nullptr;
+  uint32_t call = 0;
 };
 int logit_chunks(int V);
+// the ids and penalties of every row, before logit_rules changes any (r.refused)
+void logit_check(hipStream_t st, const LogitRules& r);
 void logit_rules(hipStream_t st, const LogitRules& r);
 
 // an array of the table; the same value for every lane of a wave where `i` is
