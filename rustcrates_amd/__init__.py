@@ -195,16 +195,35 @@ def _c128(a, n=None, what="tensor"):
     return a
 
 
+def _u32(a, what, least):
+    """A contiguous uint32 array of whole numbers from `least` to 0xFFFFFFFF (-1 becomes 0xFFFFFFFF)."""
+    if a.dtype != np.uint32:
+        if a.dtype.kind not in "iu" or (a.size and (a.min() < least or a.max() > 0xFFFFFFFF)):
+            raise ValueError(f"{what}: not 32-bit whole numbers")
+        a = (a.astype(np.int64) & 0xFFFFFFFF).astype(np.uint32)
+    return np.ascontiguousarray(a)
+
+
 def _u32_rows(a, what, shape=None):
     """A contiguous uint32 matrix (signed -1 becomes 0xFFFFFFFF)."""
     a = np.asarray(a)
     if a.ndim != 2 or (shape is not None and a.shape != shape):
         raise ValueError(f"{what}: shape {a.shape}, expected {shape or '(rows, columns)'}")
-    if a.dtype != np.uint32:
-        if a.dtype.kind not in "iu" or (a.size and (a.min() < -1 or a.max() > 0xFFFFFFFF)):
-            raise ValueError(f"{what}: not 32-bit whole numbers")
-        a = (a.astype(np.int64) & 0xFFFFFFFF).astype(np.uint32)
-    return np.ascontiguousarray(a)
+    return _u32(a, what, -1)
+
+
+def _u32_lens(a, n, what):
+    """A contiguous uint32 vector of n lengths (None: of any number)."""
+    a = np.asarray(a)
+    if a.ndim != 1 or (n is not None and len(a) != n):
+        raise ValueError(f"{what}: shape {a.shape}, expected ({'batch' if n is None else n},)")
+    return _u32(a, what, 0)
+
+
+def _check_sizes(together):
+    """`together`: a call's sizes, or-ed.  ctypes would cut one of more than 32 bits, or a negative one, to size."""
+    if together >> 32:
+        raise ValueError("a size is negative or above 32 bits")
 
 
 def _u32_vec(a, n, what):
@@ -586,8 +605,9 @@ class Network:
         that the first weigh_nodes nodes pay."""
         par = _u32_rows(parents, "parents")
         B, nodes = par.shape
-        lens = _u32_vec(kv_lens, B, "kv_lens")
-        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        lens = _u32_lens(kv_lens, B, "kv_lens")
+        cnt = None if counts is None else _u32_lens(counts, B, "counts")
+        _check_sizes(heads | head_dim | max_ctx | weigh_nodes | (bias_stride >> 32))
         _check(self._lib.mitok_tree_attention_device(self._h, _dev(d_q), _dev(d_k_cache), _dev(d_v_cache), _dev(bias),
                                                      int(bias_stride), _at(lens), _at(par), _at(cnt), B, nodes,
                                                      heads, head_dim, max_ctx, int(weigh_nodes), _dev(weights),
@@ -601,7 +621,8 @@ class Network:
         ids = _u32_rows(ids, "ids")
         B, nodes = ids.shape
         par = _u32_rows(parents, "parents", (B, nodes))
-        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        cnt = None if counts is None else _u32_lens(counts, B, "counts")
+        _check_sizes(weigh_nodes)
         out = np.empty((B, nodes), np.uint32)
         logits = np.empty((B, nodes, self.vocab), np.float64) if want_logits else None
         _check(self._lib.mitok_tree_step(self._h, _at(ids), _at(par), _at(cnt), B, nodes, int(weigh_nodes),
@@ -613,7 +634,8 @@ class Network:
         ids = _u32_rows(ids, "ids")
         B, nodes = ids.shape
         par = _u32_rows(parents, "parents", (B, nodes))
-        cnt = None if counts is None else _u32_vec(counts, B, "counts")
+        cnt = None if counts is None else _u32_lens(counts, B, "counts")
+        _check_sizes(weigh_nodes)
         _check(self._lib.mitok_tree_step_device(self._h, _at(ids), _at(par), _at(cnt), B, nodes, int(weigh_nodes),
                                                 _dev(d_logits)))
 
@@ -622,7 +644,7 @@ class Network:
         node without a parent downwards (mitok_tree_accept)."""
         path = _u32_rows(path, "path")
         B, most = path.shape
-        lens = np.full(B, most, np.uint32) if path_lens is None else _u32_vec(path_lens, B, "path_lens")
+        lens = np.full(B, most, np.uint32) if path_lens is None else _u32_lens(path_lens, B, "path_lens")
         _check(self._lib.mitok_tree_accept(self._h, _at(path), _at(lens), B, most))
 
     def evict_rows_device(self, d_k_cache, d_v_cache, d_weights, kv_lens, heads, head_dim, max_ctx, keep, sinks, recent,
@@ -631,9 +653,8 @@ class Network:
         the first `sinks`, the last `recent` and those of largest weight, packed
         into the output arrays (mitok_evict_rows_device; the same arrays: in
         place).  kept [B][heads][keep] u32: their slots.  Returns the rows left [B]."""
-        lens = np.ascontiguousarray(kv_lens, dtype=np.uint32)
-        if lens.ndim != 1:
-            raise ValueError(f"kv_lens: shape {lens.shape}, expected (batch,)")
+        lens = _u32_lens(kv_lens, None, "kv_lens")
+        _check_sizes(heads | head_dim | max_ctx | keep | sinks | recent | out_ctx)
         out = np.empty(lens.shape, np.uint32)
         _check(self._lib.mitok_evict_rows_device(self._h, _dev(d_k_cache), _dev(d_v_cache), _dev(d_weights), _at(lens),
                                                  len(lens), heads, head_dim, max_ctx, keep, sinks, recent,
@@ -645,6 +666,7 @@ class Network:
         """evict_rows_device in place on every layer's cache, by the attention
         that tree_step(weigh_nodes > 0) kept (mitok_evict_rows).  Returns the
         rows left per sequence."""
+        _check_sizes(batch | keep | sinks | recent)
         out = np.empty(int(batch), np.uint32)
         _check(self._lib.mitok_evict_rows(self._h, int(batch), int(keep), int(sinks), int(recent), _at(out)))
         return out
@@ -655,6 +677,7 @@ class Network:
         [rows][vocab] f64 logits in device memory, then the greedy ids
         (mitok_process_logits_device has the layouts).  out: the logits after
         the rules; ids [rows] u32; either may be None."""
+        _check_sizes(rows | vocab | max_history | max_bias)
         _check(self._lib.mitok_process_logits_device(self._h, _dev(d_logits), rows, vocab, _dev(history),
                                                      int(max_history), _dev(penalties), _dev(bias_ids), _dev(bias),
                                                      int(max_bias), _dev(allowed), _dev(out), _dev(ids)))
@@ -675,6 +698,8 @@ class Network:
             p = np.ascontiguousarray(penalties, dtype=np.float64)
             if h.shape[0] != R or p.shape != (R, 3):
                 raise ValueError(f"history {h.shape}, penalties {p.shape}: expected ({R}, n) and ({R}, 3)")
+        if bias is not None and bias_ids is None:
+            raise ValueError("bias without bias_ids")
         if bias_ids is not None:
             bi = _u32_rows(bias_ids, "bias_ids")
             bv = np.ascontiguousarray(bias, dtype=np.float64)
