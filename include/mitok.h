@@ -348,7 +348,10 @@ int mitok_tree_attention_device(mitok_network* net, const double* d_q, const dou
  * past counts[b]); out_logits [batch][nodes][vocab] or NULL: its Re-logits.
  * weigh_nodes > 0: the attention that the first weigh_nodes nodes pay is kept
  * per layer, head and cached row, for mitok_evict_rows (1: the root, a token
- * already decided).  The caches' committed rows stay as they are: mitok_tree_accept
+ * already decided).  The step itself adds it, whether its nodes are committed
+ * or not: a step repeated, or one whose tree is dropped, has weighed all the
+ * same (such a step weighs once if the others pass 0).  The caches' committed
+ * rows stay as they are: mitok_tree_accept
  * commits nodes, any other call on the caches drops them.  Every sequence
  * needs room for `nodes` rows.  On an error of the pass the caches are dropped. */
 int mitok_tree_step(mitok_network* net, const uint32_t* ids, const uint32_t* parents, const uint32_t* counts,

@@ -617,7 +617,8 @@ class Network:
         """A tree of drafted tokens [B][nodes] through the stack, on the caches
         (mitok_tree_step): the greedy id after each node [B][nodes] (NO_TOKEN
         past counts[b]) and, with want_logits, its Re-logits [B][nodes][V].
-        tree_accept commits nodes."""
+        tree_accept commits nodes; the first weigh_nodes ones have weighed
+        whether it does or not."""
         ids = _u32_rows(ids, "ids")
         B, nodes = ids.shape
         par = _u32_rows(parents, "parents", (B, nodes))

@@ -49,7 +49,9 @@ FILE_FLAGS = {"gemm_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               # 506 and 417 / 423.  One row behind barriers is slower with it (286 / 282), two equal
               "resident_k4.hip": ["-mllvm", "-disable-machine-licm"],
               "resident_k8.hip": ["-mllvm", "-disable-machine-licm"],
-              # 2 VGPRs spilled at head dim 64 without (exp's constants held across the loop)
+              # 2 VGPRs spilled at head dim 64 without (exp's constants held across the loop); with it
+              # 33 nodes and more still spill 26 at head dims 65 to 127 (11 at 128), and head dims
+              # above 128 278 (272 at 256)
               "tree_attention.hip": ["-mllvm", "-disable-machine-licm"],
               # the wavelet embedding follows the reference's multiply and add order
               "wavelet_init.hip": ["-ffp-contract=off"]}

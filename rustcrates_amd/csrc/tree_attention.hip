@@ -202,7 +202,11 @@ __device__ __forceinline__ void tree_put_sum(const TreeAttn& a, const TreePlan& 
 // 725 MB in 140 us, 5.1 TB/s, as a large copy runs); with 16 nodes 182 MB in 51
 // us, a block's start and end (8 us of its 50) and the longest sequence.  One
 // node takes the matrix instructions too: the 15 unused rows cost nothing that
-// the memory does not hide.
+// the memory does not hide.  Above head dim 64 a tile's rows no longer fit the
+// registers ahead of it and are requested among its products, which wait for
+// them: 32 sequences of 16 nodes, 8 heads of 128, 362 MB in 210 us.  Above 128
+// the outputs alone fill the registers (272 VGPRs spilled): 4 heads of 256, the
+// same bytes in 320 us.
 template <int DHP, int NG, bool FULL>
 __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int KG = 4 / NG;       // waves that share a node group's slots
@@ -362,8 +366,9 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 // wait in registers.  Bound by double MFMAs and the softmax's double arithmetic,
 // which take turns on a SIMD: 4 sequences of 12 heads, 1964 to 2048 slots and 64
 // nodes at head dim 64 take 92 us, 47% of it MFMAs (the padded products alone
-// are 44 us).  Tiles of a wave's own would be read four
-// times through the caches.
+// are 44 us).  Head dim 128, whose queries and outputs leave 11 VGPRs spilled
+// (26 padded) at one wave a SIMD, takes 222 us for twice the products.  Tiles of
+// a wave's own would be read four times through the caches.
 template <int DHP, bool FULL>
 __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn a, TreePlan p, TreeWs ws, OpTable own) {
   constexpr int U = DHP / 4, CT = DHP / 16;
@@ -585,7 +590,8 @@ __global__ __launch_bounds__(256) void k_tree_join(TreeAttn a, TreePlan p, TreeW
 // Whole rounds run at the average length, the last at its longest.  Measured,
 // us, head dim 64: 32 sequences of 144 to 512 slots and 16 nodes 69 in chunks of
 // 64, 57 of 128, 47 of 256, 50 whole; 64 of 400 to 512 and one node 157 of 128,
-// 146 of 256, 149 whole.
+// 146 of 256, 149 whole.  Other widths go by the same figures in proportion,
+// which nothing was fitted to there.
 TreePlan tree_plan(const TreeAttn& a, const int* kv_len, const int* count, std::vector<int>& lists) {
   TreePlan p;
   p.ng = a.n <= 16 || a.dh > 128 ? 1 : a.n <= 32 ? 2 : 4;
