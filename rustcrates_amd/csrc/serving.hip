@@ -318,8 +318,7 @@ __device__ __forceinline__ bool bad_penalties(const LogitRules& r, long row) {
 // Logits in place would be lost to a caller whose ids or penalties are refused,
 // so those are looked at before the first of them changes: 2.5 us more for one row
 // of 4096 and a history of 48, 3.7 for 512 rows of 50280 and 512.  Bound by the
-// launch; the word holds the number of the call, so
-// nothing has to clear it.
+// launch; the word holds the number of the call, so nothing has to clear it.
 __global__ __launch_bounds__(256) void k_logit_check(LogitRules r) {
   for (long row = blockIdx.x; row < r.rows; row += gridDim.x) {
     bool bad = false;

@@ -365,7 +365,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 // it in LDS after the last: a load has most of a tile's time to arrive.  The queries
 // wait in registers.  Bound by double MFMAs and the softmax's double arithmetic,
 // which take turns on a SIMD: 4 sequences of 12 heads, 1964 to 2048 slots and 64
-// nodes at head dim 64 take 92 us, 47% of it MFMAs (the padded products alone
+// nodes at head dim 64 take 90 us, 48% of it MFMAs (the padded products alone
 // are 44 us).  Head dim 128, whose queries and outputs leave 11 VGPRs spilled
 // (26 padded) at one wave a SIMD, takes 222 us for twice the products.  Tiles of
 // a wave's own would be read four times through the caches.

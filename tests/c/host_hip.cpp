@@ -5,6 +5,7 @@
  *   host_hip_calls(name)      calls of a runtime function so far
  *   host_hip_launches(part)   launches of kernels whose name contains `part`
  *   host_hip_fail(name, k)    the k-th call of `name` from now fails (0: none)
+ *   host_hip_pinned(bytes)    the pinned allocation of that size
  */
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>
@@ -19,6 +20,7 @@ std::map<std::string, long> g_calls, g_fail;
 std::map<const void*, std::string> g_kernels;
 std::map<std::string, long> g_launches;
 std::map<char*, size_t> g_memory;  // device allocations
+std::map<void*, size_t> g_pinned;
 std::map<const void*, void*> g_symbols;
 hipError_t g_last = hipSuccess;
 
@@ -59,6 +61,11 @@ long host_hip_launches(const char* part) {
 void host_hip_fail(const char* name, long k) {
   g_fail.erase(name);
   if (k > 0) g_fail[name] = k;
+}
+void* host_hip_pinned(size_t n) {
+  for (auto& m : g_pinned)
+    if (m.second == n) return m.first;
+  return nullptr;
 }
 
 void** __hipRegisterFatBinary(const void*) { return (void**)&g_handle; }
@@ -114,9 +121,14 @@ hipError_t hipFree(void* p) {
 hipError_t hipHostMalloc(void** p, size_t n, unsigned) {
   if (fails("hipHostMalloc", hipErrorOutOfMemory)) return hipErrorOutOfMemory;
   *p = calloc(1, n);
+  g_pinned[*p] = n;
   return hipSuccess;
 }
-hipError_t hipHostFree(void* p) { return free(p), hipSuccess; }
+hipError_t hipHostFree(void* p) {
+  g_pinned.erase(p);
+  free(p);
+  return hipSuccess;
+}
 hipError_t hipMemcpy(void* d, const void* s, size_t n, hipMemcpyKind) {
   CALL("hipMemcpy");
   memmove(d, s, n);

@@ -17,6 +17,8 @@ hip = ctypes.CDLL({stub!r}, mode=ctypes.RTLD_GLOBAL)  # before the library looks
 hip.host_hip_calls.restype = hip.host_hip_launches.restype = ctypes.c_long
 calls, launches = (lambda f: lambda name: f(name.encode()))(hip.host_hip_calls), lambda part: hip.host_hip_launches(part.encode())
 fail = lambda name, k=1: hip.host_hip_fail(name.encode(), ctypes.c_long(k))
+hip.host_hip_pinned.restype = ctypes.c_void_p
+pinned = lambda words: (ctypes.c_uint32 * words).from_address(hip.host_hip_pinned(ctypes.c_size_t(4 * words)))
 import rustcrates_amd as ra
 
 def device(nbytes):  # memory that the library takes for the device's

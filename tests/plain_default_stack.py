@@ -1,8 +1,8 @@
 """create_transformer's default stack in plain numpy products, one sequence at a
 time: Embedding, DiscreteWavelet on the prompt, Norm, RoPE at the uncompressed
 positions, two attention layers of 2 and 4 heads with their FeedForwards,
-Linear.  The wavelet's rows come from the CPU checker's layer.
-test_plain_default_stack.py holds it to the checker."""
+Linear.  The wavelet's rows come from the oracle's layer.
+test_plain_default_stack.py holds it to the oracle."""
 from __future__ import annotations
 
 import copy

@@ -73,8 +73,7 @@ def test_a_refused_call_leaves_logits_in_place_as_they_were(net, R, V):
 
 
 def test_an_error_is_reported_once(net):
-    """A call that ends early, here on the runtime's own last error, takes what
-    its kernels found with it."""
+    """Also where the runtime holds an older error of the thread."""
     hip = C.CDLL("libamdhip64.so.7")
     x = np.zeros((2, 40))
     good, ids = net.process_logits(x, [[1]] * 2, [[2.0, 1.0, 0.0]] * 2)

@@ -135,3 +135,21 @@ while pos < 1300:
         pos += 1
 assert 1 <= grown <= 2, grown
 """)
+
+
+@pytest.mark.parametrize("call", ["net.process_logits(np.zeros((2, 50)))", "net.tree_step([[3, 4, 5]] * 2, [[-1, 0, 0]] * 2)"])
+def test_error_words_of_a_call_that_failed_otherwise(call):
+    """What the kernels of a failing call found is not the next call's."""
+    run(TREE + f"""
+words = pinned(4)
+for word in range(3):
+    words[word] = 1  # as a kernel sets it
+    fail("hipStreamSynchronize", 1)
+    refused(2, "", lambda: {call})
+    assert not any(words)
+    net.prefill(prompt)
+    {call}
+    words[word] = 1
+    refused(4 if word == 1 else 1, "", lambda: {call})
+    net.prefill(prompt)
+""")

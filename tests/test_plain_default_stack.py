@@ -1,4 +1,4 @@
-"""The plain default stack against the CPU checker: a compressed prompt and steps."""
+"""The plain default stack against the oracle: a compressed prompt and steps."""
 from __future__ import annotations
 
 import numpy as np
@@ -11,7 +11,7 @@ from rustcrates_amd import configs, seeded
 
 
 @pytest.mark.parametrize("S", [1, 21, 40])
-def test_plain_default_stack_is_the_checkers(S):
+def test_plain_default_stack_is_the_oracles(S):
     V, ctx = 120, 64
     o = configs.build_reference_default(oracle.Network(), V, 5, ctx, wavelet_embedding=False)
     prompt = seeded.prompts(3, [S], V)
