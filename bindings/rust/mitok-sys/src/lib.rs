@@ -37,6 +37,10 @@ pub const MITOK_NO_PARENT: u32 = 0xFFFF_FFFF;
 pub const MITOK_NO_TOKEN: u32 = 0xFFFF_FFFF;
 pub const MITOK_NO_ROW: u32 = 0xFFFF_FFFF;
 pub const MITOK_TREE_MAX_NODES: u32 = 256;
+/// no page of a paged cache
+pub const MITOK_NO_PAGE: u32 = 0xFFFF_FFFF;
+/// continuations kept of a group of beams at most
+pub const MITOK_BEAM_MAX_KEEP: u32 = 64;
 
 pub const MITOK_TIME_VOCAB: c_int = 1;
 pub const MITOK_TIME_LAYER_GEMM: c_int = 2;
@@ -158,6 +162,34 @@ extern "C" {
         net: *mut MitokNetwork, logits: *const c_double, rows: u32, vocab: u32, history: *const u32,
         max_history: u32, penalties: *const c_double, bias_ids: *const u32, bias: *const c_double, max_bias: u32,
         allowed: *const u32, out: *mut c_double, out_ids: *mut u32
+    ) -> c_int;
+
+    // beams on a paged cache (no counterpart in the reference)
+    pub fn mitok_paged_attention_device(
+        net: *mut MitokNetwork, d_q: *const c_double, d_k_new: *const c_double, d_v_new: *const c_double,
+        d_k_pages: *mut c_double, d_v_pages: *mut c_double, d_table: *const u32, d_bias: *const c_double,
+        bias_stride: u64, bias_row_stride: u64, kv_lens: *const u32, counts: *const u32, batch: u32, rows: u32,
+        heads: u32, head_dim: u32, page_rows: u32, max_pages: u32, pages: u32, d_out: *mut c_double
+    ) -> c_int;
+    pub fn mitok_fork_pages_device(
+        net: *mut MitokNetwork, d_k_pages: *mut c_double, d_v_pages: *mut c_double, layers: u32, pages: u32,
+        heads: u32, page_rows: u32, head_dim: u32, d_table: *const u32, d_lens: *const u32, sequences: u32,
+        max_pages: u32, d_parents: *const u32, d_grow: *const u32, new_sequences: u32, d_table_out: *mut u32,
+        d_lens_out: *mut u32
+    ) -> c_int;
+    pub fn mitok_beam_select_device(
+        net: *mut MitokNetwork, d_logits: *const c_double, d_scores: *const c_double, d_done: *const u32,
+        d_scale: *const c_double, batch: u32, beams: u32, vocab: u32, keep: u32, d_parents: *mut u32,
+        d_tokens: *mut u32, d_scores_out: *mut c_double
+    ) -> c_int;
+    pub fn mitok_beam_select(
+        net: *mut MitokNetwork, logits: *const c_double, scores: *const c_double, done: *const u32,
+        scale: *const c_double, batch: u32, beams: u32, vocab: u32, keep: u32, parents: *mut u32,
+        tokens: *mut u32, scores_out: *mut c_double
+    ) -> c_int;
+    pub fn mitok_beam_search(
+        net: *mut MitokNetwork, prompt: *const u32, lens: *const u32, batch: u32, seq: u32, beams: u32, n_new: u32,
+        end_id: u32, length_power: c_double, out_ids: *mut u32, out_lens: *mut u32, out_scores: *mut c_double
     ) -> c_int;
 
     // measurement and scheduling (no counterpart in the reference)

@@ -51,11 +51,15 @@ extern "C" {
 #define MITOK_NETWORK_RATE 0xFFFFFFFFu
 
 /* operators of a serving loop: a drafted token without a parent among the
- * drafted ones; no token (an unused entry, or no answer); no cached row */
+ * drafted ones (or a sequence without one); no token (an unused entry, or no
+ * answer); no cached row; no page of a paged cache; continuations kept of a group
+ * of beams at most */
 #define MITOK_NO_PARENT 0xFFFFFFFFu
 #define MITOK_NO_TOKEN 0xFFFFFFFFu
 #define MITOK_NO_ROW 0xFFFFFFFFu
+#define MITOK_NO_PAGE 0xFFFFFFFFu
 #define MITOK_TREE_MAX_NODES 256
+#define MITOK_BEAM_MAX_KEEP 64
 
 /* kernel classes for mitok_timing_enable */
 #define MITOK_TIME_VOCAB 1       /* the vocab Linear (the Linear before Softmax) */
@@ -418,6 +422,95 @@ int mitok_process_logits(mitok_network* net, const double* logits, uint32_t rows
                          const uint32_t* history, uint32_t max_history, const double* penalties,
                          const uint32_t* bias_ids, const double* bias, uint32_t max_bias, const uint32_t* allowed,
                          double* out, uint32_t* out_ids);
+
+/* ---- beams on a paged cache (no reference counterpart) ----
+ * Several hypotheses per prompt, which share the cached rows that they have in
+ * common.  A cache of pages holds a sequence's slot t in row t % page_rows of page
+ * table[sequence][t / page_rows]; a pool has [pages][heads][page_rows][head_dim]
+ * complex keys, and as many values.  page_rows: a multiple of 16 up to 1024;
+ * head_dim <= 256; pages <= 2^24; at most 65535 sequences, max_pages * page_rows <=
+ * 2^30.  Streams, checks and completion are those of the operators above. */
+
+/* Attention of a chunk of new tokens: sequence b holds kv_lens[b] rows, and its
+ * counts[b] <= rows new ones (counts NULL: rows of each; rows <= 65536) are stored
+ * behind them and attend, new row i over the slots up to its own:
+ *   score(i, t) = Re(sum_e q_i[e] k_t[e]) / (1e-8 + sqrt(head_dim)) + bias[h][t],  t <= kv_lens[b] + i
+ *   out_i = sum_t softmax(score(i, .))_t v_t
+ * With bias_row_stride > 0 a head's biases are a table of rows so far apart, of
+ * which new row i takes row kv_lens[b] + i: a prompt's pass, in one chunk or
+ * several (masked_attention_head.rs:184-208); 0 is a decode step's.  Slots that a
+ * row does not see have no part in its output, finite or not; rows past
+ * counts[b] are zero.
+ *   d_q, d_k_new, d_v_new, d_out [batch][rows][heads * head_dim] complex
+ *   d_table [batch][max_pages]: entries of the slots in use, the new rows' too;
+ *     entries behind them are not read
+ *   d_bias [heads] of bias_stride apart, or NULL
+ * An entry in use that is >= pages is MITOK_ERR_ARG, and so are two pages of a call
+ * that store new rows to one page of the pool.  A page that is stored to may be
+ * in no other sequence's use (mitok_fork_pages_device sees to that): the rows read
+ * of it would depend on the order.  On an error the outputs have no meaning. */
+int mitok_paged_attention_device(mitok_network* net, const double* d_q, const double* d_k_new, const double* d_v_new,
+                                 double* d_k_pages, double* d_v_pages, const uint32_t* d_table, const double* d_bias,
+                                 uint64_t bias_stride, uint64_t bias_row_stride, const uint32_t* kv_lens,
+                                 const uint32_t* counts, uint32_t batch, uint32_t rows, uint32_t heads,
+                                 uint32_t head_dim, uint32_t page_rows, uint32_t max_pages, uint32_t pages,
+                                 double* d_out);
+/* Sequences that take other sequences' rows.  New sequence i (of new_sequences)
+ * has the rows of d_parents[i] (MITOK_NO_PARENT: none) and room for d_grow[i] more
+ * (d_grow NULL or no parent: 0).  Rows are shared by sharing pages; a page that is
+ * part filled, last of a sequence that grows, and held by another new sequence
+ * too, is copied (its used rows, in every layer), except for the first of its
+ * holders where all of them grow from it.  Pages that no new sequence holds are
+ * free; copies and room take them in ascending order, sequence by sequence, a
+ * copy before the room.
+ *   d_k_pages, d_v_pages: `layers` pools one behind the other, of one table
+ *   d_table [sequences][max_pages], d_lens [sequences] rows
+ *   d_table_out [new_sequences][max_pages]: MITOK_NO_PAGE behind a sequence's last
+ *     page; d_lens_out [new_sequences]: its rows, without the room
+ * d_table_out may be d_table and d_lens_out d_lens.  MITOK_ERR_ARG: a parent or a
+ * page that is none, rows and room past max_pages; MITOK_ERR_NOMEM: fewer free pages
+ * than needed.  Either leaves every array as it was. */
+int mitok_fork_pages_device(mitok_network* net, double* d_k_pages, double* d_v_pages, uint32_t layers, uint32_t pages,
+                            uint32_t heads, uint32_t page_rows, uint32_t head_dim, const uint32_t* d_table,
+                            const uint32_t* d_lens, uint32_t sequences, uint32_t max_pages, const uint32_t* d_parents,
+                            const uint32_t* d_grow, uint32_t new_sequences, uint32_t* d_table_out,
+                            uint32_t* d_lens_out);
+/* The best continuations of each group of beams (batch groups of `beams` <= 1024
+ * rows): of all (row r, token t) the `keep` <= MITOK_BEAM_MAX_KEEP of largest rank,
+ *   score(r, t) = scores[r] + logits[r][t] - log sum_u exp(logits[r][u])
+ *   rank(r, t) = score(r, t) * scale[r]
+ * the best first; in a row the larger logit is first, of equal ones the lower
+ * token, between rows of equal rank the lower row.  A row with done[r] != 0 has
+ * one continuation, itself (score scores[r], no token); one of score -inf has
+ * none, and a logit of -inf is none.  The logits of both kinds of row are not read.
+ *   d_logits [batch * beams][vocab], d_scores, d_scale [batch * beams] (scale NULL: 1;
+ *     else finite and above 0), d_done [batch * beams] or NULL
+ *   d_parents [batch][keep]: the row, counted over all groups, d_tokens,
+ *     d_scores_out; where there are no more continuations MITOK_NO_ROW,
+ *     MITOK_NO_TOKEN and -inf (the row alone: an ended one's own)
+ * A score or a live row's logit that is NaN or +infinity is MITOK_ERR_NAN.  On an error
+ * the outputs have no meaning. */
+int mitok_beam_select_device(mitok_network* net, const double* d_logits, const double* d_scores, const uint32_t* d_done,
+                             const double* d_scale, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t keep,
+                             uint32_t* d_parents, uint32_t* d_tokens, double* d_scores_out);
+/* The same on host arrays. */
+int mitok_beam_select(mitok_network* net, const double* logits, const double* scores, const uint32_t* done,
+                      const double* scale, uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t keep,
+                      uint32_t* parents, uint32_t* tokens, double* scores_out);
+/* predict_token_by_token's loop with `beams` <= MITOK_BEAM_MAX_KEEP hypotheses per
+ * prompt (transformer_network.rs:165-313 keeps one): up to n_new tokens each, one
+ * that chooses end_id ends there (MITOK_NO_TOKEN: none does).  A hypothesis is ranked
+ * by its score, the sum of its tokens' log probabilities, over its number of
+ * tokens to the power length_power (0: by the score; within [-16, 16]).  The prompt
+ * runs once and its rows are shared; one beam without an end gives
+ * mitok_generate's ids.  Drops the caches, as mitok_generate does, and leaves none.
+ *   prompt [batch][seq], lens [batch] as for mitok_generate
+ *   out_ids [batch][beams][n_new], the best hypothesis first, MITOK_NO_TOKEN behind its
+ *     tokens; out_lens [batch][beams] tokens (the end among them);
+ *     out_scores [batch][beams], -inf where there are fewer hypotheses than beams */
+int mitok_beam_search(mitok_network* net, const uint32_t* prompt, const uint32_t* lens, uint32_t batch, uint32_t seq,
+                      uint32_t beams, uint32_t n_new, uint32_t end_id, double length_power, uint32_t* out_ids,
+                      uint32_t* out_lens, double* out_scores);
 
 /* ---- measurement (no reference counterpart: the reference prints wall
  * clock only, transformer_network.rs:307-310) ---- */

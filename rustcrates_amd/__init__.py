@@ -26,8 +26,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libmitok.so")
 
 TRAINING, PRODUCTION = 0, 1
-# a drafted token without a parent, no token, no cached row; nodes of a tree at most
-NO_PARENT = NO_TOKEN = NO_ROW = 0xFFFFFFFF
+# a drafted token or sequence without a parent, no token, no cached row, no page; nodes of a tree at most
+NO_PARENT = NO_TOKEN = NO_ROW = NO_PAGE = 0xFFFFFFFF
+BEAM_MAX_KEEP = 64  # continuations kept of a group of beams at most
 TREE_MAX_NODES = 256
 TIME_VOCAB, TIME_LAYER_GEMM, TIME_ATTENTION, TIME_STEP, TIME_PREFILL_GEMM = 1, 2, 3, 4, 5
 
@@ -84,6 +85,13 @@ SIGNATURES = {
     "mitok_evict_rows": (_i32, [_P, _u32, _u32, _u32, _u32, _P]),
     "mitok_process_logits_device": (_i32, [_P, _P, _u32, _u32, _P, _u32, _P, _P, _P, _u32, _P, _P, _P]),
     "mitok_process_logits": (_i32, [_P, _P, _u32, _u32, _P, _u32, _P, _P, _P, _u32, _P, _P, _P]),
+    "mitok_paged_attention_device": (_i32, [_P, _P, _P, _P, _P, _P, _P, _P, _u64, _u64, _P, _P, _u32, _u32, _u32, _u32,
+                                            _u32, _u32, _u32, _P]),
+    "mitok_fork_pages_device": (_i32, [_P, _P, _P, _u32, _u32, _u32, _u32, _u32, _P, _P, _u32, _u32, _P, _P, _u32, _P,
+                                       _P]),
+    "mitok_beam_select_device": (_i32, [_P, _P, _P, _P, _P, _u32, _u32, _u32, _u32, _P, _P, _P]),
+    "mitok_beam_select": (_i32, [_P, _P, _P, _P, _P, _u32, _u32, _u32, _u32, _P, _P, _P]),
+    "mitok_beam_search": (_i32, [_P, _P, _P, _u32, _u32, _u32, _u32, _u32, _f64, _P, _P, _P]),
     "mitok_last_timings": (_i32, [_P, _P]),
     "mitok_timing_enable": (_i32, [_P, _i32]),
     "mitok_timing_read": (_i32, [_P, _P, _P, _P, _P]),
@@ -719,6 +727,94 @@ class Network:
                                               _at(bi), _at(bv), 0 if bi is None else bi.shape[1], _at(al),
                                               _at(out), _at(ids)))
         return out, ids
+
+    # ---- beams on a paged cache ----
+    def paged_attention_device(self, d_q, d_k_new, d_v_new, d_k_pages, d_v_pages, d_table, kv_lens, rows, heads, head_dim,
+                               page_rows, pages, max_pages, d_out, counts=None, bias=None, bias_stride=0,
+                               bias_row_stride=0):
+        """Attention of a chunk of new tokens over a paged cache in device memory
+        (mitok_paged_attention_device has the layouts).  Sequence b's counts[b]
+        (None: `rows`) new rows are stored behind its kv_lens[b] and attend over
+        those and causally over one another.  bias: [heads] rows of f64,
+        bias_stride apart, or with bias_row_stride tables of which each new row
+        takes the one of its position."""
+        lens = _u32_lens(kv_lens, None, "kv_lens")
+        B = len(lens)
+        cnt = None if counts is None else _u32_lens(counts, B, "counts")
+        _check_sizes(rows | heads | head_dim | page_rows | pages | max_pages | (bias_stride >> 32) | (bias_row_stride >> 32))
+        _check(self._lib.mitok_paged_attention_device(self._h, _dev(d_q), _dev(d_k_new), _dev(d_v_new), _dev(d_k_pages),
+                                                      _dev(d_v_pages), _dev(d_table), _dev(bias), int(bias_stride),
+                                                      int(bias_row_stride), _at(lens), _at(cnt), B, rows, heads, head_dim,
+                                                      page_rows, max_pages, pages, _dev(d_out)))
+
+    def fork_pages_device(self, d_k_pages, d_v_pages, layers, pages, heads, page_rows, head_dim, d_table, d_lens, sequences,
+                          max_pages, d_parents, new_sequences, d_table_out, d_lens_out, grow=None):
+        """New sequence i takes the rows of sequence d_parents[i] (NO_PARENT:
+        none), its pages shared, and room for grow[i] more; part-filled pages that
+        are shared are copied in every layer (mitok_fork_pages_device).  The
+        tables [sequences][max_pages], lens, parents and grow are u32 in device
+        memory; the new ones may replace the old."""
+        _check_sizes(layers | pages | heads | page_rows | head_dim | sequences | max_pages | new_sequences)
+        _check(self._lib.mitok_fork_pages_device(self._h, _dev(d_k_pages), _dev(d_v_pages), layers, pages, heads, page_rows,
+                                                 head_dim, _dev(d_table), _dev(d_lens), sequences, max_pages,
+                                                 _dev(d_parents), _dev(grow), new_sequences, _dev(d_table_out),
+                                                 _dev(d_lens_out)))
+
+    def beam_select_device(self, d_logits, d_scores, batch, beams, vocab, keep, d_parents, d_tokens, d_scores_out, done=None,
+                           scale=None):
+        """The `keep` best continuations of each group of `beams` rows of logits
+        [batch * beams][vocab] f64 by (score + log softmax) * scale
+        (mitok_beam_select_device).  scores, scale [batch * beams] f64 and done u32;
+        parents, tokens [batch][keep] u32 and scores_out f64."""
+        _check_sizes(batch | beams | vocab | keep)
+        _check(self._lib.mitok_beam_select_device(self._h, _dev(d_logits), _dev(d_scores), _dev(done), _dev(scale), batch,
+                                                  beams, vocab, keep, _dev(d_parents), _dev(d_tokens), _dev(d_scores_out)))
+
+    def beam_select(self, logits, scores, keep, done=None, scale=None):
+        """beam_select_device on host arrays: logits [batch][beams][V], scores,
+        done and scale [batch][beams].  Returns (parents, tokens, scores), each
+        [batch][keep]."""
+        x = np.ascontiguousarray(logits, dtype=np.float64)
+        if x.ndim != 3:
+            raise ValueError(f"logits: shape {x.shape}, expected (batch, beams, vocab)")
+        B, R, V = x.shape
+
+        def of_rows(a, dtype, what):
+            if a is None:
+                return None
+            a = np.ascontiguousarray(a, dtype=dtype)
+            if a.shape != (B, R):
+                raise ValueError(f"{what}: shape {a.shape}, expected ({B}, {R})")
+            return a
+
+        if scores is None:
+            raise ValueError("scores: missing")
+        s, c = of_rows(scores, np.float64, "scores"), of_rows(scale, np.float64, "scale")
+        d = None if done is None else of_rows(np.asarray(done, dtype=bool), np.uint32, "done")
+        _check_sizes(keep)
+        keep = int(keep)
+        parents, tokens, best = np.empty((B, keep), np.uint32), np.empty((B, keep), np.uint32), np.empty((B, keep), np.float64)
+        _check(self._lib.mitok_beam_select(self._h, _at(x), _at(s), _at(d), _at(c), B, R, V, keep, _at(parents), _at(tokens),
+                                           _at(best)))
+        return parents, tokens, best
+
+    def beam_search(self, prompt, lens=None, beams=4, n_new=1, end_id=None, length_power=0.0):
+        """Token loop with `beams` hypotheses per prompt (mitok_beam_search):
+        (ids [B][beams][n_new], tokens [B][beams], scores [B][beams]), the best
+        first; ids behind a hypothesis' tokens are NO_TOKEN.  end_id: the token
+        that ends one (None: none does)."""
+        prompt = np.ascontiguousarray(prompt, dtype=np.uint32)
+        if prompt.ndim != 2:
+            raise ValueError(f"prompt: shape {prompt.shape}, expected (batch, seq)")
+        B, S = prompt.shape
+        lens = np.full(B, S, np.uint32) if lens is None else _u32_vec(lens, B, "lens")
+        _check_sizes(beams | n_new)
+        ids = np.empty((B, int(beams), int(n_new)), np.uint32)
+        count, scores = np.empty(ids.shape[:2], np.uint32), np.empty(ids.shape[:2], np.float64)
+        _check(self._lib.mitok_beam_search(self._h, _ptr(prompt), _ptr(lens), B, S, int(beams), int(n_new),
+                                           NO_TOKEN if end_id is None else int(end_id), float(length_power), _ptr(ids),
+                                           _ptr(count), _ptr(scores)))
+        return ids, count, scores
 
     # ---- measurement ----
     def last_timings(self):

@@ -19,7 +19,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmitok.so")
 SOURCES = ["kernels.hip", "gemm.hip", "gemm_mfma.hip", "attention.hip", "resident.hip", "resident_k1.hip", "resident_k2.hip",
            "resident_k4.hip", "resident_k8.hip", "train.hip", "wavelet_init.hip", "tree_attention.hip",
-           "serving.hip", "network.hip"]
+           "serving.hip", "paged_attention.hip", "beams.hip", "network.hip"]
 ARCH = os.environ.get("MITOK_ARCH", "gfx950")
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
@@ -53,6 +53,7 @@ FILE_FLAGS = {"gemm_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
               # 33 nodes and more still spill 26 at head dims 65 to 127 (11 at 128), and head dims
               # above 128 278 (272 at 256)
               "tree_attention.hip": ["-mllvm", "-disable-machine-licm"],
+              "paged_attention.hip": ["-mllvm", "-disable-machine-licm"],
               # the wavelet embedding follows the reference's multiply and add order
               "wavelet_init.hip": ["-ffp-contract=off"]}
 

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <exception>
 #include <initializer_list>
 #include <memory>
 #include <mutex>
@@ -22,6 +23,7 @@
 #include <vector>
 
 #include "../../include/mitok.h"
+#include "paged.hpp"
 #include "serving.hpp"
 #include "train.hpp"
 
@@ -140,6 +142,7 @@ struct SelfAttentionLayer : Layer {  // self_attention_layer.rs:16-25 + masked_a
   DevBuf bias_re;  // [heads][max_ctx][max_ctx]  Re(bias_pos): only the real part reaches the softmax
   DevBuf gamma, beta;
   DevBuf kc, vc;  // [cache_B][heads][max_ctx][dh]
+  DevBuf kp, vp;  // [pages][heads][page rows][dh] of a beam search
   DevBuf aw;      // [cache_B][heads][max_ctx] attention each cached row received (mitok_tree_step)
   // training state: AdamW moments of wqkv and of the Norm's gamma and beta;
   // updates so far of the heads and of the Norm, counted apart because
@@ -288,6 +291,14 @@ struct TreePass {
   OpTable own;
 };
 
+// a pass on the pages of a beam search: its lengths and tables, and for each
+// attention layer in order how its work is cut up
+struct PagedPass {
+  PagedAttn a;
+  std::vector<PagedPlan> plans;
+  bool by_row = false;  // a prompt: bias rows go by position
+};
+
 struct Spec {
   int B = 0, S = 0;
   int mode = MODE_STATELESS;
@@ -312,6 +323,7 @@ struct Spec {
                                      // follow; S is the most they reach) and its target rows
   int ctx_bound = 0;                 // keys a decode step of this call can reach (0: the layers' context)
   const TreePass* tree = nullptr;    // a drafted tree's rows on the cache
+  const PagedPass* paged = nullptr;  // rows on the pages of a beam search
 };
 
 struct Timing {
@@ -417,8 +429,14 @@ struct mitok_network {
   size_t op_host_bytes = 0;
   mitok::DevBuf op_tab, op_ws;
   uint32_t* op_err = nullptr;
+  uint32_t* page_err = nullptr;  // and those of paged.hpp
   mitok::DevBuf op_refused;  // the number of the last call whose logits in place stayed (LogitRules)
   uint32_t op_calls = 0;
+  // forks of paged sequences: the pages' counts, zero between calls unless one
+  // failed, and the last call and sequence that stored to a page (PagedAttn)
+  mitok::DevBuf fork_held, page_stamp;
+  bool fork_dirty = false;
+  mitok::DevBuf beam_state;  // of a beam search: tables, lengths, scores, history
   hipEvent_t op_event = nullptr;
   // the last stateless pass's vocab Linear input rows [head_B * head_S][d]
   // (in act0/act1) and its softmax output (probs), which mitok_backward_head
@@ -752,7 +770,7 @@ static int prepare(Net* n, const Spec& sp) {
   if (dm.hmax) {
     if (sp.mode == MODE_CACHED && sp.S == 1)
       TRY(reserve(n, n->datt, attention_split_ws_bytes(sp.B, dm.hmax, dm.dh_max, dm.mc_max)));
-    if (sp.mode == MODE_STATELESS && !keeps(sp)) TRY(reserve(n, n->kv_scratch, 2 * rows * dm.dsa * c16));
+    if ((sp.mode == MODE_STATELESS && !keeps(sp)) || sp.paged) TRY(reserve(n, n->kv_scratch, 2 * rows * dm.dsa * c16));
   }
   TRY(reserve(n, n->sync_ws, ws));
   if (sp.mode == MODE_CACHED && sp.S == 1 && sp.B <= GEMM_PART_MAX_M) {
@@ -838,7 +856,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
   const uint32_t* lens = sp.lens;
   const int* pos = sp.pos;
   size_t wi = 0;  // next wavelet stage
-  size_t ti = 0;  // next plan of a tree's pass
+  size_t ti = 0;  // next plan of a tree's or a paged pass
   bool real = false;  // the rows in cur have zero imaginary parts: a Norm leaves Re(x) + 0i (norm_layer.rs:64-130)
   // a pass that backward may differentiate leaves every layer's input in that
   // layer's own buffer; another alternates between two
@@ -911,7 +929,7 @@ static int enqueue_forward(Net* n, const Spec& sp) {
         Attn a;
         a.q = q;
         a.ldq = d;
-        if (sp.mode == MODE_STATELESS) {
+        if (sp.mode == MODE_STATELESS || sp.paged) {
           e.kc = save ? n->sv_b[li]->as<double2>() : n->kv_scratch.as<double2>();
           e.vc = e.kc + (size_t)rows * d;
           e.ctx = S;
@@ -968,6 +986,29 @@ static int enqueue_forward(Net* n, const Spec& sp) {
           {
             TimeScope ts(n, MITOK_TIME_ATTENTION, 0.0);
             tree_attention(st, t, sp.tree->plans[ti++], sp.tree->own);
+          }
+          layernorm(st, cat, cur, nxt, rows, d, A->eps, A->gamma.as<double2>(), A->beta.as<double2>());
+        } else if (sp.paged) {
+          PagedAttn t = sp.paged->a;
+          t.q = q;
+          t.ldq = t.ldo = d;
+          t.kn = e.kc;
+          t.vn = e.vc;
+          t.new_b = (long)S * d;
+          t.new_row = dh;
+          t.new_head = (long)S * dh;
+          t.kp = A->kp.as<double2>();
+          t.vp = A->vp.as<double2>();
+          t.bias = a.bias_re;
+          t.bias_stride = (long)A->max_ctx * A->max_ctx;
+          t.bias_row = sp.paged->by_row ? A->max_ctx : 0;
+          t.H = H;
+          t.dh = dh;
+          t.scale = a.scale;
+          t.out = cat;
+          {
+            TimeScope ts(n, MITOK_TIME_ATTENTION, 0.0);
+            paged_attention(st, t, sp.paged->plans[ti++], OpTable());
           }
           layernorm(st, cat, cur, nxt, rows, d, A->eps, A->gamma.as<double2>(), A->beta.as<double2>());
         } else if (sp.mode == MODE_CACHED && S == 1) {
@@ -1900,6 +1941,16 @@ static int rope_positions_needed(const Net* n) {
   return (int)std::max<uint32_t>(m == UINT32_MAX ? 512u : m, 512u);
 }
 
+// what a call's own arrays on the host may throw, as an error
+template <class F>
+static int guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::exception&) {
+    return fail(ERR_NOMEM, "out of host memory");
+  }
+}
+
 // ---------------------------------------------------------------------------
 // staging of mitok_greedy_decoding_noalloc, for callers that cannot allocate
 // ---------------------------------------------------------------------------
@@ -1975,6 +2026,9 @@ int mitok_network_create(int device, mitok_network** out) {
   if (!rc && hipHostMalloc((void**)&n->op_err, OE_WORDS * sizeof(uint32_t), hipHostMallocCoherent) != hipSuccess)
     rc = fail(ERR_NOMEM, "hipHostMalloc of the error words failed");
   if (!rc) memset(n->op_err, 0, OE_WORDS * sizeof(uint32_t));
+  if (!rc && hipHostMalloc((void**)&n->page_err, PE_WORDS * sizeof(uint32_t), hipHostMallocCoherent) != hipSuccess)
+    rc = fail(ERR_NOMEM, "hipHostMalloc of the error words failed");
+  if (!rc) memset(n->page_err, 0, PE_WORDS * sizeof(uint32_t));
   if (!rc && hipEventCreateWithFlags(&n->op_event, hipEventDisableTiming) != hipSuccess)
     rc = fail(ERR_HIP, "hipEventCreate failed");
   if (!rc) rc = n->err_d.reserve(2 * sizeof(uint32_t));
@@ -2004,6 +2058,7 @@ void mitok_network_destroy(mitok_network* n) {
   n->layers.clear();
   if (n->op_event) (void)hipEventDestroy(n->op_event);
   if (n->op_err) (void)hipHostFree(n->op_err);
+  if (n->page_err) (void)hipHostFree(n->page_err);
   if (n->op_host) (void)hipHostFree(n->op_host);
   if (n->stream) (void)hipStreamDestroy(n->stream);
   delete n;
@@ -2365,7 +2420,7 @@ static int begin_call(Net* n, const uint32_t* lens, uint32_t B, uint32_t S, cons
   sz.S_first = wl.empty() ? 0 : (int)S;
   sz.T = T;
   TRY(prepare(n, sz));
-  if (sp.mode == MODE_PREFILL) TRY(alloc_caches(n, B));
+  if (sp.mode == MODE_PREFILL && !sp.paged) TRY(alloc_caches(n, B));
   const size_t rows = (size_t)B * S;
   mask_h.assign(rows, 0);
   std::vector<int> pos(rows);
@@ -3742,23 +3797,34 @@ static int op_hand_over(Net* n, size_t bytes, OpTable& own, const char** tab) {
 }
 
 // The operators' error words, cleared; the stream is idle.
-static void take_words(Net* n, uint32_t (&w)[OE_WORDS]) {
-  for (int i = 0; i < OE_WORDS; ++i) {
-    w[i] = __atomic_load_n(&n->op_err[i], __ATOMIC_ACQUIRE);
-    if (w[i]) __atomic_store_n(&n->op_err[i], 0u, __ATOMIC_RELEASE);
-  }
+static void take_words(Net* n, uint32_t (&w)[OE_WORDS], uint32_t (&p)[PE_WORDS]) {
+  const auto take = [](uint32_t* from, uint32_t* to, int words) {
+    for (int i = 0; i < words; ++i) {
+      to[i] = __atomic_load_n(&from[i], __ATOMIC_ACQUIRE);
+      if (to[i]) __atomic_store_n(&from[i], 0u, __ATOMIC_RELEASE);
+    }
+  };
+  take(n->op_err, w, OE_WORDS);
+  take(n->page_err, p, PE_WORDS);
 }
 
 // Waits for the network's stream and turns the operators' error words into a
 // code.  Whatever comes first, the stream is idle and the words are clear.
 static int op_finish(Net* n) {
   const hipError_t launch = hipGetLastError(), wait = hipStreamSynchronize(n->stream);
-  uint32_t w[OE_WORDS];
-  take_words(n, w);
+  uint32_t w[OE_WORDS], p[PE_WORDS];
+  take_words(n, w, p);
   HIP_TRY(launch);
   HIP_TRY(wait);
   if (w[OE_BAD_TOKEN]) return fail(ERR_ARG, "a token id of the history or the biases is outside the vocabulary");
   if (w[OE_BAD_PENALTY]) return fail(ERR_ARG, "penalties must be finite and the repetition penalty above 0");
+  if (p[PE_BAD_PARENT]) return fail(ERR_ARG, "fork: a parent is not one of the sequences");
+  if (p[PE_BAD_LENGTH]) return fail(ERR_ARG, "fork: a sequence and its room exceed max_pages");
+  if (p[PE_BAD_PAGE]) return fail(ERR_ARG, "a page of the table is outside the pool");
+  if (p[PE_NO_PAGES]) return fail(ERR_NOMEM, "fork: fewer free pages than the sequences need");
+  if (p[PE_SHARED_PAGE]) return fail(ERR_ARG, "two sequences of a call, or two pages of one, store new rows to one page: fork them first");
+  if (p[PE_BAD_SCALE]) return fail(ERR_ARG, "beam selection: scales must be finite and above 0");
+  if (p[PE_BAD_SCORE]) return fail(ERR_NAN, "beam selection: a logit or score is NaN or +infinity");
   if (w[OE_NAN]) return fail(ERR_NAN, "greedy_decoding: NaN in logits (sampling_methods.rs:12)");
   return OK;
 }
@@ -3766,9 +3832,9 @@ static int op_finish(Net* n) {
 // A call that failed once it had queued work on the caches: waits for what is
 // queued, and the caches, part-way moved, no longer count.
 static int drop_moved(Net* n, int rc) {
-  uint32_t w[OE_WORDS];
+  uint32_t w[OE_WORDS], p[PE_WORDS];
   (void)hipStreamSynchronize(n->stream);
-  take_words(n, w);
+  take_words(n, w, p);
   drop_caches(n);
   return rc;
 }
@@ -4431,6 +4497,563 @@ int mitok_process_logits(mitok_network* n, const double* logits, uint32_t rows, 
   if (out_ids) HIP_TRY(hipMemcpyAsync(out_ids, id.p, rows * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
   HIP_TRY(hipStreamSynchronize(n->stream));
   return OK;
+}
+
+// ---- beams on a paged cache ----
+constexpr uint32_t PAGED_MAX_CHUNK = 1u << 16;  // new rows of a sequence
+constexpr uint32_t POOL_MAX_PAGES = 1u << 24, POOL_MAX_SEQS = 65535, POOL_MAX_TABLE = 1u << 28;
+constexpr uint32_t BEAM_MAX = 1024;             // rows of a group
+
+// shape of a pool of pages and of its tables
+static int check_pool(const char* what, uint32_t pages, uint32_t heads, uint32_t page_rows, uint32_t dh, uint32_t seqs,
+                      uint32_t max_pages) {
+  if (!pages || !heads || !dh || !seqs || !max_pages) return fail(ERR_ARG, "%s: bad shape", what);
+  if (!page_rows || page_rows % PAGE_TILE || page_rows > (uint32_t)PAGE_MAX_ROWS)
+    return fail(ERR_ARG, "%s: %u rows of a page: a multiple of %d up to %d", what, page_rows, PAGE_TILE, PAGE_MAX_ROWS);
+  if (dh > (uint32_t)TREE_MAX_DH) return fail(ERR_ARG, "%s: head dim %u > %d unsupported", what, dh, TREE_MAX_DH);
+  if (heads > 65535 || (uint64_t)heads * page_rows * dh > 1u << 30) return fail(ERR_ARG, "%s: a page of more than 2^30 elements", what);
+  if (pages > POOL_MAX_PAGES) return fail(ERR_ARG, "%s: %u pages, at most %u", what, pages, POOL_MAX_PAGES);
+  if (seqs > POOL_MAX_SEQS || (uint64_t)seqs * max_pages > POOL_MAX_TABLE || (uint64_t)max_pages * page_rows > OP_MAX_CTX)
+    return fail(ERR_ARG, "%s: at most %u sequences, 2^28 table entries and 2^30 rows of a sequence", what, POOL_MAX_SEQS);
+  return OK;
+}
+
+// a number of the call that the kernels' words remember it by
+static uint32_t next_call(Net* n) {
+  if (++n->op_calls == 0) n->op_calls = 1;  // the words start at 0
+  return n->op_calls;
+}
+
+static int paged_attention_impl(mitok_network* n, const double* d_q, const double* d_k_new, const double* d_v_new,
+                                double* d_k_pages, double* d_v_pages, const uint32_t* d_table, const double* d_bias,
+                                uint64_t bias_stride, uint64_t bias_row_stride, const uint32_t* kv_lens,
+                                const uint32_t* counts, uint32_t B, uint32_t rows, uint32_t heads, uint32_t dh,
+                                uint32_t page_rows, uint32_t max_pages, uint32_t pages, double* d_out) {
+  const char* what = "paged attention";
+  if (!n || !d_q || !d_k_new || !d_v_new || !d_k_pages || !d_v_pages || !d_table || !kv_lens || !d_out)
+    return fail(ERR_ARG, "%s: null argument", what);
+  TRY(check_pool(what, pages, heads, page_rows, dh, B, max_pages));
+  TRY(check_heads(what, B, heads));
+  if (!rows || rows > PAGED_MAX_CHUNK) return fail(ERR_ARG, "%s: %u new rows, 1 to %u", what, rows, PAGED_MAX_CHUNK);
+  if ((uint64_t)B * ((rows + 15) / 16) > 1u << 20) return fail(ERR_ARG, "%s: more than 2^20 groups of 16 new rows", what);
+  const uint64_t room = (uint64_t)max_pages * page_rows;
+  uint32_t longest = 0;
+  std::vector<int> kv(B), cnt(B);
+  for (uint32_t b = 0; b < B; ++b) {
+    const uint32_t c = counts ? counts[b] : rows;
+    if (c > rows) return fail(ERR_ARG, "%s: counts[%u]=%u above %u rows", what, b, c, rows);
+    if ((uint64_t)kv_lens[b] + c > room)
+      return fail(ERR_ARG, "%s: kv_lens[%u]=%u and its new rows exceed %u pages of %u", what, b, kv_lens[b], max_pages, page_rows);
+    longest = std::max(longest, kv_lens[b] + c);
+    kv[b] = (int)kv_lens[b];
+    cnt[b] = (int)c;
+  }
+  if (bias_stride > (uint64_t)INT64_MAX / 16 || bias_row_stride > (uint64_t)INT64_MAX / 16)
+    return fail(ERR_ARG, "%s: a bias stride out of range", what);
+  const size_t last_row = times({longest ? longest - 1 : 0, (size_t)bias_row_stride});
+  const size_t table_b = last_row > SIZE_MAX / 4 ? SIZE_MAX : last_row + longest;  // numbers of one head's
+  if (d_bias && heads > 1 && bias_stride < table_b)
+    return fail(ERR_ARG, "%s: bias_stride %llu below the %zu numbers used of a head", what, (unsigned long long)bias_stride, table_b);
+  TRY(set_device(n));
+  const size_t qb = times({B, rows, heads, dh, sizeof(double2)}), pb = times({pages, heads, page_rows, dh, sizeof(double2)});
+  const size_t tb = times({B, max_pages, sizeof(uint32_t)});
+  const size_t strides = times({heads - 1, (size_t)bias_stride});
+  const size_t bb = strides > SIZE_MAX / 32 || table_b > SIZE_MAX / 32 ? SIZE_MAX : (strides + table_b) * sizeof(double);
+  TRY(check_device_array(n, d_q, qb, 16, "q"));
+  TRY(check_device_array(n, d_k_new, qb, 16, "k_new"));
+  TRY(check_device_array(n, d_v_new, qb, 16, "v_new"));
+  TRY(check_device_array(n, d_k_pages, pb, 16, "k_pages"));
+  TRY(check_device_array(n, d_v_pages, pb, 16, "v_pages"));
+  TRY(check_device_array(n, d_table, tb, 4, "table"));
+  TRY(check_device_array(n, d_out, qb, 16, "out"));
+  if (d_bias) TRY(check_device_array(n, d_bias, bb, 8, "bias"));
+  const Span q = {d_q, qb, "q"}, kn = {d_k_new, qb, "k_new"}, vn = {d_v_new, qb, "v_new"}, k = {d_k_pages, pb, "k_pages"},
+             v = {d_v_pages, pb, "v_pages"}, t = {d_table, tb, "table"}, bi = {d_bias, bb, "bias"}, o = {d_out, qb, "out"};
+  TRY(check_apart(o, {q, kn, vn, k, v, t, bi}));
+  TRY(check_apart(k, {q, kn, vn, v, t, bi}));
+  TRY(check_apart(v, {q, kn, vn, t, bi}));
+  PagedAttn a;
+  a.q = (const double2*)d_q;
+  a.ldq = a.ldo = a.new_row = (long)heads * dh;
+  a.kn = (const double2*)d_k_new;
+  a.vn = (const double2*)d_v_new;
+  a.new_b = (long)rows * a.new_row;
+  a.new_head = dh;
+  a.kp = (double2*)d_k_pages;
+  a.vp = (double2*)d_v_pages;
+  a.table = d_table;
+  a.max_pages = (int)max_pages;
+  a.page_rows = (int)page_rows;
+  a.pages = pages;
+  a.bias = d_bias;
+  a.bias_stride = (long)bias_stride;
+  a.bias_row = (long)bias_row_stride;
+  a.B = (int)B;
+  a.n = (int)rows;
+  a.H = (int)heads;
+  a.dh = (int)dh;
+  a.scale = 1.0 / (1e-8 + sqrt((double)dh));  // as the layers' (masked_attention_head.rs:453-465)
+  a.out = (double2*)d_out;
+  a.err = n->page_err;
+  std::vector<int> lists;
+  PagedPlan plan = paged_plan(a, kv.data(), cnt.data(), lists);
+  if ((uint64_t)plan.entries * heads > 1u << 23) return fail(ERR_ARG, "%s: more than 2^23 blocks of work", what);
+  TRY(behind_default_stream(n));
+  TRY(alloc(n, n->op_ws, paged_ws_bytes(a, plan)));
+  a.ws = n->op_ws.p;
+  const size_t stamps = (size_t)pages * sizeof(unsigned long long);
+  if (n->page_stamp.bytes < stamps) {
+    TRY(alloc(n, n->page_stamp, stamps));
+    fill_u32(n->stream, n->page_stamp.as<uint32_t>(), n->page_stamp.bytes / 4, 0);
+  }
+  a.stamp = n->page_stamp.as<unsigned long long>();
+  a.call = next_call(n);
+  const size_t lists_at = (2 * (size_t)B * sizeof(int) + 15) & ~(size_t)15, bytes = lists_at + lists.size() * sizeof(int);
+  TRY(op_staging(n, bytes));
+  memcpy(n->op_host, kv.data(), B * sizeof(int));
+  memcpy(n->op_host + B * sizeof(int), cnt.data(), B * sizeof(int));
+  memcpy(n->op_host + lists_at, lists.data(), lists.size() * sizeof(int));
+  OpTable own;
+  TRY(op_hand_over(n, bytes, own, &a.tab));
+  a.kv_len = 0;
+  a.count = (uint32_t)(B * sizeof(int));
+  plan.chunks += (uint32_t)lists_at;
+  plan.splits += (uint32_t)lists_at;
+  paged_attention(n->stream, a, plan, own);
+  return op_finish(n);
+}
+
+int mitok_paged_attention_device(mitok_network* n, const double* d_q, const double* d_k_new, const double* d_v_new,
+                                 double* d_k_pages, double* d_v_pages, const uint32_t* d_table, const double* d_bias,
+                                 uint64_t bias_stride, uint64_t bias_row_stride, const uint32_t* kv_lens,
+                                 const uint32_t* counts, uint32_t B, uint32_t rows, uint32_t heads, uint32_t dh,
+                                 uint32_t page_rows, uint32_t max_pages, uint32_t pages, double* d_out) {
+  return guarded([&] {
+    return paged_attention_impl(n, d_q, d_k_new, d_v_new, d_k_pages, d_v_pages, d_table, d_bias, bias_stride, bias_row_stride,
+                                kv_lens, counts, B, rows, heads, dh, page_rows, max_pages, pages, d_out);
+  });
+}
+
+// Room and zero counts for a fork of `news` sequences (f's sizes are set).
+static int stage_fork(Net* n, ForkPages& f) {
+  const size_t held = fork_held_words(f.pages) * sizeof(uint32_t);
+  if (n->fork_held.bytes < held) {
+    TRY(alloc(n, n->fork_held, held));
+    n->fork_dirty = true;
+  }
+  if (n->fork_dirty) fill_u32(n->stream, n->fork_held.as<uint32_t>(), n->fork_held.bytes / 4, 0);
+  n->fork_dirty = true;  // until the call has ended well
+  f.held = n->fork_held.as<uint32_t>();
+  f.refused = n->op_refused.as<uint32_t>();
+  f.call = next_call(n);
+  f.err = n->page_err;
+  return OK;
+}
+
+int mitok_fork_pages_device(mitok_network* n, double* d_k_pages, double* d_v_pages, uint32_t layers, uint32_t pages,
+                            uint32_t heads, uint32_t page_rows, uint32_t dh, const uint32_t* d_table, const uint32_t* d_lens,
+                            uint32_t sequences, uint32_t max_pages, const uint32_t* d_parents, const uint32_t* d_grow,
+                            uint32_t new_sequences, uint32_t* d_table_out, uint32_t* d_lens_out) {
+  const char* what = "fork";
+  if (!n || !d_k_pages || !d_v_pages || !d_table || !d_lens || !d_parents || !d_table_out || !d_lens_out)
+    return fail(ERR_ARG, "%s: null argument", what);
+  TRY(check_pool(what, pages, heads, page_rows, dh, sequences, max_pages));
+  TRY(check_pool(what, pages, heads, page_rows, dh, new_sequences, max_pages));
+  if (!layers || layers > 16384) return fail(ERR_ARG, "%s: %u layers", what, layers);
+  TRY(set_device(n));
+  const size_t pb = times({layers, pages, heads, page_rows, dh, sizeof(double2)});
+  const size_t tb = times({sequences, max_pages, sizeof(uint32_t)}), to = times({new_sequences, max_pages, sizeof(uint32_t)});
+  const size_t lb = times({sequences, sizeof(uint32_t)}), lo = times({new_sequences, sizeof(uint32_t)});
+  TRY(check_device_array(n, d_k_pages, pb, 16, "k_pages"));
+  TRY(check_device_array(n, d_v_pages, pb, 16, "v_pages"));
+  TRY(check_device_array(n, d_table, tb, 4, "table"));
+  TRY(check_device_array(n, d_lens, lb, 4, "lens"));
+  TRY(check_device_array(n, d_parents, lo, 4, "parents"));
+  if (d_grow) TRY(check_device_array(n, d_grow, lo, 4, "grow"));
+  TRY(check_device_array(n, d_table_out, to, 4, "table_out"));
+  TRY(check_device_array(n, d_lens_out, lo, 4, "lens_out"));
+  const Span k = {d_k_pages, pb, "k_pages"}, v = {d_v_pages, pb, "v_pages"}, t = {d_table, tb, "table"}, l = {d_lens, lb, "lens"},
+             p = {d_parents, lo, "parents"}, g = {d_grow, lo, "grow"}, t2 = {d_table_out, to, "table_out"}, l2 = {d_lens_out, lo, "lens_out"};
+  TRY(check_apart(k, {v, t, l, p, g, t2, l2}));
+  TRY(check_apart(v, {t, l, p, g, t2, l2}));
+  TRY(check_apart(t2, {l, p, g, l2}));
+  TRY(check_apart(l2, {t, p, g}));
+  if (d_table_out != d_table) TRY(check_apart(t2, {t}));
+  if (d_lens_out != d_lens) TRY(check_apart(l2, {l}));
+  TRY(behind_default_stream(n));
+  ForkPages f;
+  f.table = d_table;
+  f.lens = d_lens;
+  f.parents = d_parents;
+  f.grow = d_grow;
+  f.table_out = d_table_out;
+  f.lens_out = d_lens_out;
+  f.old = sequences;
+  f.n = new_sequences;
+  f.max_pages = max_pages;
+  f.page_rows = page_rows;
+  f.pages = pages;
+  TRY(alloc(n, n->op_ws, fork_ws_bytes(f.n, f.max_pages, f.pages)));
+  f.ws = n->op_ws.p;
+  TRY(stage_fork(n, f));
+  PagePool pool;
+  pool.k = (double2*)d_k_pages;
+  pool.v = (double2*)d_v_pages;
+  pool.layers = (int)layers;
+  pool.H = (int)heads;
+  pool.dh = (int)dh;
+  fork_plan(n->stream, f);
+  fork_copy(n->stream, f, pool, true);
+  const int rc = op_finish(n);
+  if (rc != ERR_HIP) n->fork_dirty = false;
+  return rc;
+}
+
+static int check_beams(uint32_t groups, uint32_t beams, uint32_t V, uint32_t keep) {
+  if (!groups || !beams || !V) return fail(ERR_ARG, "beam selection: bad shape");
+  if (!keep || keep > (uint32_t)BEAM_MAX_KEEP) return fail(ERR_ARG, "beam selection: %u kept, 1 to %d", keep, BEAM_MAX_KEEP);
+  if (beams > BEAM_MAX || (uint64_t)beams * V > 1u << 30 || (uint64_t)groups * beams > 1u << 23)
+    return fail(ERR_ARG, "beam selection: at most %u beams, 2^30 logits of a group and 2^23 rows", BEAM_MAX);
+  return OK;
+}
+
+int mitok_beam_select_device(mitok_network* n, const double* d_logits, const double* d_scores, const uint32_t* d_done,
+                             const double* d_scale, uint32_t B, uint32_t beams, uint32_t V, uint32_t keep,
+                             uint32_t* d_parents, uint32_t* d_tokens, double* d_scores_out) {
+  if (!n || !d_logits || !d_scores || !d_parents || !d_tokens || !d_scores_out)
+    return fail(ERR_ARG, "beam selection: null argument");
+  TRY(check_beams(B, beams, V, keep));
+  TRY(set_device(n));
+  const size_t xb = times({B, beams, V, sizeof(double)}), sb = times({B, beams, sizeof(double)}), db = times({B, beams, sizeof(uint32_t)});
+  const size_t ob = times({B, keep, sizeof(uint32_t)}), bb = times({B, keep, sizeof(double)});
+  TRY(check_device_array(n, d_logits, xb, 8, "logits"));
+  TRY(check_device_array(n, d_scores, sb, 8, "scores"));
+  if (d_done) TRY(check_device_array(n, d_done, db, 4, "done"));
+  if (d_scale) TRY(check_device_array(n, d_scale, sb, 8, "scale"));
+  TRY(check_device_array(n, d_parents, ob, 4, "parents"));
+  TRY(check_device_array(n, d_tokens, ob, 4, "tokens"));
+  TRY(check_device_array(n, d_scores_out, bb, 8, "scores_out"));
+  const Span x = {d_logits, xb, "logits"}, s = {d_scores, sb, "scores"}, d = {d_done, db, "done"}, c = {d_scale, sb, "scale"};
+  const Span p = {d_parents, ob, "parents"}, t = {d_tokens, ob, "tokens"}, o = {d_scores_out, bb, "scores_out"};
+  TRY(check_apart(p, {x, s, d, c, t, o}));
+  TRY(check_apart(t, {x, s, d, c, o}));
+  TRY(check_apart(o, {x, s, d, c}));
+  TRY(behind_default_stream(n));
+  BeamSelect b;
+  b.x = d_logits;
+  b.scores = d_scores;
+  b.done = d_done;
+  b.scale = d_scale;
+  b.groups = (int)B;
+  b.beams = (int)beams;
+  b.V = (int)V;
+  b.keep = (int)keep;
+  b.parents = d_parents;
+  b.tokens = d_tokens;
+  b.best = d_scores_out;
+  b.err = n->page_err;
+  TRY(alloc(n, n->op_ws, beam_ws_bytes(b)));
+  b.ws = n->op_ws.p;
+  beam_select(n->stream, b);
+  return op_finish(n);
+}
+
+int mitok_beam_select(mitok_network* n, const double* logits, const double* scores, const uint32_t* done, const double* scale,
+                      uint32_t B, uint32_t beams, uint32_t V, uint32_t keep, uint32_t* parents, uint32_t* tokens,
+                      double* scores_out) {
+  if (!n || !logits || !scores || !parents || !tokens || !scores_out) return fail(ERR_ARG, "beam selection: null argument");
+  TRY(check_beams(B, beams, V, keep));
+  TRY(set_device(n));
+  const size_t rows = (size_t)B * beams, out = (size_t)B * keep;
+  DevBuf x, s, d, c, p, t, o;
+  const auto put = [&](DevBuf& b, const void* src, size_t bytes) -> int {
+    if (bytes == SIZE_MAX) return fail(ERR_ARG, "beam selection: a size passes 64 bits");
+    if (!src) return OK;
+    TRY(alloc(n, b, bytes));
+    HIP_TRY(hipMemcpyAsync(b.p, src, bytes, hipMemcpyHostToDevice, n->stream));
+    return OK;
+  };
+  TRY(put(x, logits, times({rows, V, sizeof(double)})));
+  TRY(put(s, scores, rows * sizeof(double)));
+  TRY(put(d, done, rows * sizeof(uint32_t)));
+  TRY(put(c, scale, rows * sizeof(double)));
+  TRY(alloc(n, p, out * sizeof(uint32_t)));
+  TRY(alloc(n, t, out * sizeof(uint32_t)));
+  TRY(alloc(n, o, out * sizeof(double)));
+  TRY(mitok_beam_select_device(n, x.as<double>(), s.as<double>(), d.as<uint32_t>(), c.as<double>(), B, beams, V, keep,
+                               p.as<uint32_t>(), t.as<uint32_t>(), o.as<double>()));
+  HIP_TRY(hipMemcpyAsync(parents, p.p, out * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
+  HIP_TRY(hipMemcpyAsync(tokens, t.p, out * sizeof(uint32_t), hipMemcpyDeviceToHost, n->stream));
+  HIP_TRY(hipMemcpyAsync(scores_out, o.p, out * sizeof(double), hipMemcpyDeviceToHost, n->stream));
+  HIP_TRY(hipStreamSynchronize(n->stream));
+  return OK;
+}
+
+// A beam search's sizes and its arrays on the device.
+struct BeamRun {
+  uint32_t G = 0, K = 0, R = 0, P = 0, pages = 0;  // prompts, beams, G * K, pages of a sequence, of the pool
+  uint32_t *table0, *table, *lens_out, *live, *hist, *done[2], *len[2], *ids, *from;
+  double *zero, *best[2], *scale;
+  size_t layout(char* base, uint32_t n_new) {
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+      char* q = base ? base + at : nullptr;
+      at += (bytes + 255) & ~(size_t)255;
+      return q;
+    };
+    const auto words = [&](size_t k) { return (uint32_t*)take(k * sizeof(uint32_t)); };
+    zero = (double*)take(G * sizeof(double));
+    live = words(n_new);  // behind `zero`: cleared together with it
+    for (double** b : {&best[0], &best[1], &scale}) *b = (double*)take(R * sizeof(double));
+    for (uint32_t** w : {&done[0], &done[1], &len[0], &len[1], &ids, &from}) *w = words(R);
+    lens_out = words(std::max(G, R));
+    hist = words(2 * (size_t)R * n_new);  // parents and tokens of each step
+    table0 = words((size_t)G * P);
+    table = words((size_t)R * P);
+    return at;
+  }
+};
+constexpr uint32_t BEAM_PAGE_ROWS = 16;  // the smallest page: a fork copies the fewest rows
+constexpr int BEAM_WINDOW = 16;          // steps that one plan of the attention serves
+constexpr uint32_t BEAM_LOOK = 32;       // steps between two looks at whether a beam is left
+
+static int beam_search_impl(Net* n, const uint32_t* prompt, const uint32_t* lens, uint32_t G, uint32_t S, uint32_t K,
+                            uint32_t n_new, uint32_t end_id, double power, uint32_t* out_ids, uint32_t* out_lens,
+                            double* out_scores) {
+  TRY(mitok_reset(n));
+  hipStream_t st = n->stream;
+  const uint32_t V = n->layers[n->layers.size() - 2]->d_out, last = (uint32_t)n->layers.size(), steps = n_new - 1;
+  std::vector<SelfAttentionLayer*> layers;
+  for (auto& L : n->layers)
+    if (L->kind == K_SELF_ATTENTION) layers.push_back((SelfAttentionLayer*)L.get());
+  if (layers.empty()) return fail(ERR_STATE, "beam search: the stack has no attention layer");
+  const uint32_t ps = BEAM_PAGE_ROWS;
+  PagedPass first, step;
+  first.by_row = true;
+  BeamRun r;
+  r.G = G;
+  r.K = K;
+  r.R = G * K;
+  Spec sp = decode_spec(n, r.R);
+  sp.paged = &step;
+  TRY(prepare(n, sp));
+  Spec pre;
+  pre.last = last;
+  pre.last_row = true;
+  pre.paged = &first;
+  std::vector<uint32_t> mask_h;
+  TRY(begin_call(n, lens, G, S, nullptr, true, nullptr, pre, mask_h));
+  TRY(prepare(n, sp));  // the prompt's may have been the larger
+  // rows that each prompt leaves (compressed by the wavelet stages, if any), and the pages they and the beams need
+  const std::vector<uint32_t> rows(cached_lens(n, lens), cached_lens(n, lens) + G);
+  const uint32_t wide = (uint32_t)n->wS, longest = *std::max_element(rows.begin(), rows.end());
+  uint32_t far = 0;
+  uint64_t pages = (uint64_t)r.R * ((ps - 1 + n_new + ps - 1) / ps);
+  for (uint32_t g = 0; g < G; ++g) {
+    pages += (rows[g] + ps - 1) / ps;
+    far = std::max(far, lens[g]);
+  }
+  if (pages > POOL_MAX_PAGES) return fail(ERR_ARG, "beam search: %llu pages, at most %u", (unsigned long long)pages, POOL_MAX_PAGES);
+  r.pages = (uint32_t)pages;
+  r.P = (longest + n_new + ps - 1) / ps;
+  TRY(ensure_rope_for(n, 0, last, (int)std::max<uint32_t>(rope_positions_needed(n), far + n_new)));
+  for (auto* A : layers) {
+    const size_t bytes = times({r.pages, ps, A->d_in, sizeof(double2)});
+    TRY(check_heads("beam search", r.R, A->heads));
+    TRY(alloc(n, A->kp, bytes));
+    TRY(alloc(n, A->vp, bytes));
+  }
+  TRY(alloc(n, n->beam_state, r.layout(nullptr, n_new)));
+  r.layout((char*)n->beam_state.p, n_new);
+
+  // what every pass reads of the host: prompt rows, then of each step the rows before it and their positions
+  std::vector<int> tab;
+  const auto put = [&](auto&& value, uint32_t count) {
+    const uint32_t at = (uint32_t)(tab.size() * sizeof(int));
+    for (uint32_t i = 0; i < count; ++i) tab.push_back((int)value(i));
+    return at;
+  };
+  const uint32_t none_at = put([](uint32_t) { return 0; }, G), rows_at = put([&](uint32_t g) { return rows[g]; }, G);
+  const uint32_t ones_at = put([](uint32_t) { return 1; }, r.R);
+  std::vector<uint32_t> lens_at(steps), pos_at(steps);
+  for (uint32_t s = 0; s < steps; ++s) {
+    lens_at[s] = put([&](uint32_t i) { return rows[i / K] + s; }, r.R);
+    pos_at[s] = put([&](uint32_t i) { return lens[i / K] + s; }, r.R);
+  }
+  size_t ws = 0;
+  const auto plan = [&](PagedPass& pass, uint32_t B, uint32_t m, const int* kv, const int* cnt) {
+    PagedAttn& a = pass.a;
+    a.B = (int)B;
+    a.n = (int)m;
+    a.max_pages = (int)r.P;
+    a.page_rows = (int)ps;
+    a.pages = r.pages;
+    a.err = n->page_err;
+    std::vector<PagedPlan> plans;
+    for (size_t k = 0; k < layers.size(); ++k) {
+      a.H = (int)layers[k]->heads;
+      a.dh = (int)layers[k]->dh;
+      size_t same = 0;
+      while (layers[same]->heads != layers[k]->heads || layers[same]->dh != layers[k]->dh) ++same;
+      plans.push_back(same < k ? plans[same] : paged_plan(a, kv, cnt, tab));
+      ws = std::max(ws, paged_ws_bytes(a, plans.back()));
+    }
+    return plans;
+  };
+  const std::vector<int> none(G, 0), count(rows.begin(), rows.end()), ones(r.R, 1);
+  first.plans = plan(first, G, wide, none.data(), count.data());
+  first.a.table = r.table0;
+  first.a.kv_len = none_at;
+  first.a.count = rows_at;
+  std::vector<std::vector<PagedPlan>> windows;
+  for (uint32_t s = 0; s < steps; s += BEAM_WINDOW) {
+    std::vector<int> kv(r.R);
+    for (uint32_t i = 0; i < r.R; ++i) kv[i] = (int)(rows[i / K] + std::min<uint32_t>(s + BEAM_WINDOW, steps) - 1);
+    windows.push_back(plan(step, r.R, 1, kv.data(), ones.data()));
+  }
+  step.a.table = r.table;
+  step.a.count = ones_at;
+  for (const auto& plans : windows)
+    for (size_t k = 0; k < layers.size(); ++k)
+      if ((uint64_t)plans[k].entries * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
+  for (size_t k = 0; k < layers.size(); ++k)
+    if ((uint64_t)first.plans[k].entries * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
+
+  ForkPages f;
+  f.max_pages = r.P;
+  f.page_rows = ps;
+  f.pages = r.pages;
+  f.lens_out = r.lens_out;
+  BeamSelect b;
+  b.V = (int)V;
+  b.groups = (int)G;
+  b.keep = (int)K;
+  b.err = n->page_err;
+  b.beams = (int)K;
+  ws = std::max({ws, fork_ws_bytes(r.R, r.P, r.pages), beam_ws_bytes(b)});
+  TRY(alloc(n, n->op_ws, ws));
+  first.a.ws = step.a.ws = f.ws = b.ws = n->op_ws.p;
+  TRY(stage_fork(n, f));
+  TRY(op_staging(n, tab.size() * sizeof(int)));
+  memcpy(n->op_host, tab.data(), tab.size() * sizeof(int));
+  TRY(op_upload(n, tab.size() * sizeof(int)));
+  const char* d_tab = (const char*)n->op_tab.p;
+  first.a.tab = step.a.tab = d_tab;
+  std::vector<uint32_t> padded((size_t)G * S);
+  for (uint32_t g = 0; g < G; ++g)
+    for (uint32_t s = 0; s < S; ++s) padded[(size_t)g * S + s] = s < lens[g] ? prompt[(size_t)g * S + s] : 1u;
+  TRY(upload(n, n->ids_d, padded.data(), padded.size() * sizeof(uint32_t)));
+  HIP_TRY(hipStreamSynchronize(st));  // padded goes out of scope on an error
+  fill_u32(st, (uint32_t*)r.zero, ((char*)r.best[0] - (char*)r.zero) / sizeof(uint32_t), 0);
+  fill_u32(st, n->ones_d.as<uint32_t>(), r.R, 1);
+
+  const auto fork = [&](uint32_t old, uint32_t news, const uint32_t* table, uint32_t lens_of, uint32_t* to) {
+    f.old = old;
+    f.n = news;
+    f.table = table;
+    f.table_out = to;
+    f.lens = (const uint32_t*)(d_tab + lens_of);
+    fork_plan(st, f);
+    for (size_t k = 0; k < layers.size(); ++k) {
+      PagePool pool;
+      pool.k = layers[k]->kp.as<double2>();
+      pool.v = layers[k]->vp.as<double2>();
+      pool.H = (int)layers[k]->heads;
+      pool.dh = (int)layers[k]->dh;
+      fork_copy(st, f, pool, k == 0);
+    }
+  };
+  // pages for the prompts: G sequences without rows that grow by them
+  f.grow = (const uint32_t*)(d_tab + rows_at);
+  fork(G, G, r.table0, none_at, r.table0);
+  f.grow = nullptr;
+  f.grow_all = 1;
+  f.parents = r.from;
+  pre.ids = n->ids_d.as<uint32_t>();
+  pre.out_re = n->logits_re.as<double>();
+  TRY(enqueue_forward(n, pre));
+
+  sp.ids = r.ids;
+  sp.mask = n->ones_d.as<uint32_t>();
+  sp.lens = n->ones_d.as<uint32_t>();
+  sp.out_re = n->logits_re.as<double>();
+  BeamAdvance v;
+  v.groups = (int)G;
+  v.keep = (int)K;
+  v.V = (int)V;
+  v.end = end_id;
+  v.power = power;
+  v.scale_out = r.scale;
+  v.ids = r.ids;
+  v.from = r.from;
+  uint32_t s = 0;  // the last step selected
+  for (;; ++s) {
+    b.x = n->logits_re.as<double>();
+    b.beams = s ? (int)K : 1;
+    b.scores = s ? r.best[(s - 1) & 1] : r.zero;
+    b.done = s ? r.done[(s - 1) & 1] : nullptr;
+    b.scale = s ? r.scale : nullptr;
+    b.parents = r.hist + 2 * (size_t)r.R * s;
+    b.tokens = b.parents + r.R;
+    b.best = r.best[s & 1];
+    beam_select(st, b);
+    v.parents = b.parents;
+    v.tokens = b.tokens;
+    v.done = b.done;
+    v.len = s ? r.len[(s - 1) & 1] : nullptr;
+    v.beams = b.beams;
+    v.done_out = r.done[s & 1];
+    v.len_out = r.len[s & 1];
+    v.live = r.live + s;
+    beam_advance(st, v);
+    if (s == steps) break;
+    if (end_id != MITOK_NO_TOKEN && (s + 1) % BEAM_LOOK == 0) {  // all ended?
+      uint32_t live = 0;
+      HIP_TRY(hipMemcpyAsync(&live, v.live, sizeof live, hipMemcpyDeviceToHost, st));
+      HIP_TRY(hipStreamSynchronize(st));
+      if (!live) break;
+    }
+    fork(s ? r.R : G, r.R, s ? r.table : r.table0, s ? lens_at[s] : rows_at, r.table);
+    step.plans = windows[s / BEAM_WINDOW];
+    step.a.kv_len = lens_at[s];
+    sp.pos = (const int*)(d_tab + pos_at[s]);
+    TRY(enqueue_forward(n, sp));
+  }
+  std::vector<uint32_t> hist(2 * (size_t)r.R * (s + 1)), count_out(r.R);
+  HIP_TRY(hipMemcpyAsync(hist.data(), r.hist, hist.size() * sizeof(uint32_t), hipMemcpyDeviceToHost, st));
+  HIP_TRY(hipMemcpyAsync(count_out.data(), r.len[s & 1], r.R * sizeof(uint32_t), hipMemcpyDeviceToHost, st));
+  HIP_TRY(hipMemcpyAsync(out_scores, r.best[s & 1], r.R * sizeof(double), hipMemcpyDeviceToHost, st));
+  const int rc = op_finish(n);
+  collect_timing(n);
+  TRY(check_err_word(n));  // the first cause
+  TRY(rc);
+  n->fork_dirty = false;
+  // each hypothesis from its end to its start
+  std::fill(out_ids, out_ids + (size_t)r.R * n_new, MITOK_NO_TOKEN);
+  for (uint32_t i = 0; i < r.R; ++i) {
+    uint32_t at = i, left = out_lens[i] = count_out[i];
+    for (uint32_t k = s + 1; k-- > 0 && left;) {
+      const uint32_t *parents = hist.data() + 2 * (size_t)r.R * k, token = parents[r.R + at];
+      if (token != MITOK_NO_TOKEN) out_ids[(size_t)i * n_new + --left] = token;
+      at = parents[at];
+    }
+  }
+  return OK;
+}
+
+int mitok_beam_search(mitok_network* n, const uint32_t* prompt, const uint32_t* lens, uint32_t B, uint32_t S, uint32_t beams,
+                      uint32_t n_new, uint32_t end_id, double length_power, uint32_t* out_ids, uint32_t* out_lens,
+                      double* out_scores) {
+  if (!out_lens || !out_scores) return fail(ERR_ARG, "null argument");
+  TRY(check_loop_args(n, prompt, lens, B, S, n_new ? n_new - 1 : 0, out_ids));
+  if (!n_new || n_new > OP_MAX_CTX) return fail(ERR_ARG, "beam search: %u new tokens", n_new);
+  if (!beams || beams > (uint32_t)BEAM_MAX_KEEP) return fail(ERR_ARG, "beam search: %u beams, 1 to %d", beams, BEAM_MAX_KEEP);
+  if ((uint64_t)B * beams > POOL_MAX_SEQS) return fail(ERR_ARG, "beam search: more than %u sequences", POOL_MAX_SEQS);
+  if (!(std::fabs(length_power) <= 16.0)) return fail(ERR_ARG, "beam search: length_power outside [-16, 16]");
+  const int rc = guarded([&] {
+    return beam_search_impl(n, prompt, lens, B, S, beams, n_new, end_id, length_power, out_ids, out_lens, out_scores);
+  });
+  return rc ? drop_moved(n, rc) : OK;
 }
 
 int mitok_last_timings(mitok_network* n, double* t3) {

@@ -306,10 +306,6 @@ void pick_ids(hipStream_t st, const uint32_t* ids, int n, const int* last, int B
 // ===========================================================================
 // logits to a token
 // ===========================================================================
-__device__ __forceinline__ void set_err(uint32_t* err, int word) {
-  __hip_atomic_store(err + word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-}
-
 __device__ __forceinline__ bool bad_penalties(const LogitRules& r, long row) {
   const double *p = r.penalties + 3 * row;
   return !(p[0] > 0.0 && isfinite(p[0]) && isfinite(p[1]) && isfinite(p[2]));
@@ -331,8 +327,8 @@ __global__ __launch_bounds__(256) void k_logit_check(LogitRules r) {
       bad |= t != NO_TOKEN && t >= (uint32_t)r.V;
     }
     const bool pen = threadIdx.x == 0 && r.penalties && bad_penalties(r, row);
-    if (bad) set_err(r.err, OE_BAD_TOKEN);
-    if (pen) set_err(r.err, OE_BAD_PENALTY);
+    if (bad) set_word(r.err, OE_BAD_TOKEN);
+    if (pen) set_word(r.err, OE_BAD_PENALTY);
     if (bad || pen) __hip_atomic_store(r.refused, r.call, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
 }
@@ -386,7 +382,7 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
     theta = r.penalties[3 * (long)row];
     presence = r.penalties[3 * (long)row + 1];
     frequency = r.penalties[3 * (long)row + 2];
-    if (tid == 0 && bad_penalties(r, row)) set_err(r.err, OE_BAD_PENALTY);
+    if (tid == 0 && bad_penalties(r, row)) set_word(r.err, OE_BAD_PENALTY);
   }
   const bool ruled = r.hist > 0 || r.nb > 0;
   if (ruled) {
@@ -398,12 +394,12 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
   if (ruled) {
     for (int i = tid; i < r.hist; i += 256) {
       const uint32_t t = r.history[(long)row * r.hist + i];
-      if (t != NO_TOKEN && t >= (uint32_t)V) set_err(r.err, OE_BAD_TOKEN);
+      if (t != NO_TOKEN && t >= (uint32_t)V) set_word(r.err, OE_BAD_TOKEN);
       if (t - (uint32_t)c0 < (uint32_t)len) atomicAdd(&count[t - c0], 1u);
     }
     for (int i = tid; i < r.nb; i += 256) {
       const uint32_t t = r.bias_ids[(long)row * r.nb + i];
-      if (t != NO_TOKEN && t >= (uint32_t)V) set_err(r.err, OE_BAD_TOKEN);
+      if (t != NO_TOKEN && t >= (uint32_t)V) set_word(r.err, OE_BAD_TOKEN);
       if (t - (uint32_t)c0 < (uint32_t)len) atomicMax(&entry[t - c0], (uint32_t)i + 1);
     }
     __syncthreads();
@@ -439,7 +435,7 @@ __global__ __launch_bounds__(256) void k_logit_rules(LogitRules r, int row0) {
       *out = y[k].x;
     }
   }
-  if (__ballot(nan) && lane == 0) set_err(r.err, OE_NAN);
+  if (__ballot(nan) && lane == 0) set_word(r.err, OE_NAN);
   if (!r.ids) return;
   wave_argmax(bv, bi);
   if (lane == 0) sv[wave] = bv, si[wave] = bi;

@@ -15,6 +15,9 @@ namespace mitok {
 // Words a kernel sets and the host reads once the stream is idle (pinned host
 // memory: no copy back).  Plain stores of 1, so any number of lanes may set one.
 enum OpErrWord : int { OE_BAD_TOKEN = 0, OE_NAN = 1, OE_BAD_PENALTY = 2, OE_WORDS = 4 };
+__device__ __forceinline__ void set_word(uint32_t* err, int word) {
+  __hip_atomic_store(err + word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
 
 // The host's small arrays of a call (lengths, trees, lists), at byte offsets of
 // one table: in the kernels' own arguments where they fit, which saves the

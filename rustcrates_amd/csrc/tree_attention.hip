@@ -22,10 +22,10 @@
 // tile's keys are requested once the last tile's scores are formed, its values
 // once the last tile's output is.  Waves, then chunks (k_tree_join) are merged
 // by their maxima.
-// D[i][j] of a 16x16 tile sits at lane j + 16 * (i % 4), element i / 4.
 #include <algorithm>
 #include <cmath>
 
+#include "attn_run.hpp"
 #include "serving.hpp"
 
 namespace mitok {
@@ -110,77 +110,6 @@ __device__ __forceinline__ void tree_scores(const TreeAttn& a, const TreePlan& p
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (t + 4 * e + kq < at.t1) x[4 * e * (uint32_t)a.weigh] = s[e];
-}
-
-// One wave's running softmax over 16-slot tiles for the node lane % 16, and
-// its output (column 16 c + 4 e + lane / 16).
-template <int DHP>
-struct TreeRun {
-  static constexpr int CT = DHP / 16;
-  v4d o_re[CT], o_im[CT];
-  double m = -INFINITY, l = 0.0;  // l over this lane's slots alone
-  __device__ __forceinline__ TreeRun() {
-#pragma unroll
-    for (int c = 0; c < CT; ++c) o_re[c] = o_im[c] = v4d{0.0, 0.0, 0.0, 0.0};
-  }
-  // A tile's scores become its weights e^(s - m).  Any m near the largest score
-  // serves, so it moves only where a score passes it by 8 (weights up to e^8
-  // then), which after the first tiles hardly happens: no maximum across the
-  // lanes and no rescaling, which costs as much as 8 MFMAs (double arithmetic
-  // and double MFMAs take turns on a SIMD: 4 cycles an operation beside 64).
-  // Each node goes by its own scores, so its bits do not depend on the others'.
-  __device__ __forceinline__ void soften(v4d& s) {
-    const double top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
-    if (__ballot(top > m + 8.0)) {
-      double x, y;
-      pair16_f64(top, x, y);
-      pair32_f64(fmax(x, y), x, y);
-      const double most = fmax(x, y), mn = most > m + 8.0 ? most : m;
-      const double keep = mn == m ? 1.0 : exp(m - mn);
-      m = mn;
-      l *= keep;
-#pragma unroll
-      for (int c = 0; c < CT; ++c) o_re[c] *= keep, o_im[c] *= keep;
-    }
-    const double base = m == -INFINITY ? 0.0 : m;  // nothing seen yet: every weight e^-inf = 0
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      s[e] = exp(s[e] - base);
-      l += s[e];
-    }
-  }
-  __device__ __forceinline__ void output(const v4d& s, int q, int c, double2 v) {
-    o_re[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(v.x, s[q], o_re[c], 0, 0, 0);
-    o_im[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(v.y, s[q], o_im[c], 0, 0, 0);
-  }
-  // Values that are not finite are left out of a tile's products, where 0 times
-  // them is NaN in the rows of nodes that do not see them, and added here to
-  // those that do, slot by slot.
-  __device__ __forceinline__ void add_left_out(const TreeAt& at, const double2* V, int dh, int t, const v4d& s, unsigned vis) {
-    const int lane = threadIdx.x & 63, node = lane & 15, kq = lane >> 4;
-    for (int k = 0; k < 16 && t + k < at.t1; ++k) {
-      const int from = node + 16 * (k & 3), q = k >> 2;
-      const double pk = __shfl(q == 0 ? s[0] : q == 1 ? s[1] : q == 2 ? s[2] : s[3], from);
-      const bool see = (__shfl((int)vis, from) >> q) & 1;
-#pragma unroll
-      for (int c = 0; c < CT; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int col = 16 * c + 4 * e + kq;
-          if (see && col < dh) {
-            const double2 v = V[(long)(t + k) * dh + col];
-            if (!isfinite(v.x)) o_re[c][e] += pk * v.x;
-            if (!isfinite(v.y)) o_im[c][e] += pk * v.y;
-          }
-        }
-    }
-  }
-};
-__device__ __forceinline__ bool tree_finite(double2& v) {  // what is not finite becomes 0
-  const bool nx = !isfinite(v.x), ny = !isfinite(v.y);
-  if (nx) v.x = 0.0;
-  if (ny) v.y = 0.0;
-  return !(nx || ny);
 }
 
 // A node's output row element: final where the sequence has one chunk, else the chunk's part.
@@ -279,7 +208,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
   }
   __syncthreads();
 
-  TreeRun<DHP> run;
+  AttnRun<DHP> run;
   for (; t < t1; t += 16 * KG) {
     v4d s = {0.0, 0.0, 0.0, 0.0}, z = s;
 #pragma unroll
@@ -302,7 +231,7 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 #pragma unroll
       for (int q = 0; q < (PRE ? 4 : 0); ++q)
 #pragma unroll
-        for (int c = 0; c < CT; ++c) fine &= tree_finite(vf[q][c]);
+        for (int c = 0; c < CT; ++c) fine &= attn_finite(vf[q][c]);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -310,13 +239,13 @@ __global__ __launch_bounds__(256, DHP <= 128 ? 2 : 1) void k_tree_split(TreeAttn
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
         double2 v = PRE ? vf[PRE ? q : 0][PRE ? c : 0] : value_at(t, q, c);
-        if (!PRE && drafted) fine &= tree_finite(v);
+        if (!PRE && drafted) fine &= attn_finite(v);
         run.output(s, q, c, v);
       }
       if (!PRE) __builtin_amdgcn_sched_barrier(0);
     }
     if (more) load_values(t + 16 * KG);
-    if (__ballot(!fine)) run.add_left_out(at, V, dh, t, s, vis);
+    if (__ballot(!fine)) run.add_left_out([&](int k) { return V + (long)(t + k) * dh; }, dh, t1 - t, s, vis);
   }
 
   // the waves of a node group, rescaled to their common maximum and added in order
@@ -415,7 +344,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
     if (t + 16 > at.L) {
       bool fine = true;
 #pragma unroll
-      for (int c = 0; c < CT; ++c) fine &= tree_finite(next[U / 4 + c]);
+      for (int c = 0; c < CT; ++c) fine &= attn_finite(next[U / 4 + c]);
       if (!fine) left_out = 1;
     }
     double2* to = tiles + buf * F * 64;
@@ -439,7 +368,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
   leave(0, t0);
   __syncthreads();
 
-  TreeRun<DHP> run;
+  AttnRun<DHP> run;
   int buf = 0;
   for (int t = t0; t < t1; t += 16, buf ^= 1) {
     const double2* tile = tiles + buf * F * 64;
@@ -474,7 +403,7 @@ __global__ __launch_bounds__(256, DHP <= 64 ? 2 : 1) void k_tree_shared(TreeAttn
       for (int c = 0; c < CT; ++c) run.output(s, q, c, tile[(U + q * CT + c) * 64 + lane]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (t + 16 > at.L && left_out) run.add_left_out(at, V, dh, t, s, vis);
+    if (t + 16 > at.L && left_out) run.add_left_out([&](int k) { return V + (long)(t + k) * dh; }, dh, t1 - t, s, vis);
     leave(buf ^ 1, t + 16);  // read by nobody since the last barrier (after the last tile: by nobody at all)
     __syncthreads();
   }
