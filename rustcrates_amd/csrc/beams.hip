@@ -208,29 +208,27 @@ void fork_copy(hipStream_t st, const ForkPages& f, const PagePool& pool, bool co
 // ===========================================================================
 // selection
 // ===========================================================================
-// A row is cut into pieces of BS_PIECE logits, a wave each: its maximum, the
-// first token that has it, and the sum of exponentials below that.  Of the K best
-// pieces by their maxima none of the other pieces' logits can be among the K
-// best, nor any logit that comes after the least of those K maxima: so the
-// logits are read once, and of them again only K pieces.
-constexpr int BS_PER = 8, BS_PIECE = 64 * BS_PER;
+// A row is cut into pieces, a wave each: the sum of its exponentials, and the maximum
+// of each quarter, the share of 16 lanes.  Of the K best quarters by their maxima each
+// holds a continuation at least as good as the least of those maxima, so no
+// continuation below that bound is among the K best: the logits are read once, and of
+// them again only the quarters whose maximum reaches the bound.
 struct BeamWs {
-  double* m;  // [rows][pieces]
-  double* s;
-  int* at;
+  double* m;  // [rows][pieces][4]
+  double* s;  // [rows][pieces] of e^(x - the largest of the four)
 };
-static int beam_pieces(int V) { return (V + BS_PIECE - 1) / BS_PIECE; }
+// Logits of a piece: 512, or 256 where that leaves most of the chip idle.
+static int beam_piece(const BeamSelect& b) { return (long)b.groups * b.beams * ((b.V + 511) / 512) >= 2048 ? 512 : 256; }
 static size_t beam_layout(const BeamSelect& b, char* base, BeamWs& w) {
-  const size_t n = (size_t)b.groups * b.beams * beam_pieces(b.V);
+  const size_t n = (size_t)b.groups * b.beams * ((b.V + 255) / 256);
   size_t at = 0;
   const auto take = [&](size_t bytes) {
     char* q = base ? base + at : nullptr;
     at += (bytes + 255) & ~(size_t)255;
     return q;
   };
-  w.m = (double*)take(n * sizeof(double));
+  w.m = (double*)take(4 * n * sizeof(double));
   w.s = (double*)take(n * sizeof(double));
-  w.at = (int*)take(n * sizeof(int));
   return at;
 }
 size_t beam_ws_bytes(const BeamSelect& b) {
@@ -238,70 +236,94 @@ size_t beam_ws_bytes(const BeamSelect& b) {
   return beam_layout(b, nullptr, w);
 }
 
-// the larger value, of equal ones the lower index; NaN never wins
-__device__ __forceinline__ void first_max(double& v, int& i, double ov, int oi) {
-  if (ov > v || (ov == v && oi < i)) v = ov, i = oi;
-}
-template <int CTRL>
-__device__ __forceinline__ void first_max_dpp(double& v, int& i) {
-  first_max(v, i, dpp_f64<CTRL>(v), dpp_i32<CTRL>(i));
-}
-__device__ __forceinline__ void wave_first_max(double& v, int& i) {
-  first_max_dpp<DPP_XOR1>(v, i);
-  first_max_dpp<DPP_XOR2>(v, i);
-  first_max_dpp<DPP_HALF_MIRROR>(v, i);
-  first_max_dpp<DPP_MIRROR>(v, i);
-  double a, b;
-  int ia, ib;
-  pair16_f64(v, a, b);
-  pair16_i32(i, ia, ib);
-  first_max(a, ia, b, ib);
-  pair32_f64(a, v, b);
-  pair32_i32(ia, i, ib);
-  first_max(v, i, b, ib);
-}
+// two logits of a row, whose start is aligned to one
+typedef double v2logit __attribute__((ext_vector_type(2), aligned(8)));
 
 // a row without logits to read: ended, or of score -inf
 __device__ __forceinline__ bool beam_idle(const BeamSelect& b, long row) {
   return b.scores[row] == -INFINITY || (b.done && b.done[row]);
 }
 
-__global__ __launch_bounds__(256) void k_beam_pieces(BeamSelect b, BeamWs w, int pieces, long waves) {
-  const int lane = threadIdx.x & 63;
-  const long step = (long)gridDim.x * 4;
-  for (long x = (long)blockIdx.x * 4 + (threadIdx.x >> 6); x < waves; x += step) {
-    const long row = x / pieces;
-    const int piece = (int)(x - row * pieces), t0 = piece * BS_PIECE;
-    if (beam_idle(b, row)) continue;
-    const double* p = b.x + row * b.V;
-    double v[BS_PER];
-#pragma unroll
-    for (int k = 0; k < BS_PER; ++k) {
-      const int t = t0 + 64 * k + lane;
-      v[k] = t < b.V ? __builtin_nontemporal_load((const MITOK_GLOBAL double*)(p + t)) : -INFINITY;
-    }
-    double m = -INFINITY;
-    int at = INT32_MAX;
-    bool bad = false;
-#pragma unroll
-    for (int k = 0; k < BS_PER; ++k) {
-      bad |= !(v[k] < INFINITY);  // NaN, or an infinity that leaves no distribution
-      first_max(m, at, v[k], t0 + 64 * k + lane);
-    }
-    if (__ballot(bad) && lane == 0) set_word(b.err, PE_BAD_SCORE);
-    wave_first_max(m, at);
-    double s = 0.0;
-    if (m > -INFINITY) {
-#pragma unroll
-      for (int k = 0; k < BS_PER; ++k) s += exp(v[k] - m);
-    }
-    s = wave_sum(s);
-    if (lane == 0) {
-      w.m[x] = m;
-      w.s[x] = s;
-      w.at[x] = at;
-    }
+// The quarter at t0 of a row: a lane of 16 takes logits t0 + 32 k + 2 (lane % 16) and the one
+// behind, -inf past the row.  No branch between the loads, so that whoever waits for
+// them waits for them alone.
+__device__ __forceinline__ int beam_token(int t0, int k) { return t0 + 32 * k + 2 * (threadIdx.x & 15); }
+template <int PER>
+__device__ __forceinline__ void beam_load(const double* row, int V, int t0, v2logit (&v)[PER]) {
+  if (V < 2) {
+    for (int k = 0; k < PER; ++k) v[k] = v2logit{beam_token(t0, k) == 0 ? row[0] : -INFINITY, -INFINITY};
+    return;
   }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) v[k] = *(const MITOK_GLOBAL v2logit*)(row + min(beam_token(t0, k), V - 2));
+}
+template <int PER>
+__device__ __forceinline__ void beam_cut(int V, int t0, v2logit (&v)[PER]) {
+  if (V < 2) return;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int t = beam_token(t0, k);
+    if (t + 1 >= V) v[k] = v2logit{t < V ? v[k].y : -INFINITY, -INFINITY};  // the last two were read
+  }
+}
+
+// e^x for x <= 0 within a unit in the last place: x = k ln 2 + r, |r| <= ln 2 / 2 (ln 2
+// as a double and the rest of it), then Taylor's polynomial of degree 13 in r, whose
+// remainder r^14 / 14! is below 5e-18.  18 double operations: the range checks of the
+// library's exp cost a third more.
+__device__ __forceinline__ double exp_below(double x) {
+  x = fmax(x, -1100.0);  // e^-1100 is 0
+  const double k = rint(x * 0x1.71547652b82fep+0);
+  const double r = fma(-k, 0x1.abc9e3b39803fp-56, fma(-k, 0x1.62e42fefa39efp-1, x));
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return ldexp(p, (int)k);
+}
+
+template <int PER>
+__global__ __launch_bounds__(256) void k_beam_pieces(BeamSelect b, BeamWs w, int pieces, uint32_t blocks) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t row = blockIdx.x / blocks;
+  const int piece = (int)(blockIdx.x - row * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (piece >= pieces || beam_idle(b, row)) return;
+  const int t0 = piece * 128 * PER + (lane >> 4) * 32 * PER;
+  v2logit v[PER];
+  beam_load(b.x + (long)row * b.V, b.V, t0, v);
+  beam_cut(b.V, t0, v);
+  double m = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    bad |= !(v[k].x < INFINITY) || !(v[k].y < INFINITY);  // NaN, or an infinity that leaves no distribution
+    m = fmax(m, fmax(v[k].x, v[k].y));
+  }
+  if (__ballot(bad) && lane == 0) set_word(b.err, PE_BAD_SCORE);
+  m = row16_max(m);
+  const long at = (long)row * pieces + piece;
+  if ((lane & 15) == 0) w.m[4 * at + (lane >> 4)] = m;
+  double x, y;
+  pair16_f64(m, x, y);
+  pair32_f64(fmax(x, y), x, y);
+  m = fmax(x, y);
+  double s = 0.0;
+  if (m > -INFINITY) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) s += exp_below(v[k].x - m) + exp_below(v[k].y - m);
+  }
+  s = wave_sum(s);
+  if (lane == 0) w.s[at] = s;
 }
 
 // the order of continuations: rank, then the lower row, the larger logit, the lower token
@@ -309,11 +331,10 @@ struct Cont {
   double rank, x;
   int row, t;
 };
-__device__ __forceinline__ bool before(const Cont& a, const Cont& b) {
-  if (a.rank != b.rank) return a.rank > b.rank;
-  if (a.row != b.row) return a.row < b.row;
-  if (a.x != b.x) return a.x > b.x;
-  return a.t < b.t;
+__device__ __forceinline__ bool before(const Cont& a, const Cont& b) {  // without branches
+  const bool later = (a.x > b.x) | ((a.x == b.x) & (a.t < b.t));
+  const bool tied = (a.row < b.row) | ((a.row == b.row) & later);
+  return (a.rank > b.rank) | ((a.rank == b.rank) & tied);
 }
 // the first of a wave's continuations (each lane's own), in every lane
 __device__ __forceinline__ void wave_first(Cont& c) {
@@ -327,142 +348,266 @@ __device__ __forceinline__ void wave_first(Cont& c) {
   }
 }
 
-// One block per group.  Each round finds the first continuation after the last
-// one found: K rounds over the pieces' maxima give the K best pieces and the
-// bound, then the logits of those that do not come after the bound are listed
-// and each one's place is how many come before it.  Where the list overflows
-// (many equal logits, or fewer pieces than K), K rounds over the pieces' logits.
-constexpr int BS_LIST = 1024;
-__global__ __launch_bounds__(256) void k_beam_pick(BeamSelect b, BeamWs w, int pieces) {
-  __shared__ double lse[1024];  // of the group's rows
-  __shared__ Cont part[4], list[BS_LIST], chosen[BEAM_MAX_KEEP];
-  __shared__ int listed;
+// Ranks in BB_BINS equal steps of a range, a monotone whole number of each.
+constexpr int BB_BINS = 256;
+struct RankBins {
+  double lo, inv;
+  __device__ __forceinline__ RankBins(double low, double high) : lo(low) {
+    const double f = BB_BINS / (high - low);
+    inv = f < INFINITY ? f : 0.0;
+  }
+  __device__ __forceinline__ int of(double rank) const {
+    return (int)fmin(fmax((rank - lo) * inv, -1.0), (double)(BB_BINS - 1));
+  }
+};
+
+// largest value and sum of a row of 16 lanes, from one register each
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float v) {
+  return fmaxf(v, __int_as_float(dpp_i32<CTRL>(__float_as_int(v))));
+}
+__device__ __forceinline__ float row16_maxf(float v) {
+  return max_dpp<DPP_MIRROR>(max_dpp<DPP_HALF_MIRROR>(max_dpp<DPP_XOR2>(max_dpp<DPP_XOR1>(v))));
+}
+__device__ __forceinline__ int row16_sumi(int v) {
+  v += dpp_i32<DPP_XOR1>(v);
+  v += dpp_i32<DPP_XOR2>(v);
+  v += dpp_i32<DPP_HALF_MIRROR>(v);
+  return v + dpp_i32<DPP_MIRROR>(v);
+}
+__device__ __forceinline__ float wave_maxf(float v) {
+  int a, b;
+  pair16_i32(__float_as_int(row16_maxf(v)), a, b);
+  pair32_i32(__float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))), a, b);
+  return fmaxf(__int_as_float(a), __int_as_float(b));
+}
+
+// One block per group.  A histogram of the quarters' maxima gives a bound that K of
+// them reach; the continuations that reach it are listed, and a continuation's
+// place is how many of the list come before it.  Where the list is too long (few
+// quarters, or logits close together), a histogram of what reached the bound gives
+// a closer one; where that cannot part them (equal ranks), K rounds over the
+// quarters find one continuation each.
+constexpr int BS_LIST = 512, BS_PARTS = 4096, BS_WAVES = 16;
+constexpr int BS_HELD = 5;  // of a thread's quarters, maxima that wait in registers (5120: 12 rows of 50280 logits)
+template <int PER>
+__global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect b, BeamWs w, int pieces) {
+  __shared__ double lse[1024], had[1024], scale[1024];  // of the group's rows; lse NaN: ended
+  __shared__ Cont part[BS_WAVES], list[BS_LIST];
+  __shared__ int plist[BS_PARTS], bins[BB_BINS];
+  __shared__ float lows[BS_WAVES], highs[BS_WAVES];
+  __shared__ int sums[BS_WAVES], nparts, listed;
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = b.beams, K = b.keep;
+  const int parts = 4 * pieces, E = R * parts;  // quarters of a row, of the group
   const long row0 = (long)g * R;
-  for (int r = wave; r < R; r += 4) {
+  // what the rows need, requested at once; an idle row's has no meaning and is left out
+  double held[BS_HELD];
+#pragma unroll
+  for (int k = 0; k < BS_HELD; ++k) held[k] = tid + 1024 * k < E ? w.m[row0 * parts + tid + 1024 * k] : -INFINITY;
+  for (int r = wave; r < R; r += BS_WAVES) {
     const long row = row0 + r;
-    const double had = b.scores[row];
+    const double score = b.scores[row], f = b.scale ? b.scale[row] : 1.0;
+    const bool ended = b.done && b.done[row];
+    const auto largest = [&](int c) {
+      const double* q = w.m + 4 * (row * pieces + c);
+      return fmax(fmax(q[0], q[1]), fmax(q[2], q[3]));
+    };
+    double mc[2], sc[2], m = -INFINITY, s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = lane + 64 * k;
+      mc[k] = c < pieces ? largest(c) : -INFINITY;
+      sc[k] = c < pieces ? w.s[row * pieces + c] : 0.0;
+    }
+    if (score > -INFINITY && !ended) {
+      m = fmax(mc[0], mc[1]);
+      for (int c = lane + 128; c < pieces; c += 64) m = fmax(m, largest(c));
+      m = wave_max(m);
+      if (m > -INFINITY) {
+        s = sc[0] * exp_below(mc[0] - m) + sc[1] * exp_below(mc[1] - m);
+        for (int c = lane + 128; c < pieces; c += 64) s += w.s[row * pieces + c] * exp_below(largest(c) - m);
+        s = wave_sum(s);
+      }
+    }
     if (lane == 0) {
-      if (isnan(had) || had == INFINITY) set_word(b.err, PE_BAD_SCORE);
-      if (b.scale && !(b.scale[row] > 0.0 && b.scale[row] < INFINITY)) set_word(b.err, PE_BAD_SCALE);
+      if (isnan(score) || score == INFINITY) set_word(b.err, PE_BAD_SCORE);
+      if (!(f > 0.0 && f < INFINITY)) set_word(b.err, PE_BAD_SCALE);
+      had[r] = score;
+      scale[r] = f;
+      lse[r] = ended ? NAN : m > -INFINITY ? m + log(s) : 0.0;  // a row that allows nothing: every logit stays -inf
     }
-    if (beam_idle(b, row)) continue;
-    double m = -INFINITY, s = 0.0;
-    for (int c = lane; c < pieces; c += 64) m = fmax(m, w.m[row * pieces + c]);
-    m = wave_max(m);
-    if (m > -INFINITY) {
-      for (int c = lane; c < pieces; c += 64) s += w.s[row * pieces + c] * exp(w.m[row * pieces + c] - m);
-      s = wave_sum(s);
-    }
-    if (lane == 0) lse[r] = m > -INFINITY ? m + log(s) : 0.0;  // a row that allows nothing: every logit stays -inf
   }
-  if (tid == 0) listed = 0;
+  if (tid == 0) nparts = 0;
   __syncthreads();
-  const auto cont = [&](int r, double x, int t) {
-    Cont c;
-    c.row = r;
-    c.x = x;
-    c.t = t;
-    c.rank = (b.scores[row0 + r] + (x - lse[r])) * (b.scale ? b.scale[row0 + r] : 1.0);
-    return c;
-  };
   const Cont none = {-INFINITY, -INFINITY, INT32_MAX, INT32_MAX};
-  // entry e of the group's pieces: its best continuation; an ended row's one continuation is its first piece's
-  const auto entry = [&](int e) {
-    const int r = e / pieces, c = e - r * pieces;
-    const long row = row0 + r;
-    if (b.scores[row] == -INFINITY) return none;
-    if (b.done && b.done[row]) {
-      if (c) return none;
-      Cont o = {b.scores[row] * (b.scale ? b.scale[row] : 1.0), 0.0, r, -1};
-      return o;
-    }
-    return cont(r, w.m[row * pieces + c], w.at[row * pieces + c]);
+  const auto rank_of = [&](int r, double x) { return (had[r] + (x - lse[r])) * scale[r]; };
+  // the best rank of a quarter, of its maximum; an ended row's one continuation is its first quarter's
+  const auto top = [&](int e, double x) -> double {
+    const int r = e / parts;
+    if (had[r] == -INFINITY) return -INFINITY;
+    if (isnan(lse[r])) return e - r * parts ? -INFINITY : had[r] * scale[r];
+    return rank_of(r, x);
   };
-  // the first of what comes after `last`, of all the block's threads
-  const auto next = [&](Cont best) {
-    wave_first(best);
-    if (lane == 0) part[wave] = best;
-    __syncthreads();
-    best = part[0];
-    for (int k = 1; k < 4; ++k)
-      if (before(part[k], best)) best = part[k];
-    __syncthreads();
-    return best;
-  };
-  int n = 0;  // pieces chosen
-  for (; n < K; ++n) {
-    Cont best = none;
-    for (int e = tid; e < R * pieces; e += 256) {
-      const Cont c = entry(e);
-      if (c.rank > -INFINITY && before(c, best) && (!n || before(chosen[n - 1], c))) best = c;
+  const auto look = [&](int e) { return top(e, w.m[row0 * parts + e]); };
+#pragma unroll
+  for (int k = 0; k < BS_HELD; ++k) held[k] = tid + 1024 * k < E ? top(tid + 1024 * k, held[k]) : -INFINITY;
+  // this thread's quarters and their best ranks above -inf
+  const auto tops = [&](auto&& f) {
+#pragma unroll
+    for (int k = 0; k < BS_HELD; ++k)
+      if (held[k] > -INFINITY) f(tid + 1024 * k, held[k]);
+    for (int e = tid + 1024 * BS_HELD; e < E; e += 1024) {
+      const double t = look(e);
+      if (t > -INFINITY) f(e, t);
     }
-    best = next(best);
-    if (best.rank == -INFINITY) break;
-    if (tid == 0) chosen[n] = best;
+  };
+  // smallest, largest (as floats, outwards) and number of the block's ranks above -inf
+  const auto extent = [&](double& lo, double& hi, int& n) {
+    float l = wave_maxf(-__double2float_rd(lo)), h = wave_maxf(__double2float_ru(hi));
+    int a, b;
+    pair16_i32(row16_sumi(n), a, b);
+    pair32_i32(a + b, a, b);
     __syncthreads();
+    if (lane == 0) lows[wave] = l, highs[wave] = h, sums[wave] = a + b;
+    __syncthreads();
+    lo = -(double)row16_maxf(lows[lane & 15]);
+    hi = row16_maxf(highs[lane & 15]);
+    n = row16_sumi(sums[lane & 15]);
+  };
+  // the highest bin that K ranks reach, once they are counted in `bins`: every wave
+  // on its own, a lane four bins from the highest down
+  const auto bound = [&]() {
+    __syncthreads();
+    const int4 q = ((const int4*)bins)[BB_BINS / 4 - 1 - lane];
+    const int own = q.x + q.y + q.z + q.w;
+    int upto = own;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    const int from = __ffsll((unsigned long long)__ballot(upto >= K)) - 1;  // K ranks are counted
+    int level = BB_BINS - 4 - 4 * lane, above = upto - own + q.w;
+    if (above >= K) level += 3;
+    else if ((above += q.z) >= K) level += 2;
+    else if (above + q.y >= K) level += 1;
+    level = __shfl(level, from);
+    __syncthreads();  // before anybody counts anew
+    return level;
+  };
+  double lo = INFINITY, hi = -INFINITY;
+  int n = 0;
+  tops([&](int, double t) { lo = fmin(lo, t), hi = fmax(hi, t), ++n; });
+  if (tid < BB_BINS) bins[tid] = 0;
+  extent(lo, hi, n);
+  RankBins in(lo, hi);
+  int least = -1;  // continuations of this bin and above are listed; those below every maximum are in bin -1 or 0
+  if (n > K) {
+    tops([&](int, double t) { atomicAdd(&bins[in.of(t)], 1); });
+    least = bound();
   }
-  const Cont bound = n == K ? chosen[K - 1] : none;
-  // the continuations of a chosen piece, this thread's
-  const auto each = [&](int k, auto&& f) {
-    const Cont p = chosen[k];
-    if (p.t < 0) {
-      if (tid == 0) f(p);
-      return;
-    }
-    const int t0 = p.t / BS_PIECE * BS_PIECE;
-    for (int t = t0 + tid; t < min(t0 + BS_PIECE, b.V); t += 256) {
-      const Cont c = cont(p.row, b.x[(row0 + p.row) * b.V + t], t);
-      if (c.rank > -INFINITY) f(c);
+  tops([&](int e, double t) {
+    if (in.of(t) < least) return;
+    const int at = atomicAdd(&nparts, 1);
+    if (at < BS_PARTS) plist[at] = e;
+  });
+  __syncthreads();
+  const bool all_parts = nparts > BS_PARTS;
+  const int np = all_parts ? E : nparts;
+  // every continuation of the listed quarters that reaches the bound
+  const auto visit = [&](auto&& f) {
+    for (int p = tid >> 4; p < np; p += 4 * BS_WAVES) {
+      const int e = all_parts ? p : plist[p], r = e / parts, t0 = (e - r * parts) * 32 * PER;
+      if (all_parts && !(look(e) > -INFINITY)) continue;
+      if (isnan(lse[r])) {
+        const Cont c = {had[r] * scale[r], 0.0, r, -1};
+        if ((lane & 15) == 0 && in.of(c.rank) >= least) f(c);
+        continue;
+      }
+      v2logit v[PER];
+      beam_load(b.x + (row0 + r) * b.V, b.V, t0, v);
+      beam_cut(b.V, t0, v);
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const double x = h ? v[k].y : v[k].x;
+          const Cont c = {rank_of(r, x), x, r, beam_token(t0, k) + h};
+          if (c.rank > -INFINITY && in.of(c.rank) >= least) f(c);
+        }
     }
   };
-  for (int k = 0; k < n; ++k)
-    each(k, [&](const Cont& c) {
-      if (before(bound, c)) return;
-      const int at = atomicAdd(&listed, 1);
-      if (at < BS_LIST) list[at] = c;
-    });
-  __syncthreads();
   const auto put = [&](int j, const Cont& c) {
     const long at = (long)g * K + j;
     const bool there = c.rank > -INFINITY;
     b.parents[at] = there ? (uint32_t)(row0 + c.row) : NO_ROW;
     b.tokens[at] = there && c.t >= 0 ? (uint32_t)c.t : NO_TOKEN;
-    b.best[at] = !there ? -INFINITY : c.t < 0 ? b.scores[row0 + c.row] : b.scores[row0 + c.row] + (c.x - lse[c.row]);
+    b.best[at] = !there ? -INFINITY : c.t < 0 ? had[c.row] : had[c.row] + (c.x - lse[c.row]);
   };
-  if (listed <= BS_LIST) {
-    for (int i = tid; i < listed; i += 256) {
+  for (int round = 0;; ++round) {
+    if (tid == 0) listed = 0;
+    __syncthreads();
+    visit([&](const Cont& c) {
+      const int at = atomicAdd(&listed, 1);
+      if (at < BS_LIST) list[at] = c;
+    });
+    __syncthreads();
+    if (listed <= BS_LIST || round == 4) break;
+    // a closer bound among what reached this one
+    lo = INFINITY, hi = -INFINITY, n = 0;
+    visit([&](const Cont& c) { lo = fmin(lo, c.rank), hi = fmax(hi, c.rank), ++n; });
+    extent(lo, hi, n);
+    if (!(lo < hi)) break;
+    const RankBins closer(lo, hi);
+    if (tid < BB_BINS) bins[tid] = 0;
+    __syncthreads();
+    visit([&](const Cont& c) { atomicAdd(&bins[closer.of(c.rank)], 1); });
+    least = bound();
+    in = closer;
+  }
+  if (listed <= BS_LIST) {  // a wave to a continuation, a lane to another it is compared with
+    const int m = listed;
+    for (int i = wave; i < m; i += BS_WAVES) {
       const Cont c = list[i];
       int at = 0;
-      for (int j = 0; j < listed; ++j) at += before(list[j], c);
-      if (at < K) put(at, c);
+      for (int j0 = 0; j0 < m; j0 += 64) {
+        const Cont o = list[min(j0 + lane, m - 1)];
+        at += __popcll(__ballot(j0 + lane < m && before(o, c)));
+      }
+      if (at < K && lane == 0) put(at, c);
     }
-    for (int j = listed + tid; j < K; j += 256) put(j, none);
+    if (tid >= m && tid < K) put(tid, none);
     return;
   }
   Cont last = none;
   for (int j = 0; j < K; ++j) {
     Cont best = none;
-    for (int k = 0; k < n; ++k)
-      each(k, [&](const Cont& c) {
-        if (before(c, best) && (!j || before(last, c))) best = c;
-      });
-    last = next(best);
+    visit([&](const Cont& c) {
+      if (before(c, best) && (!j || before(last, c))) best = c;
+    });
+    wave_first(best);
+    __syncthreads();
+    if (lane == 0) part[wave] = best;
+    __syncthreads();
+    last = part[0];
+    for (int k = 1; k < BS_WAVES; ++k)
+      if (before(part[k], last)) last = part[k];
     if (tid == 0) put(j, last);
-    if (last.rank == -INFINITY) {
-      for (int i = j + 1 + tid; i < K; i += 256) put(i, none);
-      return;
-    }
   }
 }
 
 void beam_select(hipStream_t st, const BeamSelect& b) {
   BeamWs w;
   beam_layout(b, (char*)b.ws, w);
-  const int pieces = beam_pieces(b.V);
-  const long waves = (long)b.groups * b.beams * pieces;
-  hipLaunchKernelGGL(k_beam_pieces, dim3((unsigned)std::min<long>((waves + 3) / 4, 65536)), dim3(256), 0, st, b, w, pieces, waves);
-  hipLaunchKernelGGL(k_beam_pick, dim3(b.groups), dim3(256), 0, st, b, w, pieces);
+  const int piece = beam_piece(b), pieces = (b.V + piece - 1) / piece;
+  const uint32_t blocks = (uint32_t)(pieces + 3) / 4;
+  const dim3 grid((unsigned)(b.groups * b.beams) * blocks);  // below 2^24 threads for every GB of logits
+  if (piece == 512) {
+    hipLaunchKernelGGL(k_beam_pieces<4>, grid, dim3(256), 0, st, b, w, pieces, blocks);
+    hipLaunchKernelGGL(k_beam_pick<4>, dim3(b.groups), dim3(1024), 0, st, b, w, pieces);
+  } else {
+    hipLaunchKernelGGL(k_beam_pieces<2>, grid, dim3(256), 0, st, b, w, pieces, blocks);
+    hipLaunchKernelGGL(k_beam_pick<2>, dim3(b.groups), dim3(1024), 0, st, b, w, pieces);
+  }
 }
 
 __global__ __launch_bounds__(256) void k_beam_advance(BeamAdvance a) {
