@@ -26,6 +26,10 @@ struct AttnRun {
   // and double MFMAs take turns on a SIMD: 4 cycles an operation beside 64).
   // Each query goes by its own scores, so its bits do not depend on the others'.
   __device__ __forceinline__ void soften(v4d& s) {
+    rescale(s);
+    weigh(s);
+  }
+  __device__ __forceinline__ void rescale(const v4d& s) {
     const double top = fmax(fmax(s[0], s[1]), fmax(s[2], s[3]));
     if (__ballot(top > m + 8.0)) {
       double x, y;
@@ -38,6 +42,8 @@ struct AttnRun {
 #pragma unroll
       for (int c = 0; c < CT; ++c) o_re[c] *= keep, o_im[c] *= keep;
     }
+  }
+  __device__ __forceinline__ void weigh(v4d& s) {
     const double base = m == -INFINITY ? 0.0 : m;  // nothing seen yet: every weight e^-inf = 0
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

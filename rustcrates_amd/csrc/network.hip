@@ -4597,7 +4597,7 @@ static int paged_attention_impl(mitok_network* n, const double* d_q, const doubl
   a.err = n->page_err;
   std::vector<int> lists;
   PagedPlan plan = paged_plan(a, kv.data(), cnt.data(), lists);
-  if ((uint64_t)plan.entries * heads > 1u << 23) return fail(ERR_ARG, "%s: more than 2^23 blocks of work", what);
+  if ((uint64_t)plan.blocks * heads > 1u << 23) return fail(ERR_ARG, "%s: more than 2^23 blocks of work", what);
   TRY(behind_default_stream(n));
   TRY(alloc(n, n->op_ws, paged_ws_bytes(a, plan)));
   a.ws = n->op_ws.p;
@@ -4617,8 +4617,7 @@ static int paged_attention_impl(mitok_network* n, const double* d_q, const doubl
   TRY(op_hand_over(n, bytes, own, &a.tab));
   a.kv_len = 0;
   a.count = (uint32_t)(B * sizeof(int));
-  plan.chunks += (uint32_t)lists_at;
-  plan.splits += (uint32_t)lists_at;
+  for (uint32_t* at : {&plan.pieces, &plan.places, &plan.ranges, &plan.cuts}) *at += (uint32_t)lists_at;
   paged_attention(n->stream, a, plan, own);
   return op_finish(n);
 }
@@ -4915,9 +4914,9 @@ static int beam_search_impl(Net* n, const uint32_t* prompt, const uint32_t* lens
   step.a.count = ones_at;
   for (const auto& plans : windows)
     for (size_t k = 0; k < layers.size(); ++k)
-      if ((uint64_t)plans[k].entries * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
+      if ((uint64_t)plans[k].blocks * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
   for (size_t k = 0; k < layers.size(); ++k)
-    if ((uint64_t)first.plans[k].entries * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
+    if ((uint64_t)first.plans[k].blocks * layers[k]->heads > 1u << 23) return fail(ERR_ARG, "beam search: more than 2^23 blocks of work");
 
   ForkPages f;
   f.max_pages = r.P;

@@ -55,20 +55,23 @@ struct PagedAttn {
   uint32_t call = 0;
   uint32_t* err = nullptr;  // PageErrWord
 };
-// How a call's work is cut up, from its lengths: groups of 16 ng new rows, their
-// slots in chunks, the longest first.  The lists are appended to `lists`;
-// chunks and splits are their byte offsets, once the lists' own place is known.
-// A plan also serves shorter sequences of up to 32 rows each: a chunk ends where
-// the sequence does.
+// How a call's work is cut up, from its lengths: groups of `rows` new rows, and
+// ranges of pieces of them, a block each (for every head).  The lists are appended
+// to `lists`; pieces, ranges and cuts are their byte offsets, once the lists' own
+// place is known.  A plan also serves shorter sequences of up to 32 rows each: a
+// piece ends where the sequence does.
 struct PagedPlan {
-  int ng = 1;       // groups of 16 rows per block
-  int groups = 1;   // of a sequence
-  int entries = 0;
-  int nsplit = 1;   // the most chunks of one group
-  uint32_t chunks = 0;  // int4 [entries]: sequence, first slot, end, group * 64 + chunk * 2 + (one of several)
-  uint32_t splits = 0;  // int [B][groups]
+  bool beams = false;   // a piece is a bunch of sequences of one row: the first one, how many
+  int ng = 1;           // groups of 16 rows that a block's waves have of their own
+  int rows = 16;        // 16 ng
+  int groups = 1;       // of a sequence
+  int blocks = 0;       // of a head
+  int part_rows = 0;    // rows of the pieces of groups that were cut
+  uint32_t pieces = 0;  // int4 each: sequence, first row, first slot, end
+  uint32_t places = 0;  // int each: place of its rows among the partials, or -1
+  uint32_t ranges = 0;  // int [blocks + 1] (ng 4): a block's pieces
+  uint32_t cuts = 0;    // int2 [B][groups] (part_rows > 0): place of the first piece's rows, pieces
 };
-constexpr int PAGED_MAX_SPLIT = 32;
 PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, std::vector<int>& lists);
 size_t paged_ws_bytes(const PagedAttn& a, const PagedPlan& p);
 void paged_attention(hipStream_t st, const PagedAttn& a, const PagedPlan& p, const OpTable& own);

@@ -209,6 +209,72 @@ def test_more_sequences_than_the_arguments_hold(net):
     check(net, make(17, lens[:120], 18, 1, 16, 16))
 
 
+def beams(seed, G, K, L, H, dh, ps, shared, bias="decode"):
+    """G prompts of K sequences of one row each: sequence k of a prompt holds the prompt's first shared[k] pages."""
+    c = make(seed, np.repeat(L, K) if np.ndim(L) else [L] * (G * K), 1, H, dh, ps, bias=bias)
+    for b in range(G * K):
+        j = min(shared[b % K], int(c["lens"][b]) // ps)
+        c["table"][b, :j] = c["table"][b - b % K, :j]
+    return c
+
+
+@pytest.mark.parametrize("L", [0, 5, 15, 16, 17, 47, 48, 100, 128])
+def test_beams_of_many_prompts(net, L):
+    """Bunches of sequences of equal length, which share all, some or none of their pages."""
+    check(net, beams(L, 20, 4, L, 16, 16, 16, [9, 9, 9, 9]))
+    check(net, beams(L + 1, 20, 4, L, 16, 16, 16, [9, 1, 2, 0]))
+
+
+@pytest.mark.parametrize("dh", [3, 16, 24, 32, 40, 64])
+@pytest.mark.parametrize("K", [2, 3, 7, 16, 20])
+def test_beams_of_every_width(net, dh, K):
+    r = np.random.default_rng(K)
+    G = -(-70 // K)
+    check(net, beams(K, G, K, r.integers(0, 90, G), 8 * 4, dh, 16, r.integers(0, 6, K), bias="rows" if dh == 24 else "decode"))
+
+
+def test_equal_lengths_that_share_nothing(net):
+    check(net, make(30, [77] * 96, 1, 8, 16, 32))
+    c = beams(31, 24, 4, 130, 8, 16, 80, [1, 1, 1, 1])  # pages of five tiles
+    check(net, c)
+
+
+def test_what_a_beam_does_not_see_has_no_part_in_it(net):
+    """Values that are not finite in one beam's own rows leave the others' alone, those
+    of shared rows reach all that see them, and what lies behind a row reaches none."""
+    c = beams(32, 24, 4, 43, 16, 16, 16, [2, 2, 2, 2])
+    plain, _, _ = call(net, c)
+    for pool in (c["k"], c["v"]):
+        for b in range(96):
+            pool[c["table"][b, 2], :, 43 % 16:] = np.nan  # where the new row goes and behind it
+    out = check(net, c)
+    assert np.array_equal(out, plain)
+    c["v"][c["table"][5, 2], :, 3] = np.inf  # beam 1 of prompt 1
+    c["k"][c["table"][10, 2], :, 0] = np.nan  # beam 2 of prompt 2
+    c["v"][c["table"][12, 1], 3, 7, 2] = -np.inf  # a shared row of prompt 3
+    c["vn"][17] = np.nan
+    out = check(net, c)
+    touched = [5, 10, 12, 13, 14, 15, 17]
+    rest = np.setdiff1d(np.arange(96), touched)
+    assert np.array_equal(out[rest], plain[rest])
+
+
+def test_pages_of_beams_that_are_none_are_refused(net):
+    c = beams(33, 24, 4, 43, 16, 16, 16, [2, 2, 2, 2])
+    good = c["table"].copy()
+    for at in ((3, 2), (4, 1)):
+        c["table"] = good.copy()
+        c["table"][at] = c["pages"]
+        with pytest.raises(ra.MitokError, match="outside the pool"):
+            call(net, c)
+    c["table"] = good.copy()
+    c["table"][1, 2] = c["table"][0, 2]
+    with pytest.raises(ra.MitokError, match="one page"):
+        call(net, c)
+    c["table"] = good
+    check(net, c)
+
+
 def part(buf, nbytes, offset):
     """`nbytes` of a buffer at `offset`, as a buffer that does not own them"""
     x = ra.DeviceBuffer.__new__(ra.DeviceBuffer)
