@@ -43,48 +43,53 @@ size_t fork_ws_bytes(uint32_t n, uint32_t max_pages, uint32_t pages) {
   return fork_layout(n, max_pages, pages, nullptr, w);
 }
 
-// One block per new sequence: its parent's rows and pages, and what it does to
-// the counts of those.  A sequence that is refused holds nothing.
+// A new sequence's parent, its rows and its room; one that is refused holds nothing.
+struct ForkOne {
+  uint32_t p, len = 0, room = 0;
+  __device__ __forceinline__ ForkOne(const ForkPages& f, uint32_t i) {
+    p = f.parents ? f.parents[i] : i;
+    if (p == NO_ROW) return;
+    if (p >= f.old) {
+      refuse(f, PE_BAD_PARENT);
+      return;
+    }
+    len = f.lens[p];
+    room = f.grow ? f.grow[i] : f.grow_all;
+    if ((uint64_t)len + room > (uint64_t)f.max_pages * f.page_rows) refuse(f, PE_BAD_LENGTH);
+  }
+  __device__ __forceinline__ void refuse(const ForkPages& f, int word) {
+    len = room = 0;
+    set_word(f.err, word);
+    *f.refused = f.call;  // the same value, whoever writes it
+  }
+};
+// its page j, and what that does to the page's counts
+__device__ __forceinline__ void fork_hold(const ForkPages& f, const ForkWs& w, uint32_t i, uint32_t p, uint32_t j, uint32_t had,
+                                          bool writes) {
+  const uint32_t id = f.table[(size_t)p * f.max_pages + j];
+  w.table[(size_t)i * f.max_pages + j] = id;
+  if (id >= f.pages) {
+    set_word(f.err, PE_BAD_PAGE);
+    *f.refused = f.call;
+    return;
+  }
+  atomicAdd(f.held + id, 1u);
+  if (writes && j + 1 == had) {
+    atomicAdd(f.held + f.pages + id, 1u);
+    atomicMax(f.held + 2 * (size_t)f.pages + id, f.n - i);
+  }
+}
+
+// One block per new sequence.
 __global__ __launch_bounds__(256) void k_fork_take(ForkPages f, ForkWs w) {
   const uint32_t i = blockIdx.x, tid = threadIdx.x;
-  const uint32_t p = f.parents ? f.parents[i] : i;
-  uint32_t len = 0, room = 0;
-  bool bad = false;
-  if (p != NO_ROW) {
-    if (p >= f.old) {
-      bad = true;
-      if (tid == 0) set_word(f.err, PE_BAD_PARENT);
-    } else {
-      len = f.lens[p];
-      room = f.grow ? f.grow[i] : f.grow_all;
-      if ((uint64_t)len + room > (uint64_t)f.max_pages * f.page_rows) {
-        bad = true;
-        len = room = 0;
-        if (tid == 0) set_word(f.err, PE_BAD_LENGTH);
-      }
-    }
-  }
-  const uint32_t had = (len + f.page_rows - 1) / f.page_rows;
-  const bool writes = room > 0 && len % f.page_rows;
-  for (uint32_t j = tid; j < had; j += 256) {
-    const uint32_t id = f.table[(size_t)p * f.max_pages + j];
-    w.table[(size_t)i * f.max_pages + j] = id;
-    if (id >= f.pages) {
-      bad = true;
-      set_word(f.err, PE_BAD_PAGE);
-      continue;
-    }
-    atomicAdd(f.held + id, 1u);
-    if (writes && j + 1 == had) {
-      atomicAdd(f.held + f.pages + id, 1u);
-      atomicMax(f.held + 2 * (size_t)f.pages + id, f.n - i);
-    }
-  }
+  const ForkOne x(f, i);
+  const uint32_t had = (x.len + f.page_rows - 1) / f.page_rows;
+  for (uint32_t j = tid; j < had; j += 256) fork_hold(f, w, i, x.p, j, had, x.room > 0 && x.len % f.page_rows);
   if (tid == 0) {
-    w.len[i] = len;
-    w.room[i] = room;
+    w.len[i] = x.len;
+    w.room[i] = x.room;
   }
-  if (bad) *f.refused = f.call;  // the same value, whoever writes it
 }
 
 // what comes before this thread's number in the block's order, and the block's sum
@@ -109,9 +114,28 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t* part, uin
 
 // One block: which last pages are copied, where each sequence's share of the free
 // pages starts, and the list of these.  Leaves the counts at zero.
+// SMALL: what k_fork_take does, too.
+constexpr uint32_t FORK_SMALL = 1024;  // table entries, one of a thread
+template <bool SMALL>
 __global__ __launch_bounds__(1024) void k_fork_assign(ForkPages f, ForkWs w) {
   __shared__ uint32_t part[16];
   const uint32_t tid = threadIdx.x;
+  if constexpr (SMALL) {
+    __shared__ uint32_t from[1024], lens[1024], rooms[1024];
+    if (tid < f.n) {
+      const ForkOne x(f, tid);
+      from[tid] = x.p;
+      w.len[tid] = lens[tid] = x.len;
+      w.room[tid] = rooms[tid] = x.room;
+    }
+    __syncthreads();
+    for (uint32_t x = tid; x < f.n * f.max_pages; x += 1024) {
+      const uint32_t i = x / f.max_pages, j = x - i * f.max_pages, had = (lens[i] + f.page_rows - 1) / f.page_rows;
+      if (j < had) fork_hold(f, w, i, from[i], j, had, rooms[i] > 0 && lens[i] % f.page_rows);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the counts are there before any wave reads them
+    __syncthreads();
+  }
   uint32_t total = 0, all;
   for (uint32_t i0 = 0; i0 < f.n; i0 += 1024) {
     const uint32_t i = i0 + tid;
@@ -123,7 +147,7 @@ __global__ __launch_bounds__(1024) void k_fork_assign(ForkPages f, ForkWs w) {
       if (room > 0 && len % f.page_rows) {
         const uint32_t id = w.table[(size_t)i * f.max_pages + had - 1];
         if (id < f.pages) {
-          const bool all_write = f.held[f.pages + id] == f.held[id], first = f.held[2 * (size_t)f.pages + id] == f.n - i;
+          const bool all_write = ld_dev(f.held + f.pages + id) == ld_dev(f.held + id), first = ld_dev(f.held + 2 * (size_t)f.pages + id) == f.n - i;
           copy = !(all_write && first);
         }
       }
@@ -138,7 +162,7 @@ __global__ __launch_bounds__(1024) void k_fork_assign(ForkPages f, ForkWs w) {
   uint32_t found = 0;
   for (uint32_t p0 = 0; p0 < f.pages; p0 += 1024) {
     const uint32_t id = p0 + tid;
-    const bool is_free = id < f.pages && f.held[id] == 0;
+    const bool is_free = id < f.pages && ld_dev(f.held + id) == 0;
     if (id < f.pages) f.held[id] = f.held[f.pages + id] = f.held[2 * (size_t)f.pages + id] = 0;
     if (found < total) {
       const uint32_t at = found + block_before(is_free ? 1u : 0u, part, all);
@@ -153,7 +177,9 @@ __global__ __launch_bounds__(1024) void k_fork_assign(ForkPages f, ForkWs w) {
 }
 
 // y 0: the new tables and lengths; others, of one layer's keys or values: the
-// used rows of a copied page, head by head (a head's rows are contiguous).
+// used rows of a copied page, head by head (a head's rows are contiguous).  Bound by
+// HBM: 12 layers of 12 heads of 64 and pages of 32 rows, 64 sequences, 42 us at about 6
+// TB/s, read and written.
 constexpr int FC_PER = 4;
 __global__ __launch_bounds__(256) void k_fork_commit(ForkPages f, ForkWs w, PagePool pool, int parts, int commit) {
   if (*f.refused == f.call) return;
@@ -193,8 +219,13 @@ static ForkWs fork_ws(const ForkPages& f) {
 
 void fork_plan(hipStream_t st, const ForkPages& f) {
   const ForkWs w = fork_ws(f);
+  // us a call, one block / two launches: 4 sequences with 32 entries each 22.9 / 24.4, 128 37.3 / 36.0
+  if ((uint64_t)f.n * f.max_pages <= FORK_SMALL) {
+    hipLaunchKernelGGL(k_fork_assign<true>, dim3(1), dim3(1024), 0, st, f, w);
+    return;
+  }
   hipLaunchKernelGGL(k_fork_take, dim3(f.n), dim3(256), 0, st, f, w);
-  hipLaunchKernelGGL(k_fork_assign, dim3(1), dim3(1024), 0, st, f, w);
+  hipLaunchKernelGGL(k_fork_assign<false>, dim3(1), dim3(1024), 0, st, f, w);
 }
 
 void fork_copy(hipStream_t st, const ForkPages& f, const PagePool& pool, bool commit) {
@@ -292,6 +323,9 @@ __device__ __forceinline__ double exp_below(double x) {
   return ldexp(p, (int)k);
 }
 
+// Bound by the bytes and, beside them, by 20 double operations a logit: 192 rows of
+// 50280, 67 MB of live rows in 16.8 us (4 TB/s), where a read with the maxima alone
+// takes 12.  Waves that walk several pieces, the next one's loads in flight, took 22.
 template <int PER>
 __global__ __launch_bounds__(256) void k_beam_pieces(BeamSelect b, BeamWs w, int pieces, uint32_t blocks) {
   const int lane = threadIdx.x & 63;
@@ -387,7 +421,9 @@ __device__ __forceinline__ float wave_maxf(float v) {
 // place is how many of the list come before it.  Where the list is too long (few
 // quarters, or logits close together), a histogram of what reached the bound gives
 // a closer one; where that cannot part them (equal ranks), K rounds over the
-// quarters find one continuation each.
+// quarters find one continuation each.  Bound by that chain's latency, a memory round
+// trip or a few barriers a link: 7.4 us for 4 rows of 4096, 12 for 12 rows of 50280 and
+// 24 kept (K rounds of a block-wide maximum took 120).
 constexpr int BS_LIST = 512, BS_PARTS = 4096, BS_WAVES = 16;
 constexpr int BS_HELD = 5;  // of a thread's quarters, maxima that wait in registers (5120: 12 rows of 50280 logits)
 template <int PER>
@@ -600,7 +636,7 @@ void beam_select(hipStream_t st, const BeamSelect& b) {
   beam_layout(b, (char*)b.ws, w);
   const int piece = beam_piece(b), pieces = (b.V + piece - 1) / piece;
   const uint32_t blocks = (uint32_t)(pieces + 3) / 4;
-  const dim3 grid((unsigned)(b.groups * b.beams) * blocks);  // below 2^24 threads for every GB of logits
+  const dim3 grid((unsigned)(b.groups * b.beams) * blocks);  // the caller sees to fewer than 2^24
   if (piece == 512) {
     hipLaunchKernelGGL(k_beam_pieces<4>, grid, dim3(256), 0, st, b, w, pieces, blocks);
     hipLaunchKernelGGL(k_beam_pick<4>, dim3(b.groups), dim3(1024), 0, st, b, w, pieces);

@@ -4711,8 +4711,9 @@ int mitok_fork_pages_device(mitok_network* n, double* d_k_pages, double* d_v_pag
 static int check_beams(uint32_t groups, uint32_t beams, uint32_t V, uint32_t keep) {
   if (!groups || !beams || !V) return fail(ERR_ARG, "beam selection: bad shape");
   if (!keep || keep > (uint32_t)BEAM_MAX_KEEP) return fail(ERR_ARG, "beam selection: %u kept, 1 to %d", keep, BEAM_MAX_KEEP);
-  if (beams > BEAM_MAX || (uint64_t)beams * V > 1u << 30 || (uint64_t)groups * beams > 1u << 23)
-    return fail(ERR_ARG, "beam selection: at most %u beams, 2^30 logits of a group and 2^23 rows", BEAM_MAX);
+  if (beams > BEAM_MAX || (uint64_t)beams * V > 1u << 30 || (uint64_t)groups * beams > 1u << 23 ||
+      (uint64_t)groups * beams * ((V + 1023ull) / 1024) > 1u << 23)
+    return fail(ERR_ARG, "beam selection: at most %u beams, 2^30 logits of a group, 2^23 rows and as many pieces of 1024 logits", BEAM_MAX);
   return OK;
 }
 

@@ -107,7 +107,7 @@ fork()
 fork(grow=None)
 fork(old=3, table_out=a["table"], lens_out=a["lens"])
 fork(parents=a["grow"])
-assert launches("k_fork_take") == launches("k_fork_assign") == launches("k_fork_commit") == 4
+assert launches("k_fork_assign") == launches("k_fork_commit") == 4
 """
 
 
@@ -131,7 +131,7 @@ bad("overlap", table_out=a["table"] + 16)
 bad("overlap", lens_out=a["lens"] + 4)
 bad("overlap", lens_out=a["table_out"])
 bad("overlap", v=a["k"])
-assert launches("k_fork_take") == 4
+assert launches("k_fork_assign") == 4
 """)
 
 
