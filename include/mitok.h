@@ -483,6 +483,7 @@ int mitok_fork_pages_device(mitok_network* net, double* d_k_pages, double* d_v_p
  * token, between rows of equal rank the lower row.  A row with done[r] != 0 has
  * one continuation, itself (score scores[r], no token); one of score -inf has
  * none, and a logit of -inf is none.  The logits of both kinds of row are not read.
+ * At most 2^30 logits of a group, 2^23 rows and 2^23 pieces of 1024 logits in all.
  *   d_logits [batch * beams][vocab], d_scores, d_scale [batch * beams] (scale NULL: 1;
  *     else finite and above 0), d_done [batch * beams] or NULL
  *   d_parents [batch][keep]: the row, counted over all groups, d_tokens,
@@ -504,6 +505,7 @@ int mitok_beam_select(mitok_network* net, const double* logits, const double* sc
  * tokens to the power length_power (0: by the score; within [-16, 16]).  The prompt
  * runs once and its rows are shared; one beam without an end gives
  * mitok_generate's ids.  Drops the caches, as mitok_generate does, and leaves none.
+ * At most 65535 hypotheses and 2^26 tokens of all of them.
  *   prompt [batch][seq], lens [batch] as for mitok_generate
  *   out_ids [batch][beams][n_new], the best hypothesis first, MITOK_NO_TOKEN behind its
  *     tokens; out_lens [batch][beams] tokens (the end among them);

@@ -5049,6 +5049,7 @@ int mitok_beam_search(mitok_network* n, const uint32_t* prompt, const uint32_t* 
   if (!n_new || n_new > OP_MAX_CTX) return fail(ERR_ARG, "beam search: %u new tokens", n_new);
   if (!beams || beams > (uint32_t)BEAM_MAX_KEEP) return fail(ERR_ARG, "beam search: %u beams, 1 to %d", beams, BEAM_MAX_KEEP);
   if ((uint64_t)B * beams > POOL_MAX_SEQS) return fail(ERR_ARG, "beam search: more than %u sequences", POOL_MAX_SEQS);
+  if ((uint64_t)B * beams * n_new > 1u << 26) return fail(ERR_ARG, "beam search: more than 2^26 tokens of all hypotheses");
   if (!(std::fabs(length_power) <= 16.0)) return fail(ERR_ARG, "beam search: length_power outside [-16, 16]");
   const int rc = guarded([&] {
     return beam_search_impl(n, prompt, lens, B, S, beams, n_new, end_id, length_power, out_ids, out_lens, out_scores);

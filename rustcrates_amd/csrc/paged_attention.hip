@@ -459,21 +459,23 @@ __device__ __forceinline__ void paged_tile(const PagedAttn& a, const PagedPlan& 
 // each one sequence's; the products' other columns get weight 0.  Which tiles are
 // shared is read off the tables, whatever the caller took them for: a run of
 // sequences holds in common the pages up to the first in which a neighbour differs.
-// 32 prompts of 4 beams, 200 to 248 slots of which 128 are shared, 8 heads: 72 us a
-// block per CU, the longest bunch's time; 512 blocks of single sequences' pieces and
-// more read 470 MB instead of 275 in 78 to 90 us.
+// 32 prompts of 4 beams, 200 to 248 slots of which 128 are shared, 8 heads: the 256
+// blocks take the longest bunch's time, and eight waves each, two a SIMD, 74 us a call
+// against 82 with four; 512 blocks of single sequences' pieces and more read 470 MB
+// instead of 275 and take longer than either.  More blocks than CUs stand two on a CU
+// with four waves: 64 prompts of 8 beams 217 us a call, 228 with eight waves.
 struct BeamRuns {  // in LDS
   int4 at[32];     // tiles [x, y) of all from tile z of sequence w & 15 for columns w >> 8
   int n;
 };
-template <int DHP, bool FULL>
-__global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p, OpTable own) {
+template <int DHP, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void k_paged_beams(PagedAttn a, PagedPlan p, OpTable own) {
   constexpr int U = DHP / 4, CT = DHP / 16, OSTR = DHP + 1;
-  __shared__ __align__(16) unsigned char lds[split_lds<DHP>(1)];
-  __shared__ PagedSums sh;
+  __shared__ __align__(16) unsigned char lds[std::max((size_t)U * 64, (size_t)WAVES * 16 * OSTR) * sizeof(double2)];
+  __shared__ double sm[WAVES][16], sl[WAVES][16], sums[16];
   __shared__ BeamRuns runs;
   __shared__ int same[16];  // pages in common with the sequence before
-  double2* qs = (double2*)lds;  // [U][64], then outputs [4][16][OSTR]
+  double2* qs = (double2*)lds;  // [U][64], then outputs [waves][16][OSTR]
   double2* os = (double2*)lds;
   const int bunch = blockIdx.x / a.H, h = blockIdx.x - bunch * a.H;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -481,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p
   const int4 mine = op_array<int4>(a.tab, own, p.pieces)[bunch];
   const int b0 = __builtin_amdgcn_readfirstlane(mine.x), m = __builtin_amdgcn_readfirstlane(mine.y);
   const int L = op_int(a.tab, own, a.kv_len, b0), tiles = L / PAGE_TILE + 1;
-  for (int k = wave; k < m; k += 4) {
+  for (int k = wave; k < m; k += WAVES) {
     PagedAt at(a, b0 + k, h, L, 1, 0, L + 1);
     if (lane == 0) same[k] = 0;
     if (k) {  // whole pages of rows that both have
@@ -504,7 +506,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p
     paged_store(a, at, 1);
   }
   // the queries, [sequence] where k_paged_split has [row]
-  for (int x = tid; x < U * 64; x += 256) {
+  for (int x = tid; x < U * 64; x += 64 * WAVES) {
     const int r = x & 15, e = 4 * (x >> 6) + (x & 63) / 16;
     double2 q = make_double2(0.0, 0.0);
     if (r < m && e < dh) q = a.q[(long)(b0 + r) * a.n * a.ldq + (long)h * dh + e];
@@ -584,10 +586,10 @@ __global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p
     now = place(v);
     load_keys(now);
     load_values(now);
-    ahead = place(min(v + 4, all - 1));
+    ahead = place(min(v + WAVES, all - 1));
   }
   const double2* qw = qs + lane;
-  for (; v < all; v += 4) {
+  for (; v < all; v += WAVES) {
     v4d s = {0.0, 0.0, 0.0, 0.0}, z = s;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -605,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p
       vis |= (unsigned)see << e;
       s[e] = see ? s[e] + z[e] + bf[e] : -INFINITY;
     }
-    const bool more = v + 4 < all;
+    const bool more = v + WAVES < all;
     if (more) load_keys(ahead);
     run.soften(s);
     bool fine = true;  // 0 times what is not finite is NaN in the other columns
@@ -621,32 +623,32 @@ __global__ __launch_bounds__(256, 2) void k_paged_beams(PagedAttn a, PagedPlan p
     if (more) load_values(ahead);
     if (__ballot(!fine)) run.add_left_out([&](int k) { return now.value(a, k, L); }, dh, L + 1 - t, s, vis);
     now = ahead;
-    if (more) ahead = place(min(v + 8, all - 1));
+    if (more) ahead = place(min(v + 2 * WAVES, all - 1));
   }
   // the waves, rescaled to their common maximum and added in order
   run.l = xor32_sum(xor16_sum(run.l));
-  if (kq == 0) sh.m[wave][row] = run.m, sh.l[wave][row] = run.l;
+  if (kq == 0) sm[wave][row] = run.m, sl[wave][row] = run.l;
   __syncthreads();  // and the queries' last read
   double M = -INFINITY, sum = 0.0;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) M = fmax(M, sh.m[g][row]);
+  for (int g = 0; g < WAVES; ++g) M = fmax(M, sm[g][row]);
   const double base = M == -INFINITY ? 0.0 : M, f = exp(run.m - base);
 #pragma unroll
-  for (int g = 0; g < 4; ++g) sum += sh.l[g][row] * exp(sh.m[g][row] - base);
+  for (int g = 0; g < WAVES; ++g) sum += sl[g][row] * exp(sm[g][row] - base);
   if (row < m)
 #pragma unroll
     for (int c = 0; c < CT; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         os[(wave * 16 + row) * OSTR + 16 * c + 4 * e + kq] = make_double2(run.o_re[c][e] * f, run.o_im[c][e] * f);
-  if (wave == 0 && kq == 0) sh.sum[row] = sum;
+  if (wave == 0 && kq == 0) sums[row] = sum;
   __syncthreads();
-  for (int x = tid; x < m * dh; x += 256) {
+  for (int x = tid; x < m * dh; x += 64 * WAVES) {
     const int r = x / dh, e = x - r * dh;
     double2 o = os[r * OSTR + e];
 #pragma unroll
-    for (int g = 1; g < 4; ++g) o = cadd(o, os[(g * 16 + r) * OSTR + e]);
-    a.out[(long)(b0 + r) * a.n * a.ldo + (long)h * dh + e] = make_double2(o.x / sh.sum[r], o.y / sh.sum[r]);
+    for (int g = 1; g < WAVES; ++g) o = cadd(o, os[(g * 16 + r) * OSTR + e]);
+    a.out[(long)(b0 + r) * a.n * a.ldo + (long)h * dh + e] = make_double2(o.x / sums[r], o.y / sums[r]);
   }
 }
 
@@ -725,8 +727,8 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan p, Pa
 // place of the chip is busy; 8 us go to a block's start and end, and the partials
 // pass through memory twice.  Other widths go by the same figures in proportion.
 // With more rows a block takes as many steps as any other, of as many groups as that
-// needs: 700 rows behind 512 to 1024 slots, 12 heads, take 280 us in blocks of 14
-// steps at most, 261 in 504 blocks of equal steps.
+// needs: 700 rows behind 512 to 1024 slots, 12 heads, take 280 us a call in
+// blocks of 14 steps at most, 252 in 504 blocks of equal steps.
 PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, std::vector<int>& lists) {
   PagedPlan p;
   p.ng = a.n <= 16 || a.dh > 128 ? 1 : a.n <= 32 ? 2 : 4;
@@ -749,7 +751,9 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
     }
   // One row of many sequences: neighbours of equal length may be beams that share
   // pages, which are then read once.  In bunches where that leaves a block for
-  // every CU; sequences that share nothing lose nothing by it there.
+  // three of four CUs: 16 prompts of 16 beams, 12 heads, take 324 us a call so in 192
+  // blocks, 375 in 384 of 11 and 5 sequences.  Sequences that share nothing lose nothing
+  // by it there (64 of 480 slots, 12 heads: 171 us, 173 in 264 blocks).
   if (a.n == 1 && a.dh <= 64 && std::all_of(count, count + a.B, [](int c) { return c == 1; }))
     for (int most = 16; most > 1 && !p.beams; --most) {
       std::vector<int4> bunches;
@@ -758,7 +762,7 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
         bunches.push_back(make_int4(b, end - b, 0, 0));
       }
       if (3 * bunches.size() > 2 * (size_t)a.B) break;
-      if (bunches.size() * a.H < 256) continue;
+      if (bunches.size() * a.H < 192) continue;
       std::stable_sort(bunches.begin(), bunches.end(),
                        [&](const int4& x, const int4& y) { return (long)x.y * kv_len[x.x] > (long)y.y * kv_len[y.x]; });
       p.beams = true;
@@ -884,7 +888,10 @@ static void launch_paged(hipStream_t st, const PagedAttn& a, const PagedPlan& p,
   const dim3 grid((unsigned)((long)p.blocks * a.H));
   const auto go = [&](auto kern) { MITOK_LAUNCH(kern, grid, dim3(256), 0, st, a, p, ws, own); };
   if constexpr (DHP <= 64)
-    if (p.beams) return (void)[&] { MITOK_LAUNCH((k_paged_beams<DHP, FULL>), grid, dim3(256), 0, st, a, p, own); }();
+    if (p.beams) {
+      const auto bunches = [&](auto kern, int waves) { MITOK_LAUNCH(kern, grid, dim3(64 * waves), 0, st, a, p, own); };
+      return grid.x <= 256 ? bunches(k_paged_beams<DHP, FULL, 8>, 8) : bunches(k_paged_beams<DHP, FULL, 4>, 4);
+    }
   if constexpr (DHP <= 128) {
     if (p.ng == 4) return go(k_paged_tile<DHP, FULL>);
     if (p.ng == 2) return go(k_paged_split<DHP, 2, FULL>);

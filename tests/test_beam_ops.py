@@ -202,6 +202,7 @@ refused(3, "Embedding", lambda: empty.beam_search(prompt))
 flat = ra.Network(0)
 flat.add_embedding(9, 4), flat.add_linear(4, 9), flat.add_softmax(1)
 refused(3, "no attention", lambda: flat.beam_search(prompt, n_new=2))
+refused(1, "all hypotheses", lambda: flat.beam_search([[3]] * 1000, beams=60, n_new=2000))
 """)
 
 

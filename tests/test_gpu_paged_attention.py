@@ -233,6 +233,15 @@ def test_beams_of_every_width(net, dh, K):
     check(net, beams(K, G, K, r.integers(0, 90, G), 8 * 4, dh, 16, r.integers(0, 6, K), bias="rows" if dh == 24 else "decode"))
 
 
+@pytest.mark.parametrize("K", [2, 4])
+@pytest.mark.parametrize("G", [24, 40])
+def test_beams_in_blocks_of_either_size(net, G, K):
+    """Prompts of their own lengths each, 10 heads: 240 blocks, one a CU, and 400."""
+    for dh in (16, 24, 64):
+        lens = np.random.default_rng(G + K + dh).permutation(np.arange(0, 6 * G, 6))
+        check(net, beams(G + K, G, K, lens, 10, dh, 16, [14, 3, 0, 9][:K]))
+
+
 def test_equal_lengths_that_share_nothing(net):
     check(net, make(30, [77] * 96, 1, 8, 16, 32))
     c = beams(31, 24, 4, 130, 8, 16, 80, [1, 1, 1, 1])  # pages of five tiles
