@@ -482,7 +482,9 @@ int mitok_fork_pages_device(mitok_network* net, double* d_k_pages, double* d_v_p
  * the best first; in a row the larger logit is first, of equal ones the lower
  * token, between rows of equal rank the lower row.  A row with done[r] != 0 has
  * one continuation, itself (score scores[r], no token); one of score -inf has
- * none, and a logit of -inf is none.  The logits of both kinds of row are not read.
+ * none, and a logit of -inf is none (nor is one whose score or rank passes the
+ * doubles to -inf; finite masks down to the lowest double are logits like others).
+ * The logits of both kinds of row are not read.
  * At most 2^30 logits of a group, 2^23 rows and 2^23 pieces of 1024 logits in all.
  *   d_logits [batch * beams][vocab], d_scores, d_scale [batch * beams] (scale NULL: 1;
  *     else finite and above 0), d_done [batch * beams] or NULL
