@@ -402,15 +402,16 @@ __device__ __forceinline__ int row16_sumi(int v) {
 // trip or a few barriers a link: 7.4 us for 4 rows of 4096, 12 for 12 rows of 50280 and
 // 24 kept (K rounds of a block-wide maximum took 120).
 constexpr int BS_LIST = 512, BS_PARTS = 4096, BS_WAVES = 16;
+constexpr int BS_GROUPS = 1 << 21;  // of a launch, which has fewer than 2^32 threads
 constexpr int BS_HELD = 5;  // of a thread's quarters, maxima that wait in registers (5120: 12 rows of 50280 logits)
 template <int PER>
-__global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect b, BeamWs w, int pieces) {
+__global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect b, BeamWs w, int pieces, int first) {
   __shared__ double lse[1024], had[1024], scale[1024];  // of the group's rows; lse NaN: ended
   __shared__ Cont part[BS_WAVES], list[BS_LIST];
   __shared__ int plist[BS_PARTS], bins[BB_BINS];
   __shared__ double lows[BS_WAVES], highs[BS_WAVES];
   __shared__ int sums[BS_WAVES], nparts, listed;
-  const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = b.beams, K = b.keep;
+  const int g = first + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = b.beams, K = b.keep;
   const int parts = 4 * pieces, E = R * parts;  // quarters of a row, of the group
   const long row0 = (long)g * R;
   // what the rows need, requested at once; an idle row's has no meaning and is left out
@@ -614,13 +615,13 @@ void beam_select(hipStream_t st, const BeamSelect& b) {
   const int piece = beam_piece(b), pieces = (b.V + piece - 1) / piece;
   const uint32_t blocks = (uint32_t)(pieces + 3) / 4;
   const dim3 grid((unsigned)(b.groups * b.beams) * blocks);  // the caller sees to fewer than 2^24
-  if (piece == 512) {
-    hipLaunchKernelGGL(k_beam_pieces<4>, grid, dim3(256), 0, st, b, w, pieces, blocks);
-    hipLaunchKernelGGL(k_beam_pick<4>, dim3(b.groups), dim3(1024), 0, st, b, w, pieces);
-  } else {
-    hipLaunchKernelGGL(k_beam_pieces<2>, grid, dim3(256), 0, st, b, w, pieces, blocks);
-    hipLaunchKernelGGL(k_beam_pick<2>, dim3(b.groups), dim3(1024), 0, st, b, w, pieces);
-  }
+  const auto run = [&](auto piece_kern, auto pick_kern) {
+    hipLaunchKernelGGL(piece_kern, grid, dim3(256), 0, st, b, w, pieces, blocks);
+    for (int g = 0; g < b.groups; g += BS_GROUPS)
+      hipLaunchKernelGGL(pick_kern, dim3(std::min(BS_GROUPS, b.groups - g)), dim3(1024), 0, st, b, w, pieces, g);
+  };
+  if (piece == 512) run(k_beam_pieces<4>, k_beam_pick<4>);
+  else run(k_beam_pieces<2>, k_beam_pick<2>);
 }
 
 __global__ __launch_bounds__(256) void k_beam_advance(BeamAdvance a) {
