@@ -433,9 +433,10 @@ struct mitok_network {
   mitok::DevBuf op_refused;  // the number of the last call whose logits in place stayed (LogitRules)
   uint32_t op_calls = 0;
   // forks of paged sequences: the pages' counts, zero between calls unless one
-  // failed, and the last call and sequence that stored to a page (PagedAttn)
+  // failed, and the last call and sequence that stored to a page (PagedAttn), no
+  // call's before the first unless the call that clears them failed
   mitok::DevBuf fork_held, page_stamp;
-  bool fork_dirty = false;
+  bool fork_dirty = false, stamp_dirty = false;
   mitok::DevBuf beam_state;  // of a beam search: tables, lengths, scores, history
   hipEvent_t op_event = nullptr;
   // the last stateless pass's vocab Linear input rows [head_B * head_S][d]
@@ -4604,8 +4605,9 @@ static int paged_attention_impl(mitok_network* n, const double* d_q, const doubl
   const size_t stamps = (size_t)pages * sizeof(unsigned long long);
   if (n->page_stamp.bytes < stamps) {
     TRY(alloc(n, n->page_stamp, stamps));
-    fill_u32(n->stream, n->page_stamp.as<uint32_t>(), n->page_stamp.bytes / 4, 0);
+    n->stamp_dirty = true;
   }
+  if (n->stamp_dirty) fill_u32(n->stream, n->page_stamp.as<uint32_t>(), n->page_stamp.bytes / 4, 0);
   a.stamp = n->page_stamp.as<unsigned long long>();
   a.call = next_call(n);
   const size_t lists_at = (2 * (size_t)B * sizeof(int) + 15) & ~(size_t)15, bytes = lists_at + lists.size() * sizeof(int);
@@ -4619,7 +4621,9 @@ static int paged_attention_impl(mitok_network* n, const double* d_q, const doubl
   a.count = (uint32_t)(B * sizeof(int));
   for (uint32_t* at : {&plan.pieces, &plan.places, &plan.ranges, &plan.cuts}) *at += (uint32_t)lists_at;
   paged_attention(n->stream, a, plan, own);
-  return op_finish(n);
+  const int rc = op_finish(n);
+  if (rc != ERR_HIP) n->stamp_dirty = false;
+  return rc;
 }
 
 int mitok_paged_attention_device(mitok_network* n, const double* d_q, const double* d_k_new, const double* d_v_new,
