@@ -737,7 +737,7 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
   const int unit = 64 / p.ng;  // slots of a step
   const bool even = p.ng == 4;
   struct Group {
-    int b, n0, len, steps;  // slots that its rows see (0 without rows)
+    int b, n0, len, steps;  // slots that its rows see (0 without rows), at most 2^26 steps
   };
   std::vector<Group> groups;
   long steps = 0;
@@ -798,8 +798,8 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
   // pieces of one group a block where that costs no more than the two steps that another piece does
   bool own_block = !even;
   if (even) {
-    int c = (int)((steps + ranges - 1) / ranges);
-    const int bar = c + 2;
+    long c = (steps + ranges - 1) / ranges;  // past 32 bits where many groups have long caches
+    const long bar = c + 2;
     const auto blocks = [&] {
       long n = 0;
       for (const Group& g : groups) n += (g.steps + c - 1) / c;
@@ -807,7 +807,7 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
     };
     while (c < bar && blocks() > ranges) ++c;
     own_block = blocks() <= ranges;
-    if (own_block) each = c;
+    if (own_block) each = (int)c;
     else each = INT32_MAX;
   }
   const auto cut = [&](auto&& piece) {
