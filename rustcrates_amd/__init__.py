@@ -803,17 +803,15 @@ class Network:
         (ids [B][beams][n_new], tokens [B][beams], scores [B][beams]), the best
         first; ids behind a hypothesis' tokens are NO_TOKEN.  end_id: the token
         that ends one (None: none does)."""
-        prompt = np.ascontiguousarray(prompt, dtype=np.uint32)
-        if prompt.ndim != 2:
-            raise ValueError(f"prompt: shape {prompt.shape}, expected (batch, seq)")
+        prompt = _u32_rows(prompt, "prompt")
         B, S = prompt.shape
-        lens = np.full(B, S, np.uint32) if lens is None else _u32_vec(lens, B, "lens")
+        lens = np.full(B, S, np.uint32) if lens is None else _u32_lens(lens, B, "lens")
+        end = NO_TOKEN if end_id is None else _u32(np.asarray(end_id), "end_id", -1).item()
         _check_sizes(beams | n_new)
         ids = np.empty((B, int(beams), int(n_new)), np.uint32)
         count, scores = np.empty(ids.shape[:2], np.uint32), np.empty(ids.shape[:2], np.float64)
         _check(self._lib.mitok_beam_search(self._h, _ptr(prompt), _ptr(lens), B, S, int(beams), int(n_new),
-                                           NO_TOKEN if end_id is None else int(end_id), float(length_power), _ptr(ids),
-                                           _ptr(count), _ptr(scores)))
+                                           end, float(length_power), _ptr(ids), _ptr(count), _ptr(scores)))
         return ids, count, scores
 
     # ---- measurement ----
