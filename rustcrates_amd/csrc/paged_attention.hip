@@ -752,8 +752,15 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
   // One row of many sequences: neighbours of equal length may be beams that share
   // pages, which are then read once.  In bunches where that leaves a block for
   // three of four CUs: 16 prompts of 16 beams, 12 heads, take 324 us a call so in 192
-  // blocks, 375 in 384 of 11 and 5 sequences.  Sequences that share nothing lose nothing
-  // by it there (64 of 480 slots, 12 heads: 171 us, 173 in 264 blocks).
+  // blocks, 375 in 384 of 11 and 5 sequences.  Sequences of one length that share nothing
+  // lose nothing by it there (64 of 480 slots, 12 heads: 171 us, 173 in 264 blocks).
+  // A bunch is one block however long it is, and what it shares is not known here: one
+  // that holds 1.9 times a CU's even share of all rows or more is cut into smaller ones,
+  // and where pairs are too long yet, no bunch is formed.  us a call, 12 heads, with
+  // 90% / 50% / none of the slots shared: 16 of 2000 slots beside 42 pairs of 100 to 141
+  // 172 / 194 / 234 so (pieces by slots), 173 / 253 / 335 in pairs (2.0 even shares), 423 /
+  // 1181 / 2108 in one bunch; 16 prompts of 16 beams, 100 to 500 slots (1.8), 138 / 313 /
+  // 521 whole, 172 / 351 / 571 in bunches of 13 and 3.
   if (a.n == 1 && a.dh <= 64 && std::all_of(count, count + a.B, [](int c) { return c == 1; }))
     for (int most = 16; most > 1 && !p.beams; --most) {
       std::vector<int4> bunches;
@@ -763,6 +770,13 @@ PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, st
       }
       if (3 * bunches.size() > 2 * (size_t)a.B) break;
       if (bunches.size() * a.H < 192) continue;
+      long longest = 0, all = 0;  // tiles
+      for (const int4& x : bunches) {
+        const long tiles = (long)x.y * (kv_len[x.x] / PAGE_TILE + 1);
+        longest = std::max(longest, tiles);
+        all += tiles;
+      }
+      if (longest * 256 > 1.9 * all * a.H) continue;
       std::stable_sort(bunches.begin(), bunches.end(),
                        [&](const int4& x, const int4& y) { return (long)x.y * kv_len[x.x] > (long)y.y * kv_len[y.x]; });
       p.beams = true;
