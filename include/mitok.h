@@ -428,8 +428,9 @@ int mitok_process_logits(mitok_network* net, const double* logits, uint32_t rows
  * common.  A cache of pages holds a sequence's slot t in row t % page_rows of page
  * table[sequence][t / page_rows]; a pool has [pages][heads][page_rows][head_dim]
  * complex keys, and as many values.  page_rows: a multiple of 16 up to 1024;
- * head_dim <= 256; pages <= 2^24; at most 65535 sequences, max_pages * page_rows <=
- * 2^30.  Streams, checks and completion are those of the operators above. */
+ * head_dim <= 256; pages <= 2^24, each of at most 2^30 complex keys; at most
+ * 65535 sequences, sequences * max_pages <= 2^28, max_pages * page_rows <= 2^30.
+ * Streams, checks and completion are those of the operators above. */
 
 /* Attention of a chunk of new tokens: sequence b holds kv_lens[b] rows, and its
  * counts[b] <= rows new ones (counts NULL: rows of each; rows <= 65536) are stored
@@ -445,6 +446,8 @@ int mitok_process_logits(mitok_network* net, const double* logits, uint32_t rows
  *   d_table [batch][max_pages]: entries of the slots in use, the new rows' too;
  *     entries behind them are not read
  *   d_bias [heads] of bias_stride apart, or NULL
+ * batch * heads <= 2^18, and at most 2^20 groups of 16 new rows (counted from `rows`)
+ * and 2^23 blocks of work, of up to 64 rows of a head each: MITOK_ERR_ARG.
  * An entry in use that is >= pages is MITOK_ERR_ARG, and so are two pages of a call
  * that store new rows to one page of the pool.  A page that is stored to may be
  * in no other sequence's use (mitok_fork_pages_device sees to that): the rows read
@@ -463,7 +466,7 @@ int mitok_paged_attention_device(mitok_network* net, const double* d_q, const do
  * holders where all of them grow from it.  Pages that no new sequence holds are
  * free; copies and room take them in ascending order, sequence by sequence, a
  * copy before the room.
- *   d_k_pages, d_v_pages: `layers` pools one behind the other, of one table
+ *   d_k_pages, d_v_pages: `layers` <= 16384 pools one behind the other, of one table
  *   d_table [sequences][max_pages], d_lens [sequences] rows
  *   d_table_out [new_sequences][max_pages]: MITOK_NO_PAGE behind a sequence's last
  *     page; d_lens_out [new_sequences]: its rows, without the room
@@ -507,7 +510,7 @@ int mitok_beam_select(mitok_network* net, const double* logits, const double* sc
  * tokens to the power length_power (0: by the score; within [-16, 16]).  The prompt
  * runs once and its rows are shared; one beam without an end gives
  * mitok_generate's ids.  Drops the caches, as mitok_generate does, and leaves none.
- * At most 65535 hypotheses and 2^26 tokens of all of them.
+ * At most 65535 hypotheses, hypotheses * heads <= 2^18, 2^26 tokens of all of them.
  *   prompt [batch][seq], lens [batch] as for mitok_generate
  *   out_ids [batch][beams][n_new], the best hypothesis first, MITOK_NO_TOKEN behind its
  *     tokens; out_lens [batch][beams] tokens (the end among them);

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(1024) void k_fork_assign(ForkPages f, ForkWs w) {
 
 // y 0: the new tables and lengths; others, of one layer's keys or values: the
 // used rows of a copied page, head by head (a head's rows are contiguous).  Bound by
-// HBM: 12 layers of 12 heads of 64 and pages of 32 rows, 64 sequences, 42 us at about 6
+// HBM: 12 layers of 12 heads of 64 and pages of 32 rows, 64 sequences, 41 us at about 6
 // TB/s, read and written.
 constexpr int FC_PER = 4;
 __global__ __launch_bounds__(256) void k_fork_commit(ForkPages f, ForkWs w, PagePool pool, int parts, int commit) {
@@ -325,7 +325,7 @@ __device__ __forceinline__ double exp_below(double x) {
 }
 
 // Bound by the bytes and, beside them, by 20 double operations a logit: 192 rows of
-// 50280, 67 MB of live rows in 16.8 us (4 TB/s), where a read with the maxima alone
+// 50280, 67 MB of live rows in 15.9 us (4.2 TB/s), where a read with the maxima alone
 // takes 12.  Waves that walk several pieces, the next one's loads in flight, took 22.
 template <int PER>
 __global__ __launch_bounds__(256) void k_beam_pieces(BeamSelect b, BeamWs w, int pieces, uint32_t blocks) {
@@ -403,7 +403,7 @@ __device__ __forceinline__ int row16_sumi(int v) {
 // 24 kept (K rounds of a block-wide maximum took 120).
 constexpr int BS_LIST = 512, BS_PARTS = 4096, BS_WAVES = 16;
 constexpr int BS_GROUPS = 1 << 21;  // of a launch, which has fewer than 2^32 threads
-constexpr int BS_HELD = 5;  // of a thread's quarters, maxima that wait in registers (5120: 12 rows of 50280 logits)
+constexpr int BS_HELD = 5;  // of a thread's quarters, maxima that wait in registers (5120: 12 rows of 50280 logits); later ones are read anew
 template <int PER>
 __global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect b, BeamWs w, int pieces, int first) {
   __shared__ double lse[1024], had[1024], scale[1024];  // of the group's rows; lse NaN: ended

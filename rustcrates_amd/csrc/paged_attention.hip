@@ -315,9 +315,11 @@ __device__ __forceinline__ void paged_split(const PagedAttn& a, const PagedPlan&
 // order the matrix cores take it, among the first products of the current one
 // and leaves it in LDS after the last.  The queries wait in registers.  A wave
 // whose rows lie before a tile leaves its products out.  Bound by a wave's waits between
-// its MFMAs (31% of its time: LDS reads, the barrier a tile, loads), which two waves a
-// SIMD hide in part: 193 to 700 rows behind 774 to 1024 slots, 12 heads of 64, 219 us
-// of which the matrix cores are busy for 112.
+// its MFMAs (33% of its time: LDS reads, the barrier a tile, loads), which two waves a
+// SIMD hide in part.  Three sequences of 12 heads of 64, inputs changing from call to
+// call: 193 to 700 rows behind 774 to 1024 slots 237 us, of which the matrix cores are
+// busy for 112 (219 us where the inputs stay); 392 to 700 behind 568 to 1024 302 us, 145
+// busy.
 template <int DHP>
 constexpr size_t tile_lds() {  // keys [U] and values [4][CT] in 1 KB fragments, twice; then outputs [64][DHP + 1]
   return std::max(2 * (size_t)(DHP / 2) * 64 * sizeof(double2), (size_t)64 * (DHP + 1) * sizeof(double2));
@@ -460,10 +462,12 @@ __device__ __forceinline__ void paged_tile(const PagedAttn& a, const PagedPlan& 
 // shared is read off the tables, whatever the caller took them for: a run of
 // sequences holds in common the pages up to the first in which a neighbour differs.
 // 32 prompts of 4 beams, 200 to 248 slots of which 128 are shared, 8 heads: the 256
-// blocks take the longest bunch's time, and eight waves each, two a SIMD, 74 us a call
-// against 82 with four; 512 blocks of single sequences' pieces and more read 470 MB
-// instead of 275 and take longer than either.  More blocks than CUs stand two on a CU
-// with four waves: 64 prompts of 8 beams 217 us a call, 228 with eight waves.
+// blocks take the longest bunch's time, 67 us (4.1 TB/s of the 275 MB that have to be
+// read), with eight waves each, two a SIMD; a call 85 us against 89 with four waves
+// where the inputs change from call to call, 74 against 82 where they stay.  512 blocks of
+// single sequences' pieces and more read 470 MB and take longer than either.  More
+// blocks than CUs stand two on a CU with four waves: 64 prompts of 8 beams 258 us a call,
+// 253 with eight waves, where the inputs change, 216 and 226 where they stay.
 struct BeamRuns {  // in LDS
   int4 at[32];     // tiles [x, y) of all from tile z of sequence w & 15 for columns w >> 8
   int n;
@@ -727,8 +731,9 @@ __global__ __launch_bounds__(256) void k_paged_join(PagedAttn a, PagedPlan p, Pa
 // place of the chip is busy; 8 us go to a block's start and end, and the partials
 // pass through memory twice.  Other widths go by the same figures in proportion.
 // With more rows a block takes as many steps as any other, of as many groups as that
-// needs: 700 rows behind 512 to 1024 slots, 12 heads, take 280 us a call in
-// blocks of 14 steps at most, 252 in 504 blocks of equal steps.
+// needs: up to 700 rows of three sequences behind 555 to 1024 slots, 12 heads, take 352 us
+// a call in blocks of 14 steps at most, 291 in 504 blocks of equal steps (inputs changing
+// from call to call).
 PagedPlan paged_plan(const PagedAttn& a, const int* kv_len, const int* count, std::vector<int>& lists) {
   PagedPlan p;
   p.ng = a.n <= 16 || a.dh > 128 ? 1 : a.n <= 32 ? 2 : 4;
