@@ -408,7 +408,8 @@ template <int PER>
 __global__ __launch_bounds__(1024) void k_beam_pick(BeamSelect b, BeamWs w, int pieces, int first) {
   __shared__ double lse[1024], had[1024], scale[1024];  // of the group's rows; lse NaN: ended
   __shared__ Cont part[BS_WAVES], list[BS_LIST];
-  __shared__ int plist[BS_PARTS], bins[BB_BINS];
+  __shared__ int plist[BS_PARTS];
+  __shared__ __align__(16) int bins[BB_BINS];  // read by fours
   __shared__ double lows[BS_WAVES], highs[BS_WAVES];
   __shared__ int sums[BS_WAVES], nparts, listed;
   const int g = first + blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = b.beams, K = b.keep;
